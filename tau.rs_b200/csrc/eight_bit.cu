@@ -1,0 +1,422 @@
+// Weights, activations and caches held in 8 bits (e4m3): quantising, the plain product over such operands, the store into cache pages
+// and the pages read back.  The rule of scales is in eight_bit.cuh.
+//
+// The reference keeps weights and caches in 16 and 32 bits (crates/models/src/components/gated_attention/kv_cache.rs:12-24); this is
+// the library's own.
+#include "eight_bit.cuh"
+
+namespace {
+
+template <typename T> struct alignas(sizeof(T) * 4) Four { T v[4]; };
+
+// ---- quantising ---------------------------------------------------------------------------------------------------------------------
+// One block to 128 x 128 values of a weight; a thread holds 64 of them between the maximum and the codes, so the weight is read once.
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_blocks_kernel(const T* __restrict__ values, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows, int columns) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    __shared__ float greatest_of[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row0 = blockIdx.y * kScaleBlock, column = blockIdx.x * kScaleBlock + lane * 4;
+    float held[16][4];
+    float greatest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = row0 + warp + 8 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            held[i][j] = (row < rows && column + j < columns) ? to_float(values[static_cast<size_t>(row) * stride + column + j]) : 0.0f;
+            greatest = fmaxf(greatest, finite_magnitude(held[i][j]));
+        }
+    }
+    greatest = warp_max(greatest);
+    if (lane == 0) greatest_of[warp] = greatest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) greatest = fmaxf(greatest, greatest_of[w]);
+    const int exponent = scale_exponent(greatest);
+    const float inverse = power_of_two(-exponent);
+    if (threadIdx.x == 0) scales[static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x] = power_of_two(exponent);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = row0 + warp + 8 * i;
+        if (row >= rows || column >= columns) continue;      // columns are a multiple of 16: a group of four is whole or absent
+        *reinterpret_cast<unsigned*>(codes + static_cast<size_t>(row) * columns + column) = encode_four(held[i][0], held[i][1], held[i][2], held[i][3], inverse);
+    }
+}
+
+// A warp to 128 columns of a row.  scales[block of columns][row].
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_rows_kernel(const T* __restrict__ values, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows, int columns, int across) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (item >= static_cast<long long>(rows) * across) return;
+    const int row = static_cast<int>(item / across), block = static_cast<int>(item % across);
+    const int column = block * kScaleBlock + lane * 4;
+    Four<T> held = {};
+    const bool live = column < columns;
+    if (live) held = *reinterpret_cast<const Four<T>*>(values + static_cast<size_t>(row) * stride + column);
+    float greatest = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) greatest = fmaxf(greatest, live ? finite_magnitude(to_float(held.v[j])) : 0.0f);
+    const int exponent = scale_exponent(warp_max(greatest));
+    if (lane == 0) scales[static_cast<size_t>(block) * rows + row] = power_of_two(exponent);
+    if (live)
+        *reinterpret_cast<unsigned*>(codes + static_cast<size_t>(row) * columns + column) =
+            encode_four(to_float(held.v[0]), to_float(held.v[1]), to_float(held.v[2]), to_float(held.v[3]), power_of_two(-exponent));
+}
+
+// ---- the plain product ----------------------------------------------------------------------------------------------------------------
+// 32 rows x 32 features to a block of 256 threads, four results to a thread; 32 columns at a time in shared memory, decoded.  The sum
+// over a block of 128 columns is kept apart and joins times both scales.  The kernel that the fast ones are checked against.
+template <typename TOut>
+__global__ void __launch_bounds__(256)
+gemm8_simt_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scales, const uint8_t* __restrict__ w, const float* __restrict__ w_scales,
+                  const float* __restrict__ bias, TOut* __restrict__ out, int M, int N, int K, long long out_stride) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    __shared__ float x_tile[32][33], w_tile[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int feature = blockIdx.x * 32 + tx, across = (K + kScaleBlock - 1) / kScaleBlock;
+    const int row0 = blockIdx.y * 32;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < K; k0 += 32) {
+        __syncthreads();
+        {   // 32 x 8 words of four codes from each operand, one to a thread
+            const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+            float values[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (row0 + r < M && k0 + c < K) decode_four(*reinterpret_cast<const unsigned*>(x + static_cast<size_t>(row0 + r) * K + k0 + c), values);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x_tile[r][c + j] = values[j];
+            float weights[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (static_cast<int>(blockIdx.x) * 32 + r < N && k0 + c < K)
+                decode_four(*reinterpret_cast<const unsigned*>(w + static_cast<size_t>(blockIdx.x * 32 + r) * K + k0 + c), weights);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w_tile[r][c + j] = weights[j];
+        }
+        __syncthreads();
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) {
+            const float weight = w_tile[tx][k];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[i] = fmaf(x_tile[ty + 8 * i][k], weight, part[i]);
+        }
+        if ((k0 + 32) % kScaleBlock == 0 || k0 + 32 >= K) {
+            const int block = k0 / kScaleBlock;
+            const float w_scale = feature < N ? w_scales[static_cast<size_t>(feature / kScaleBlock) * across + block] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = row0 + ty + 8 * i;
+                if (row < M) sum[i] = fmaf(part[i], x_scales[static_cast<size_t>(block) * M + row] * w_scale, sum[i]);
+                part[i] = 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = row0 + ty + 8 * i;
+        if (row < M && feature < N) out[static_cast<size_t>(row) * out_stride + feature] = from_float<TOut>(sum[i] + (bias ? bias[feature] : 0.0f));
+    }
+}
+
+// What a gated product makes of the rows that an ungated one left: groups of 8 gate columns and their 8 up columns.
+__global__ void gate_groups_kernel(const bf16* __restrict__ stacked, bf16* __restrict__ out, long long count, int inner, long long out_stride, float limit) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const long long index = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (index >= count) return;
+    const long long row = index / inner;
+    const int column = static_cast<int>(index % inner);
+    const bf16* source = stacked + row * 2 * inner + (column >> 3) * 16 + (column & 7);
+    out[row * out_stride + column] = __float2bfloat16_rn(gated_value(to_float(source[0]), to_float(source[8]), limit));
+}
+
+// ---- the cache ------------------------------------------------------------------------------------------------------------------------
+constexpr int kPage = 64;
+
+// How keys, values and queries of new tokens come: as they are to be kept (`prepared` false), or as a stacked projection left them: then
+// queries and keys are normalised per head (rounded to bfloat16), rotated in 32 bits (rounded again), and queries written out.
+struct StoreSource {
+    const bf16* keys;             // head h of token i at keys + i * key_stride + h * D
+    const bf16* values;
+    long long key_stride, value_stride;
+    const bf16* query_rows;       // or nullptr: no queries
+    long long query_stride;
+    bf16* queries;                // [tokens, n_heads * D]
+    const float* q_weight;        // or nullptr: no norm
+    const float* k_weight;
+    float eps;
+    const float* cos_table;       // [positions, rotary_dim / 2]
+    const float* sin_table;
+    int rotary_dim;
+    int n_heads;
+};
+constexpr int kQueryHeads = 4;      // query heads to a block
+
+// One warp: norm and rotation of one head into `row` (shared memory).
+__device__ __forceinline__ void prepare_row(const bf16* __restrict__ source, const float* __restrict__ weight, float eps, const float* __restrict__ cosines,
+                                            const float* __restrict__ sines, int rotary_dim, int D, bf16* row, int lane) {
+    float inverse = 1.0f;
+    if (weight) {
+        float squares = 0.0f;
+        for (int e = lane; e < D; e += 32) {
+            const float value = to_float(source[e]);
+            squares += value * value;
+        }
+        inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + eps);
+    }
+    for (int e = lane; e < D; e += 32) row[e] = weight ? __float2bfloat16_rn(to_float(source[e]) * inverse * weight[e]) : source[e];
+    __syncwarp();
+    const int half = rotary_dim / 2;
+    for (int j = lane; j < half; j += 32) {      // a pair is one lane's
+        const float first = to_float(row[j]), second = to_float(row[j + half]), c = cosines[j], s = sines[j];
+        row[j] = __float2bfloat16_rn(first * c - second * s);
+        row[j + half] = __float2bfloat16_rn(second * c + first * s);
+    }
+    __syncwarp();
+}
+
+// grid (pages touched, key heads + value heads + groups of query heads).  A block serves the new tokens of one sequence in one page: it
+// alone reads and writes that page of that head, so a scale that has to grow and the older codes that are rounded to it need no meeting.
+__global__ void __launch_bounds__(256)
+store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __restrict__ value_pages, float* __restrict__ key_scales, float* __restrict__ value_scales,
+             const int* __restrict__ cu_seqlens, const int* __restrict__ seq_start, const int* __restrict__ page_rows, int page_stride, int n_seqs, int n_kv_heads, int D, int most) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    extern __shared__ __align__(16) bf16 staged[];      // [tokens here][D]; queries: [warp][D]
+    __shared__ float greatest_of[8];
+    __shared__ int found[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // Which sequence and page: the first warp adds up the pages that 32 sequences at a time touch.
+    if (warp == 0) {
+        int before = 0, seq = -1, page = 0, start = 0, first = 0, count = 0;
+        const int item = blockIdx.x;
+        for (int base = 0; base < n_seqs; base += 32) {
+            const int s = base + lane;
+            int s_first = 0, s_count = 0, s_start = 0, touched = 0;
+            if (s < n_seqs) {
+                s_first = cu_seqlens[s];
+                s_count = cu_seqlens[s + 1] - s_first;
+                s_start = seq_start[s];
+                touched = s_count > 0 ? (s_start + s_count - 1) / kPage - s_start / kPage + 1 : 0;
+            }
+            int through = touched;
+#pragma unroll
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, through, offset);
+                if (lane >= offset) through += other;
+            }
+            const bool mine = item >= before + through - touched && item < before + through;
+            const unsigned who = __ballot_sync(0xffffffffu, mine);
+            if (who != 0u) {
+                const int owner = __ffs(who) - 1;
+                seq = base + owner;
+                start = __shfl_sync(0xffffffffu, s_start, owner);
+                first = __shfl_sync(0xffffffffu, s_first, owner);
+                count = __shfl_sync(0xffffffffu, s_count, owner);
+                page = start / kPage + item - before - __shfl_sync(0xffffffffu, through - touched, owner);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, through, 31);
+        }
+        if (lane == 0) {
+            const int low = max(start, page * kPage), high = min(start + count, (page + 1) * kPage);
+            found[0] = seq;
+            found[1] = first + low - start;      // first packed row
+            found[2] = low;
+            found[3] = min(high - low, most);      // what the staging holds
+        }
+    }
+    __syncthreads();
+    const int seq = found[0], row0 = found[1], position0 = found[2], count = found[3];
+    if (seq < 0) return;      // the host counts pages from above
+    const int half = source.rotary_dim / 2;
+    if (static_cast<int>(blockIdx.y) >= 2 * n_kv_heads) {      // queries
+        const int head0 = (blockIdx.y - 2 * n_kv_heads) * kQueryHeads, heads = min(kQueryHeads, source.n_heads - head0);
+        bf16* row = staged + warp * D;
+        for (int task = warp; task < count * heads; task += 8) {
+            const int token = task / heads, head = head0 + task % heads;
+            const size_t table = static_cast<size_t>(position0 + token) * half;
+            prepare_row(source.query_rows + static_cast<size_t>(row0 + token) * source.query_stride + static_cast<size_t>(head) * D, source.q_weight, source.eps,
+                        source.cos_table + table, source.sin_table + table, source.rotary_dim, D, row, lane);
+            bf16* target = source.queries + (static_cast<size_t>(row0 + token) * source.n_heads + head) * D;
+            for (int e = lane; e < D; e += 32) target[e] = row[e];
+            __syncwarp();
+        }
+        return;
+    }
+    const bool is_key = static_cast<int>(blockIdx.y) < n_kv_heads;
+    const int head = is_key ? blockIdx.y : blockIdx.y - n_kv_heads;
+    const size_t place = static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + position0 / kPage]) * n_kv_heads + head;
+    uint8_t* page = (is_key ? key_pages : value_pages) + place * kPage * D;
+    float* scale_at = (is_key ? key_scales : value_scales) + place;
+    const int older = position0 % kPage;
+    float greatest = 0.0f;
+    for (int token = warp; token < count; token += 8) {
+        bf16* row = staged + token * D;
+        const bf16* from = is_key ? source.keys + static_cast<size_t>(row0 + token) * source.key_stride + static_cast<size_t>(head) * D
+                                  : source.values + static_cast<size_t>(row0 + token) * source.value_stride + static_cast<size_t>(head) * D;
+        const size_t table = static_cast<size_t>(position0 + token) * half;
+        prepare_row(from, is_key ? source.k_weight : nullptr, source.eps, source.cos_table + table, source.sin_table + table, is_key ? source.rotary_dim : 0, D, row, lane);
+        for (int e = lane; e < D; e += 32) greatest = fmaxf(greatest, finite_magnitude(to_float(row[e])));
+    }
+    greatest = warp_max(greatest);
+    if (lane == 0) greatest_of[warp] = greatest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) greatest = fmaxf(greatest, greatest_of[w]);
+    float scale = power_of_two(scale_exponent(greatest));
+    if (older > 0) {      // the page holds positions of this sequence: its scale counts, and grows where the new ones need it
+        const float kept = fmaxf(*scale_at, kLeastScale);
+        if (kept >= scale) {
+            scale = kept;
+        } else {
+            const float ratio = kept / scale;      // powers of two
+            for (int piece = threadIdx.x; piece < older * D / 4; piece += 256) {
+                unsigned* word = reinterpret_cast<unsigned*>(page) + piece;
+                float v[4];
+                decode_four(*word, v);
+                *word = encode_four(v[0], v[1], v[2], v[3], ratio);
+            }
+        }
+    }
+    const float inverse = 1.0f / scale;
+    for (int piece = threadIdx.x; piece < count * D / 8; piece += 256) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(staged + piece * 8);
+        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint2 codes;
+        codes.x = encode_four(__uint_as_float(words[0] << 16), __uint_as_float(words[0] & 0xffff0000u), __uint_as_float(words[1] << 16), __uint_as_float(words[1] & 0xffff0000u), inverse);
+        codes.y = encode_four(__uint_as_float(words[2] << 16), __uint_as_float(words[2] & 0xffff0000u), __uint_as_float(words[3] << 16), __uint_as_float(words[3] & 0xffff0000u), inverse);
+        *reinterpret_cast<uint2*>(page + static_cast<size_t>(older) * D + piece * 8) = codes;
+    }
+    __syncthreads();      // every thread has read the old scale
+    if (threadIdx.x == 0) *scale_at = scale;
+}
+
+// Pages of the step's sequences as the bfloat16 values that they stand for (exact: 4 significant bits times a power of two).
+// grid (page of a sequence, sequence, 2 n_kv_heads).  Positions that a sequence does not have are zeros; with `sparse` only pages that a query sees
+// are written at all, and positions that none sees are zeros: what a window left behind may be NaN, and a weight of zero would not hide that.
+__global__ void __launch_bounds__(256)
+read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
+            bf16* __restrict__ keys, bf16* __restrict__ values, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
+            int page_stride, int n_kv_heads, int D, int window, int sparse) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int page = blockIdx.x, seq = blockIdx.y;
+    const bool is_key = static_cast<int>(blockIdx.z) < n_kv_heads;
+    const int head = is_key ? blockIdx.z : blockIdx.z - n_kv_heads;
+    const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
+    const int first = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) - page * kPage : 0;      // the first position of this page that a query sees
+    if (sparse && (live <= 0 || first >= kPage)) return;
+    const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * n_kv_heads + head : 0;
+    const uint8_t* codes = (is_key ? key_pages : value_pages) + place * kPage * D;
+    const float scale = live > 0 ? (is_key ? key_scales : value_scales)[place] : 0.0f;
+    bf16* target = (is_key ? keys : values) + ((static_cast<size_t>(seq) * page_stride + page) * n_kv_heads + head) * kPage * D;
+    for (int piece = threadIdx.x; piece < kPage * D / 16; piece += 256) {
+        const bool held = piece * 16 < live * D && piece * 16 >= first * D;
+        const uint4 raw = held ? __ldg(reinterpret_cast<const uint4*>(codes) + piece) : make_uint4(0u, 0u, 0u, 0u);
+        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint4 wide[2];
+        unsigned* out = reinterpret_cast<unsigned*>(wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[4];
+            decode_four(words[i], v);
+            out[2 * i] = pack_bf16_pair(v[0] * scale, v[1] * scale);
+            out[2 * i + 1] = pack_bf16_pair(v[2] * scale, v[3] * scale);
+        }
+        reinterpret_cast<uint4*>(target)[2 * piece] = wide[0];
+        reinterpret_cast<uint4*>(target)[2 * piece + 1] = wide[1];
+    }
+}
+
+}  // namespace
+
+// Codes [rows, columns] (contiguous) and scales [blocks of rows, blocks of columns] of a matrix whose columns are a multiple of 16.
+TAU_EXPORT int tau_quantize_blocks(int dtype, const void* values, long long stride, void* codes, float* scales, int rows, int columns, void* stream) {
+    if (rows <= 0 || columns <= 0) return 0;
+    if (!values || !codes || !scales || (columns & 15) || (dtype != TAU_BF16 && dtype != TAU_F32) || (rows + kScaleBlock - 1) / kScaleBlock > 65535) return cudaErrorInvalidValue;
+    const dim3 grid((columns + kScaleBlock - 1) / kScaleBlock, (rows + kScaleBlock - 1) / kScaleBlock);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == TAU_BF16)
+        tau_launch(quantize_blocks_kernel<bf16>, grid, dim3(256), 0, s, static_cast<const bf16*>(values), stride, static_cast<uint8_t*>(codes), scales, rows, columns);
+    else
+        tau_launch(quantize_blocks_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(values), stride, static_cast<uint8_t*>(codes), scales, rows, columns);
+    return tau_launch_status();
+}
+
+// Codes [rows, columns] (contiguous) and scales [blocks of columns, rows]; columns a multiple of 16, rows of values on 16-byte borders.
+TAU_EXPORT int tau_quantize_rows(int dtype, const void* values, long long stride, void* codes, float* scales, int rows, int columns, void* stream) {
+    if (rows <= 0 || columns <= 0) return 0;
+    const int across = (columns + kScaleBlock - 1) / kScaleBlock;
+    const long long blocks = (static_cast<long long>(rows) * across + 7) / 8;
+    if (!values || !codes || !scales || (columns & 15) || (stride & 7) || (reinterpret_cast<uintptr_t>(values) & 15) || (dtype != TAU_BF16 && dtype != TAU_F32) || blocks > 0x7fffffffll)
+        return cudaErrorInvalidValue;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == TAU_BF16)
+        tau_launch(quantize_rows_kernel<bf16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, static_cast<const bf16*>(values), stride, static_cast<uint8_t*>(codes), scales, rows, columns, across);
+    else
+        tau_launch(quantize_rows_kernel<float>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, static_cast<const float*>(values), stride, static_cast<uint8_t*>(codes), scales, rows, columns, across);
+    return tau_launch_status();
+}
+
+// x codes [M, K] with scales [blocks, M]; w codes [N, K] with scales [blocks of N, blocks]; both contiguous, K a multiple of 16.
+TAU_EXPORT int tau_gemm8_simt(int out_dtype, const void* x, const float* x_scales, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K,
+                              long long out_stride, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!x || !x_scales || !w || !w_scales || !out || K <= 0 || (K & 15) || (out_dtype != TAU_BF16 && out_dtype != TAU_F32)) return cudaErrorInvalidValue;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (M > 65535 * 32) return cudaErrorInvalidValue;
+    const dim3 grid((N + 31) / 32, (M + 31) / 32);
+    if (out_dtype == TAU_BF16)
+        tau_launch(gemm8_simt_kernel<bf16>, grid, dim3(256), 0, s, static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(w), w_scales, bias, static_cast<bf16*>(out), M, N, K, out_stride);
+    else
+        tau_launch(gemm8_simt_kernel<float>, grid, dim3(256), 0, s, static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(w), w_scales, bias, static_cast<float*>(out), M, N, K, out_stride);
+    return tau_launch_status();
+}
+
+TAU_EXPORT int tau_gate_groups(const void* stacked, void* out, long long rows, int inner, long long out_stride, float limit, void* stream) {
+    if (rows <= 0 || inner <= 0) return 0;
+    if (!stacked || !out || (inner & 7) || (rows * inner + 255) / 256 > 0x7fffffffll) return cudaErrorInvalidValue;
+    tau_launch(gate_groups_kernel, dim3(static_cast<unsigned>((rows * inner + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const bf16*>(stacked),
+               static_cast<bf16*>(out), rows * inner, inner, out_stride, limit);
+    return tau_launch_status();
+}
+
+// Stores the keys and values of `tokens` new tokens; with `query_rows` the queries are prepared beside them.  `cos_table` == nullptr needs rotary_dim 0.
+TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const void* values, long long value_stride, void* key_pages, void* value_pages, float* key_scales,
+                                float* value_scales, const int* cu_seqlens, const int* seq_start, const int* page_rows, int page_stride, int n_seqs, int tokens, int single,
+                                int n_kv_heads, int D, const void* query_rows, long long query_stride, void* queries, int n_heads, const float* q_weight, const float* k_weight,
+                                float eps, const float* cos_table, const float* sin_table, int rotary_dim, void* stream) {
+    if (tokens <= 0 || n_seqs <= 0) return 0;
+    if (!keys || !values || !key_pages || !value_pages || !key_scales || !value_scales || !cu_seqlens || !seq_start || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 ||
+        D > 256 || (D & 15) || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) || (rotary_dim > 0 && (!cos_table || !sin_table)) || (query_rows && (!queries || n_heads <= 0)))
+        return cudaErrorInvalidValue;
+    const StoreSource source = {static_cast<const bf16*>(keys), static_cast<const bf16*>(values), key_stride, value_stride, static_cast<const bf16*>(query_rows), query_stride,
+                                static_cast<bf16*>(queries), q_weight, k_weight, eps, cos_table, sin_table, rotary_dim, n_heads};
+    // A run of n tokens touches at most (n + 62) / 64 + 1 pages, and no more pages than it has tokens.
+    const long long bound = static_cast<long long>(tokens) / kPage + 2ll * n_seqs;
+    const unsigned items = single ? static_cast<unsigned>(n_seqs) : static_cast<unsigned>(bound < tokens ? bound : tokens);
+    const unsigned parts = 2u * n_kv_heads + (query_rows ? (n_heads + kQueryHeads - 1) / kQueryHeads : 0);
+    if (parts > 65535u) return cudaErrorInvalidValue;
+    const int rows = single ? 8 : kPage;      // staged rows; queries stage one for each of 8 warps
+    tau_launch(store_kernel, dim3(items, parts), dim3(256), static_cast<size_t>(rows) * D * sizeof(bf16), static_cast<cudaStream_t>(stream), source, static_cast<uint8_t*>(key_pages),
+               static_cast<uint8_t*>(value_pages), key_scales, value_scales, cu_seqlens, seq_start, page_rows, page_stride, n_seqs, n_kv_heads, D, rows);
+    return tau_launch_status();
+}
+
+TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* keys, void* values, const int* seq_start,
+                               const int* seq_len, const int* page_rows, int page_stride, int n_seqs, int n_kv_heads, int D, int window, int sparse, void* stream) {
+    if (n_seqs <= 0) return 0;
+    if (!key_pages || !value_pages || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
+        (D & 15) || n_seqs > 65535 || 2 * n_kv_heads > 65535)
+        return cudaErrorInvalidValue;
+    tau_launch(read_kernel, dim3(page_stride, n_seqs, 2 * n_kv_heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
+               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), seq_start, seq_len, page_rows, page_stride, n_kv_heads, D,
+               window, sparse);
+    return tau_launch_status();
+}

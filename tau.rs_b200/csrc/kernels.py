@@ -88,6 +88,7 @@ _CLASS_OF = {
     "side_gate": "activation", "unit_add_mix": "norm", "norm_rows": "norm", "relu_squared": "activation",
     "short_conv": "recurrence", "delta_prepare": "recurrence", "delta_rule": "recurrence", "selective_scan": "recurrence",
     "masked_prepare": "attention", "masked_attention": "attention", "talking_decode": "attention", "shared_key_decode": "attention", "gated_rows": "attention",
+    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gate_groups": "activation", "cache8_store": "attention", "cache8_read": "attention",
     "token_shift": "recurrence", "tanh": "activation", "channel_decay": "recurrence", "wkv": "recurrence", "forget_gates": "recurrence", "turn_heads": "recurrence",
 }
 _timing = None     # while timing: [last event, [(class, event after the launch), ...]]
@@ -1007,6 +1008,192 @@ def attention(queries, keys, values, out, step, page_rows, n_heads: int, n_kv_he
             return attention_tiled(*shapes)
         return attention_f32_tc(*shapes, ranges=-1 if step.n_seqs * step.max_len <= 2 * queries.shape[0] else 0)      # tiles of mostly new positions see very different numbers of keys
     attention_generic(queries, keys, values, out, step.positions, step.token_seq, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
+
+
+# ---------------------------------------------------------------------------- weights and caches in 8 bits
+# Held as e4m3 codes with 32-bit scales (csrc/eight_bit.cuh has the rule): a scale for each 128 x 128 of a weight, for each row and 128 columns of
+# activations, for each page of 64 positions and head of a cache.
+SCALE_BLOCK = 128
+CODE_DTYPE = torch.float8_e4m3fn
+
+
+def _here(*tensors) -> None:
+    """`_on_device` for kernels that also refuse tensors of another device than the current one, whose stream they are launched on."""
+    _on_device(*tensors)
+    current = torch.cuda.current_device()
+    for tensor in tensors:
+        _require(tensor is None or tensor.device.index == current, "tensors must lie on the current CUDA device")
+
+
+def _scale_blocks(count: int) -> int:
+    return -(-count // SCALE_BLOCK)
+
+
+def linear8_fits(in_features: int, out_features: int, dtype, gated: bool = False) -> bool:
+    """Whether a product of these sizes can have its weight in 8 bits: bfloat16 runs, rows of whole 16 bytes, gated pairs in whole groups."""
+    return dtype == torch.bfloat16 and in_features > 0 and in_features % 16 == 0 and out_features > 0 and (not gated or out_features % GATE_GROUP == 0)
+
+
+def quantize_blocks(weight):
+    """A weight [out, in] (bfloat16 or float32, `in` a multiple of 16) as codes (float8_e4m3fn, the same shape) and scales (float32
+    [ceil(out / 128), ceil(in / 128)]): what `linear8` and `linear8_gated` read."""
+    _require(weight.dim() == 2 and weight.shape[1] % 16 == 0 and weight.stride(1) == 1, "a weight to be held in 8 bits must be [out, in] with `in` a multiple of 16")
+    _code(weight)
+    _here(weight)
+    rows, columns = weight.shape
+    codes = torch.empty((rows, columns), dtype=CODE_DTYPE, device=weight.device)
+    scales = torch.empty((_scale_blocks(rows), _scale_blocks(columns)), dtype=torch.float32, device=weight.device)
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_quantize_blocks(_code(weight), _pointer(weight), ctypes.c_longlong(weight.stride(0)), _pointer(codes), _pointer(scales), ctypes.c_int(rows),
+                                       ctypes.c_int(columns), _stream()), "quantize_blocks")
+    return codes, scales
+
+
+def quantize_rows(values):
+    """Activations [rows, columns] (bfloat16 or float32, rows on 16-byte borders, columns a multiple of 16) as codes and scales (float32
+    [ceil(columns / 128), rows])."""
+    _require(values.dim() == 2 and values.shape[1] % 16 == 0 and values.stride(1) == 1 and values.stride(0) % 8 == 0 and values.data_ptr() % 16 == 0,
+             "activations must be [rows, columns] with columns a multiple of 16 and rows on 16-byte borders")
+    _code(values)
+    _here(values)
+    rows, columns = values.shape
+    codes = torch.empty((rows, columns), dtype=CODE_DTYPE, device=values.device)
+    scales = torch.empty((_scale_blocks(columns), rows), dtype=torch.float32, device=values.device)
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_quantize_rows(_code(values), _pointer(values), ctypes.c_longlong(values.stride(0)), _pointer(codes), _pointer(scales), ctypes.c_int(rows),
+                                     ctypes.c_int(columns), _stream()), "quantize_rows")
+    return codes, scales
+
+
+def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
+    _require(values.dim() == 2 and codes.dim() == 2 and values.shape[1] == codes.shape[1], "shapes must be [M,K] x [N,K] -> [M,N]")
+    rows, depth = values.shape
+    features = codes.shape[0]
+    _require(codes.dtype == CODE_DTYPE and codes.is_contiguous() and codes.data_ptr() % 16 == 0, "the weight must be contiguous float8_e4m3fn codes on a 16-byte border")
+    _require(depth > 0 and depth % 16 == 0, "the depth must be a multiple of 16")
+    _require(scales.dtype == torch.float32 and scales.shape == (_scale_blocks(features), _scale_blocks(depth)) and scales.is_contiguous(),
+             "the weight's scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)]")
+    _require(values.dtype in (torch.bfloat16, torch.float32) and values.stride(1) == 1 and values.stride(0) % 8 == 0 and values.data_ptr() % 16 == 0,
+             "activations must be bfloat16 or float32 with rows on 16-byte borders")
+    _require(out.shape == (rows, features // 2 if gated else features) and (out.stride(1) == 1 or out.shape[1] == 1) and (rows < 2 or out.stride(0) >= out.shape[1]),
+             "the output must be [M, N], or [M, N / 2] of a gated product")
+    _require(out.dtype == torch.bfloat16 if gated else out.dtype in (torch.bfloat16, torch.float32), "the output must be bfloat16 (or float32 where nothing is gated)")
+    _require(not gated or features % (2 * GATE_GROUP) == 0, "a gated product needs a multiple of 16 weight rows")
+    _f32_vector(bias, features, "the bias")
+    _here(values, codes, scales, bias, out)
+
+
+def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
+    """The plain product of operands in 8 bits (`quantize_rows`, `quantize_blocks`), on the 32-bit pipes: every size, the kernel that the others are checked against."""
+    rows, depth = x_codes.shape
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_gemm8_simt(_code(out), _pointer(x_codes), _pointer(x_scales), _pointer(codes), _pointer(scales), _pointer(bias), _pointer(out), ctypes.c_int(rows),
+                                  ctypes.c_int(codes.shape[0]), ctypes.c_int(depth), ctypes.c_longlong(out.stride(0)), _stream()), "gemm8_simt")
+
+
+def linear8(values, codes, scales, bias, out) -> None:
+    """`out = values @ weight.T + bias` with the weight in 8 bits (`quantize_blocks`) and the activations brought to 8 bits within the call, a scale for each
+    row and 128 columns; sums in 32 bits, one rounding to the output's type."""
+    _check_linear8(values, codes, scales, bias, out, False)
+    if values.shape[0] == 0 or codes.shape[0] == 0:
+        return
+    gemm8_simt(*quantize_rows(values), codes, scales, bias, out)
+
+
+def linear8_gated(values, codes, scales, out, limit: float = 0.0) -> None:
+    """`out = silu(values @ gate.T) * (values @ up.T)` with the stacked weight (groups of 8 gate rows followed by their 8 up rows) in 8 bits; `limit` > 0: the
+    clamped form of `silu_mul`.  Gate and up values are rounded to bfloat16 as a product that is not gated would store them."""
+    _check_linear8(values, codes, scales, None, out, True)
+    rows, features = values.shape[0], codes.shape[0]
+    if rows == 0 or features == 0:
+        return
+    stacked = torch.empty((rows, features), dtype=torch.bfloat16, device=values.device)
+    gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_gate_groups(_pointer(stacked), _pointer(out), ctypes.c_longlong(rows), ctypes.c_int(features // 2), ctypes.c_longlong(out.stride(0)),
+                                   ctypes.c_float(limit), _stream()), "gate_groups")
+
+
+def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows) -> None:
+    _require(key_pages.dtype == CODE_DTYPE == value_pages.dtype and key_pages.dim() == 4 and key_pages.shape[2] == PAGE_TOKENS and key_pages.shape == value_pages.shape
+             and key_pages.is_contiguous() and value_pages.is_contiguous() and key_pages.data_ptr() % 16 == 0 and value_pages.data_ptr() % 16 == 0,
+             "cache pages must be float8_e4m3fn [pages, n_kv_heads, 64, head_dim]")
+    _require(key_pages.shape[3] % 16 == 0 and 16 <= key_pages.shape[3] <= 256, "head_dim must be a multiple of 16 between 16 and 256")
+    for scales in (key_scales, value_scales):
+        _require(scales.dtype == torch.float32 and scales.shape == key_pages.shape[:2] and scales.is_contiguous(), "the pages' scales must be float32 [pages, n_kv_heads]")
+    _require(page_rows.dtype == torch.int32 and page_rows.dim() == 2 and page_rows.is_contiguous() and page_rows.shape[0] == step.n_seqs, "page rows must be int32 [sequences, stride]")
+    for what, tensor, count in (("cu_seqlens", step.cu_seqlens, step.n_seqs + 1), ("seq_start", step.seq_start, step.n_seqs), ("seq_len", step.seq_len, step.n_seqs)):
+        _int_vector(tensor, what)
+        _require(tensor.numel() == count, f"{what} must have {count} elements")
+
+
+def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales, step, page_rows, prepare=None) -> None:
+    """Keys and values of the step's new tokens (bfloat16 [tokens, n_kv_heads, head_dim], tokens any distance apart) enter the pages of their sequences.
+
+    A page's scale of a head covers the positions that it holds: it is chosen anew with a page's first position and grows where later ones need it; the codes that are
+    there are then rounded to the new one.  `prepare` = (projected, queries, q_weight, k_weight, eps, cos, sin, rotary_dim, n_heads): keys are normalised per head and
+    rotated first, and so are the queries in `projected` [tokens, n_heads * head_dim or more], which land in `queries`."""
+    _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
+    n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
+    for tensor in (keys, values):
+        _require(tensor.dtype == torch.bfloat16 and tensor.shape == (step.n_tokens, n_kv_heads, head_dim) and tensor.stride(2) == 1 and (n_kv_heads == 1 or tensor.stride(1) == head_dim),
+                 "keys and values must be bfloat16 [tokens, n_kv_heads, head_dim], a token's heads one behind the other")
+    projected = queries = q_weight = k_weight = cos = sin = None
+    eps, rotary_dim, n_heads = 0.0, 0, 0
+    if prepare is not None:
+        projected, queries, q_weight, k_weight, eps, cos, sin, rotary_dim, n_heads = prepare
+        _f32_vector(q_weight, head_dim, "the q norm weight")
+        _f32_vector(k_weight, head_dim, "the k norm weight")
+        _require(projected.dtype == torch.bfloat16 and projected.dim() == 2 and projected.shape[0] == step.n_tokens and projected.shape[1] >= n_heads * head_dim and projected.stride(1) == 1,
+                 "projected rows must hold every query head in bfloat16")
+        _require(queries.dtype == torch.bfloat16 and queries.shape == (step.n_tokens, n_heads * head_dim) and queries.is_contiguous(), "queries must be [tokens, n_heads * head_dim]")
+        if rotary_dim:
+            _require(rotary_dim % 2 == 0 and 0 < rotary_dim <= head_dim and cos is not None and sin is not None and cos.dtype == torch.float32 == sin.dtype and cos.shape == sin.shape
+                     and cos.shape[1] == rotary_dim // 2 and cos.is_contiguous() and sin.is_contiguous(), "rotation tables must be float32 [positions, rotary_dim / 2]")
+    _here(keys, values, key_pages, value_pages, key_scales, value_scales, step.cu_seqlens, step.seq_start, page_rows, projected, queries, q_weight, k_weight, cos, sin)
+    if step.n_tokens == 0:
+        return
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_cache8_store(
+        _pointer(keys), ctypes.c_longlong(keys.stride(0)), _pointer(values), ctypes.c_longlong(values.stride(0)), _pointer(key_pages), _pointer(value_pages), _pointer(key_scales),
+        _pointer(value_scales), _pointer(step.cu_seqlens), _pointer(step.seq_start), _pointer(page_rows), ctypes.c_int(page_rows.shape[1]), ctypes.c_int(step.n_seqs),
+        ctypes.c_int(step.n_tokens), ctypes.c_int(1 if step.all_single else 0), ctypes.c_int(n_kv_heads), ctypes.c_int(head_dim), _pointer(projected),
+        ctypes.c_longlong(0 if projected is None else projected.stride(0)), _pointer(queries), ctypes.c_int(n_heads), _pointer(q_weight), _pointer(k_weight), ctypes.c_float(eps),
+        _pointer(cos), _pointer(sin), ctypes.c_int(rotary_dim), _stream()), "cache8_store")
+
+
+def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int = 0, sparse: bool = False):
+    """The pages of the step's sequences as the bfloat16 values that they stand for: keys and values [sequences * stride, n_kv_heads, 64, head_dim], page `j` of
+    sequence `i` at `i * stride + j`; zeros where a sequence has no position.  `sparse`: pages that no query of the step sees (behind the sequence's end, or wholly before
+    the `window` of its first new token) are left unwritten."""
+    _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
+    _here(key_pages, value_pages, key_scales, value_scales, step.seq_start, step.seq_len, page_rows)
+    n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
+    _require(step.n_seqs <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
+    shape = (step.n_seqs * page_rows.shape[1], n_kv_heads, PAGE_TOKENS, head_dim)
+    keys, values = (torch.empty(shape, dtype=torch.bfloat16, device=key_pages.device) for _ in range(2))
+    library = build.load_library("eight_bit.cu")
+    _check(library.tau_cache8_read(
+        _pointer(key_pages), _pointer(value_pages), _pointer(key_scales), _pointer(value_scales), _pointer(keys), _pointer(values), _pointer(step.seq_start), _pointer(step.seq_len),
+        _pointer(page_rows), ctypes.c_int(page_rows.shape[1]), ctypes.c_int(step.n_seqs), ctypes.c_int(n_kv_heads), ctypes.c_int(head_dim), ctypes.c_int(window),
+        ctypes.c_int(1 if sparse else 0), _stream()), "cache8_read")
+    return keys, values
+
+
+def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
+    """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
+    _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
+    _require(key_pages.shape[1] == n_kv_heads and key_pages.shape[3] == head_dim and n_kv_heads > 0 and n_heads % n_kv_heads == 0,
+             "the pages must be [pages, n_kv_heads, 64, head_dim] and n_heads a multiple of n_kv_heads")
+    _require(queries.dtype == torch.bfloat16 == out.dtype and queries.shape == (step.n_tokens, n_heads * head_dim) and out.shape == queries.shape and queries.is_contiguous()
+             and out.is_contiguous(), "queries and output must be bfloat16 [tokens, n_heads * head_dim]")
+    _require(window >= 0, "a window must not be negative")
+    _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
+    if step.n_tokens == 0:
+        return
+    keys, values = cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, sparse=True)
+    places = torch.arange(keys.shape[0], dtype=torch.int32, device=keys.device).view(step.n_seqs, -1)
+    attention(queries, keys, values, out, step, places, n_heads, n_kv_heads, head_dim, scale, window)
 
 
 # ---------------------------------------------------------------------------- latent attention

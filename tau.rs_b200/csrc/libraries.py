@@ -13,6 +13,7 @@ def all_libraries() -> List[Tuple[str, Sequence[str]]]:
         ("gemm_f32_tc.cu", ()),
         ("attention_f32_tc.cu", ()),
         ("attention_generic.cu", ()),
+        ("eight_bit.cu", ()),
         ("sampling.cu", ()),
         ("random_init.cu", ()),
         ("stream32.cu", ()),
