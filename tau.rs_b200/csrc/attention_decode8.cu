@@ -1,0 +1,542 @@
+// Decode attention over pages held in 8 bits: one new token per sequence over its cached context, split along the context.
+//
+// Compiled for one head size (-DTAU_HEAD_DIM=...).  With codes c and a scale for each page (64 positions) and head,
+//     o = sum_j w_j s_V[page j] c_V[j] / sum_j w_j,   w_j = exp(scale * s_K[page j] * (q . c_K[j]) - max),
+// so a page's scales are factors outside its sums: the score's is multiplied into the softmax scale, the value's into the page's part of the
+// accumulator.  e4m3's numbers are numbers of 16-bit floats (the conversion is exact), so both products run on f16 operands with 32-bit sums:
+// queries are brought to [1, 2) per head by a power of two (exact for a bfloat16 within 2^-14 of the head's greatest element, and off by at most
+// 2^-25 of that below), weights are at most one and are rounded to 11 bits.
+//
+// What bounds it: 2 D bytes of codes for each cached position and key/value head, read once for the head's whole group of query heads.
+// A block serves up to 8 (or 16) query heads of one key/value head and a range of the sequence's pages; one warp asks for pages by TMA (a page of
+// a head is a box of 64 rows in 128-byte swizzled rows, several pages ahead), four warps take 16 positions each of every page.  Scores are
+// computed transposed (rows are keys, columns the group's query heads, mma.sync m16n8k16: with at most 16 columns there is nothing for
+// tcgen05's 128 rows to do), probabilities cross over by movmatrix, and values meet them as O^T = V^T P.  The order of elements inside a head is free
+// as long as both operands share it, so a lane's 16-byte load of a key serves four products.
+// Up to 8 ranges of a sequence form a cluster and are joined through shared memory, in the order of the ranges; more leave records for a second kernel.
+#include "tcgen05.cuh"
+#include "eight_bit.cuh"
+
+#ifndef TAU_HEAD_DIM
+#error "compile with -DTAU_HEAD_DIM=<multiple of 16 up to 256>"
+#endif
+
+namespace {
+
+constexpr int D = TAU_HEAD_DIM;
+static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head_dim must be a multiple of 16 between 16 and 256");
+constexpr int kPage = 64;
+constexpr int kWarps = 4;                         // consumers; one more asks for pages
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kHalves = (D + 127) / 128;          // boxes of 128 bytes to a row
+constexpr int kBoxBytes = kPage * 128;
+constexpr int kTileBytes = kHalves * kBoxBytes;   // a page of a head's keys, or of its values
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kStages = kHalves == 1 ? 4 : 3;
+constexpr int kKeySteps = D / 16;                 // products of 16 head elements
+constexpr int kMostClustered = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Shared {
+    uint64_t full[kStages];
+    uint64_t empty[kStages];
+    float key_scale[kStages], value_scale[kStages];
+    int abort_flag;
+};
+
+__device__ __forceinline__ void tma_load_3d(void* destination, const CUtensorMap* map, int x, int y, int z, uint64_t* barrier) {
+    if (operands_lost()) return;
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_address(destination)),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_address(barrier))
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack_half2(float low, float high) {
+    unsigned packed;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(packed) : "f"(high), "f"(low));
+    return packed;
+}
+
+// 16 bytes of a page in shared memory: chunk `chunk` of row `row` (of 128-byte rows whose chunks the copy permuted by the row's number).
+__device__ __forceinline__ uint4 page_chunk(const uint8_t* tile, int row, int chunk) {
+    return *reinterpret_cast<const uint4*>(tile + (chunk >> 3) * kBoxBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ unsigned page_word(const uint8_t* tile, int row, int byte) {
+    return *reinterpret_cast<const unsigned*>(tile + (byte >> 7) * kBoxBytes + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15));
+}
+
+// The element of a head that lane t holds as number `i` (0..3) of product `step`: whole groups of 64 elements give each lane 16 neighbours, what is left
+// behind them four for each 16 elements.
+__device__ __forceinline__ int key_element(int step, int t, int i) {
+    const int group = step >> 2;
+    return group < D / 64 ? group * 64 + t * 16 + (step & 3) * 4 + i : step * 16 + t * 4 + i;
+}
+
+constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a lane holds 16 columns, 8 tiles of 16 rows
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads)
+decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
+               const float* __restrict__ key_scales, const float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
+               const int* __restrict__ seq_len, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale, int window, int splits,
+               int clustered) {
+    grid_dependents_launch();
+    constexpr int kHeads = 8 * NT;
+    extern __shared__ uint8_t shared_raw[];
+    Shared* shared = reinterpret_cast<Shared*>(shared_raw);
+    uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + sizeof(Shared) + 1023) & ~uintptr_t(1023));
+    // Once every page has been read the stages hold what the warps bring to the join.
+    float (*merge_o)[kHeads][D] = reinterpret_cast<float (*)[kHeads][D]>(stages);
+    static_assert(kWarps * kHeads * D * 4 <= kStages * kStageBytes, "the join must fit the stages");
+    __shared__ float merge_ml[kWarps][kHeads][2];
+    __shared__ float block_ml[kHeads][2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x, seq = blockIdx.z;
+    const int kv_head = blockIdx.y / passes, pass = blockIdx.y % passes;
+    const int group = n_heads / n_kv_heads;
+    const int head0 = kv_head * group + pass * kHeads;
+    const int heads_here = min(kHeads, group - pass * kHeads);
+    volatile int* abort_flag = &shared->abort_flag;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            barrier_init(&shared->full[s], 1);
+            barrier_init(&shared->empty[s], kWarps);
+        }
+        shared->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    const int length = seq_len[seq];
+    const int first = (window > 0 && length > window) ? length - window : 0;
+    const int first_page = first / kPage, pages_end = (length + kPage - 1) / kPage;
+    const int per_split = (max(0, pages_end - first_page) + splits - 1) / splits;
+    const int page_lo = first_page + split * per_split, page_hi = min(pages_end, page_lo + per_split);
+    const int count = max(0, page_hi - page_lo);
+    float running_max[NT][2], running_sum[NT][2];
+    float acc[NT][kValueRounds][8][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        running_max[n][0] = running_max[n][1] = -INFINITY;
+        running_sum[n][0] = running_sum[n][1] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kValueRounds; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[n][r][i][j] = 0.0f;
+    }
+
+    if (warp == kWarps) {
+        // ---- the pages, in order: the numbers and scales of 32 at a time, a lane each
+        const int* pages = page_rows + static_cast<size_t>(seq) * page_stride;
+        bool alive = true;
+        int asked = 0;
+        for (int base = 0; base < count && alive; base += 32) {
+            const bool mine = base + lane < count;
+            const int place = mine ? pages[page_lo + base + lane] * n_kv_heads + kv_head : 0;
+            const float k_scale = mine ? key_scales[place] : 0.0f, v_scale = mine ? value_scales[place] : 0.0f;
+            for (int i = 0; i < min(32, count - base); ++i) {
+                const int number = base + i, stage = number % kStages;
+                const int box = __shfl_sync(0xffffffffu, place, i);
+                const float k_of = __shfl_sync(0xffffffffu, k_scale, i), v_of = __shfl_sync(0xffffffffu, v_scale, i);
+                bool ready = true;
+                if (number >= kStages) ready = barrier_wait(&shared->empty[stage], (number / kStages - 1) & 1, abort_flag);
+                if (!__all_sync(0xffffffffu, ready)) {
+                    alive = false;
+                    break;
+                }
+                if (lane == 0) {
+                    shared->key_scale[stage] = k_of;
+                    shared->value_scale[stage] = v_of;
+                    barrier_expect_bytes(&shared->full[stage], kStageBytes);
+                    uint8_t* tile = stages + stage * kStageBytes;
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) tma_load_3d(tile + h * kBoxBytes, &key_map, h * 128, 0, box, &shared->full[stage]);
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) tma_load_3d(tile + kTileBytes + h * kBoxBytes, &value_map, h * 128, 0, box, &shared->full[stage]);
+                }
+                __syncwarp();
+                asked = number + 1;
+            }
+        }
+        if (!alive && lane == 0)      // giving up: the copies in flight own their stages until they have landed
+            for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
+    } else {
+        // ---- queries: this lane's elements of heads g (and g + 8), brought to [1, 2) per head
+        unsigned q_frag[NT][kKeySteps][2];
+        float q_power[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int head = n * 8 + g;
+            const bool live = head < heads_here && count > 0;
+            const bf16* row = queries + (static_cast<size_t>(seq) * n_heads + head0 + (live ? head : 0)) * D;
+            float greatest = 0.0f;
+#pragma unroll
+            for (int step = 0; step < kKeySteps; ++step) {
+                const uint2 raw = live ? *reinterpret_cast<const uint2*>(row + key_element(step, t, 0)) : make_uint2(0u, 0u);
+                q_frag[n][step][0] = raw.x;
+                q_frag[n][step][1] = raw.y;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    greatest = fmaxf(greatest, finite_magnitude(__uint_as_float(q_frag[n][step][i] << 16)));
+                    greatest = fmaxf(greatest, finite_magnitude(__uint_as_float(q_frag[n][step][i] & 0xffff0000u)));
+                }
+            }
+            greatest = fmaxf(greatest, __shfl_xor_sync(0xffffffffu, greatest, 1));
+            greatest = fmaxf(greatest, __shfl_xor_sync(0xffffffffu, greatest, 2));
+            const int exponent = min(max(static_cast<int>(__float_as_uint(greatest) >> 23) - 127, -100), 126);
+            const float inverse = power_of_two(-exponent);
+            q_power[n] = power_of_two(exponent);
+#pragma unroll
+            for (int step = 0; step < kKeySteps; ++step)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    q_frag[n][step][i] = pack_half2(__uint_as_float(q_frag[n][step][i] << 16) * inverse, __uint_as_float(q_frag[n][step][i] & 0xffff0000u) * inverse);
+        }
+        // The factor of the scores of heads 2t and 2t + 1, but for the page's scale (log2 units).
+        float factor[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) factor[n][h] = __shfl_sync(0xffffffffu, q_power[n], (2 * t + h) * 4) * scale * kLog2e;
+
+        bool alive = true;
+        for (int number = 0; number < count; ++number) {
+            const int stage = number % kStages;
+            alive = __all_sync(0xffffffffu, barrier_wait(&shared->full[stage], (number / kStages) & 1, abort_flag));
+            if (!alive) break;
+            const int base = (page_lo + number) * kPage + warp * 16;      // position of this warp's first key
+            if (base < length && base + 16 > first) {
+                const uint8_t* key_tile = stages + stage * kStageBytes;
+                const uint8_t* value_tile = key_tile + kTileBytes;
+                const float k_scale = shared->key_scale[stage], v_scale = shared->value_scale[stage];
+                const bool whole = base >= first && base + 16 <= length;
+                // Scores of 16 keys and 8 heads: rows g and g + 8 are keys base + g and base + g + 8.
+                float score[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) score[n][j] = 0.0f;
+                const int row_lo = warp * 16 + g, row_hi = row_lo + 8;
+                constexpr int kGroups = D / 64;
+#pragma unroll
+                for (int c = 0; c < kGroups; ++c) {
+                    // Odd rows take the groups of a pair in the other order, so that eight lanes read 128 different bytes.
+                    const int swapped = (c ^ 1) < kGroups && (g & 1) ? c ^ 1 : c;
+                    uint4 lo = page_chunk(key_tile, row_lo, swapped * 4 + t), hi = page_chunk(key_tile, row_hi, swapped * 4 + t);
+                    if ((c ^ 1) < kGroups) {
+                        if (c & 1) continue;
+                        uint4 lo2 = page_chunk(key_tile, row_lo, (swapped ^ 1) * 4 + t), hi2 = page_chunk(key_tile, row_hi, (swapped ^ 1) * 4 + t);
+                        const bool turn = (g & 1) != 0;
+                        const uint4 lo_first = turn ? lo2 : lo, lo_second = turn ? lo : lo2, hi_first = turn ? hi2 : hi, hi_second = turn ? hi : hi2;
+                        const unsigned low[8] = {lo_first.x, lo_first.y, lo_first.z, lo_first.w, lo_second.x, lo_second.y, lo_second.z, lo_second.w};
+                        const unsigned high[8] = {hi_first.x, hi_first.y, hi_first.z, hi_first.w, hi_second.x, hi_second.y, hi_second.z, hi_second.w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const unsigned a0 = decode_half2(low[j]), a2 = decode_half2(low[j] >> 16), a1 = decode_half2(high[j]), a3 = decode_half2(high[j] >> 16);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
+                        }
+                    } else {
+                        const unsigned low[4] = {lo.x, lo.y, lo.z, lo.w}, high[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const unsigned a0 = decode_half2(low[j]), a2 = decode_half2(low[j] >> 16), a1 = decode_half2(high[j]), a3 = decode_half2(high[j] >> 16);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int step = kGroups * 4; step < kKeySteps; ++step) {
+                    const unsigned low = page_word(key_tile, row_lo, step * 16 + t * 4), high = page_word(key_tile, row_hi, step * 16 + t * 4);
+                    const unsigned a0 = decode_half2(low), a2 = decode_half2(low >> 16), a1 = decode_half2(high), a3 = decode_half2(high >> 16);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][step][0], q_frag[n][step][1]);
+                }
+                const bool live_lo = base + g >= first && base + g < length, live_hi = base + g + 8 >= first && base + g + 8 < length;
+                float correction[NT][2];
+                unsigned pb0[NT], pb1[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float p[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float by = factor[n][h] * k_scale;
+                        const float low = live_lo ? score[n][h] * by : -INFINITY, high = live_hi ? score[n][2 + h] * by : -INFINITY;
+                        float most = fmaxf(low, high);
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                        const float new_max = fmaxf(running_max[n][h], most);      // finite: one of the 16 keys is visible
+                        correction[n][h] = exp2f(running_max[n][h] - new_max);
+                        running_max[n][h] = new_max;
+                        p[h] = exp2f(low - new_max);
+                        p[2 + h] = exp2f(high - new_max);
+                        running_sum[n][h] = running_sum[n][h] * correction[n][h] + p[h] + p[2 + h];
+                    }
+                    pb0[n] = pack_half2(p[0], p[1]);
+                    pb1[n] = pack_half2(p[2], p[3]);
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb0[n]) : "r"(pb0[n]));
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb1[n]) : "r"(pb1[n]));
+                }
+                // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9, columns 128 r + 16 g .. + 16.
+#pragma unroll
+                for (int r = 0; r < kValueRounds; ++r) {
+                    const int chunk = 8 * r + g;
+                    uint4 v[4];
+                    const int slots[4] = {2 * t, 2 * t + 1, 2 * t + 8, 2 * t + 9};
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        v[s] = chunk * 16 < D ? page_chunk(value_tile, warp * 16 + slots[s], chunk) : make_uint4(0u, 0u, 0u, 0u);
+                        // What nobody sees may be NaN, and a weight of zero would not hide that.
+                        if (!whole && (base + slots[s] < first || base + slots[s] >= length)) v[s] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    const unsigned w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+                    const unsigned w8[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {      // columns 2 i (row g) and 2 i + 1 (row g + 8) of this lane's 16
+                        const unsigned pick = (i & 1) ? 0x7362u : 0x5140u;
+                        const unsigned near = __byte_perm(w0[i >> 1], w1[i >> 1], pick), far = __byte_perm(w8[i >> 1], w9[i >> 1], pick);
+                        const unsigned a0 = decode_half2(near), a1 = decode_half2(near >> 16), a2 = decode_half2(far), a3 = decode_half2(far >> 16);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(part, a0, a1, a2, a3, pb0[n], pb1[n]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[n][r][i][j] = fmaf(acc[n][r][i][j], correction[n][j & 1], part[j] * v_scale);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) barrier_arrive(&shared->empty[stage]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                running_sum[n][h] += __shfl_xor_sync(0xffffffffu, running_sum[n][h], 4);
+                running_sum[n][h] += __shfl_xor_sync(0xffffffffu, running_sum[n][h], 8);
+                running_sum[n][h] += __shfl_xor_sync(0xffffffffu, running_sum[n][h], 16);
+            }
+    }
+    __syncthreads();      // the stages are done with
+    if (warp < kWarps) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int head = n * 8 + 2 * t + h;
+#pragma unroll
+                for (int r = 0; r < kValueRounds; ++r)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int column = 128 * r + 16 * g + 2 * i;
+                        if (column < D) *reinterpret_cast<float2*>(&merge_o[warp][head][column]) = make_float2(acc[n][r][i][h], acc[n][r][i][2 + h]);
+                    }
+                if (g == 0) {
+                    merge_ml[warp][head][0] = running_max[n][h];
+                    merge_ml[warp][head][1] = running_sum[n][h];
+                }
+            }
+    }
+    __syncthreads();
+    const bool failed = *abort_flag != 0;
+    const size_t record = (static_cast<size_t>(seq) * n_heads + head0) * splits + split;
+    for (int index = threadIdx.x; index < heads_here * D; index += kThreads) {
+        const int h = index / D, c = index % D;
+        float total_max = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) total_max = fmaxf(total_max, merge_ml[w][h][0]);
+        float o = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (merge_ml[w][h][1] == 0.0f) continue;      // saw no key
+            const float by = exp2f(merge_ml[w][h][0] - total_max);
+            o += merge_o[w][h][c] * by;
+            sum += merge_ml[w][h][1] * by;
+        }
+        if (splits == 1) {
+            if (!failed) out[(static_cast<size_t>(seq) * n_heads + head0 + h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);      // a sequence without positions: zeros
+        } else if (clustered) {
+            merge_o[0][h][c] = o;      // this thread alone reads and writes (h, c) of the first warp's part
+            if (c == 0) {
+                block_ml[h][0] = total_max;
+                block_ml[h][1] = sum;
+            }
+        } else if (!failed) {
+            const size_t slot = record + static_cast<size_t>(h) * splits;
+            if (sum != 0.0f) partial_o[slot * D + c] = o;
+            if (c == 0) {
+                partial_ml[slot * 2] = total_max;
+                partial_ml[slot * 2 + 1] = sum;
+            }
+        }
+    }
+    if (splits == 1 || !clustered) return;
+    cluster_share_abort(&shared->abort_flag, splits);
+    cluster_sync_all();
+    if (*abort_flag == 0) {
+        const int rank = blockIdx.x;      // the cluster spans the grid's x
+        for (int index = rank * kThreads + threadIdx.x; index < heads_here * D; index += splits * kThreads) {
+            const int h = index / D, c = index % D;
+            const uint32_t o_address = smem_address(&merge_o[0][h][c]), ml_address = smem_address(&block_ml[h][0]);
+            float split_max[kMostClustered], split_sum[kMostClustered], split_o[kMostClustered];
+#pragma unroll
+            for (int s = 0; s < kMostClustered; ++s) {
+                split_max[s] = -INFINITY;
+                split_sum[s] = split_o[s] = 0.0f;
+                if (s < splits) {
+                    const uint32_t remote = cluster_address_of(ml_address, s);
+                    split_max[s] = cluster_load(remote);
+                    split_sum[s] = cluster_load(remote + 4);
+                    split_o[s] = cluster_load(cluster_address_of(o_address, s));
+                }
+            }
+            float total_max = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < kMostClustered; ++s) total_max = fmaxf(total_max, split_max[s]);
+            float o = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kMostClustered; ++s) {
+                if (split_sum[s] == 0.0f) continue;      // a range without a position
+                const float by = exp2f(split_max[s] - total_max);
+                o += split_o[s] * by;
+                sum += split_sum[s] * by;
+            }
+            out[(static_cast<size_t>(seq) * n_heads + head0 + h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);
+        }
+    }
+    cluster_sync_all();      // nobody leaves while its results are read
+}
+
+// Joins the records of a sequence's ranges in their order: a block to a head, a thread to a column.
+__global__ void join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out, int n_heads, int splits) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    __shared__ float factor[256];
+    __shared__ float inverse;
+    const int head = blockIdx.x, seq = blockIdx.y;
+    const size_t base = (static_cast<size_t>(seq) * n_heads + head) * splits;
+    if (threadIdx.x < 32) {
+        float total_max = -INFINITY, sum = 0.0f;
+        for (int s = threadIdx.x; s < splits; s += 32)
+            if (partial_ml[(base + s) * 2 + 1] != 0.0f) total_max = fmaxf(total_max, partial_ml[(base + s) * 2]);
+        total_max = warp_max(total_max);
+        for (int s = threadIdx.x; s < splits; s += 32) {
+            const float own = partial_ml[(base + s) * 2 + 1];
+            factor[s] = own != 0.0f ? exp2f(partial_ml[(base + s) * 2] - total_max) : 0.0f;
+            sum += own != 0.0f ? own * factor[s] : 0.0f;
+        }
+        sum = warp_sum(sum);
+        if (threadIdx.x == 0) inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += blockDim.x) {
+        float o = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) {
+            const float by = factor[s];
+            const float value = by != 0.0f ? partial_o[(base + s) * D + c] : 0.0f;      // a range without a position left no context
+            o += value * by;
+        }
+        out[(static_cast<size_t>(seq) * n_heads + head) * D + c] = __float2bfloat16_rn(o * inverse);
+    }
+}
+
+int page_map(CUtensorMap* map, const void* pages, long long boxes) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t extents[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(kPage), static_cast<cuuint64_t>(boxes)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(D) * kPage};
+    const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(kPage), 1};      // rows shorter than a box are filled with zeros
+    const cuuint32_t steps[3] = {1, 1, 1};
+    const CUresult result = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), extents, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return result == CUDA_SUCCESS ? 0 : cudaErrorInvalidValue;
+}
+
+constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + kStages * kStageBytes; }
+
+template <int NT>
+int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const bf16* queries, bf16* out, const float* key_scales, const float* value_scales, float* partial_o,
+           float* partial_ml, const int* seq_len, const int* page_rows, int page_stride, int n_seqs, int n_heads, int n_kv_heads, int passes, float scale, int window, int splits,
+           cudaStream_t stream) {
+    static bool ready[64] = {};
+    int device = 0;
+    cudaError_t status = cudaGetDevice(&device);
+    if (status != cudaSuccess) return static_cast<int>(status);
+    if (device >= 64 || !ready[device]) {
+        status = cudaFuncSetAttribute(decode8_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes());
+        if (status != cudaSuccess) return static_cast<int>(status);
+        if (device < 64) ready[device] = true;
+    }
+    const dim3 grid(splits, n_kv_heads * passes, n_seqs);
+    const bool clustered = splits > 1 && splits <= kMostClustered;
+    int code;
+    if (clustered)
+        code = tau_launch_clusters_as(false, splits, decode8_kernel<NT>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, queries, out, key_scales, value_scales, partial_o,
+                                      partial_ml, seq_len, page_rows, page_stride, n_heads, n_kv_heads, passes, scale, window, splits, 1);
+    else
+        code = tau_launch_as(false, decode8_kernel<NT>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, queries, out, key_scales, value_scales, partial_o, partial_ml, seq_len,
+                             page_rows, page_stride, n_heads, n_kv_heads, passes, scale, window, splits, 0);
+    return code ? code : tau_launch_status();
+}
+
+}  // namespace
+
+// Query heads to a block: 16 where a group has more than 8 and a head's accumulators leave room for them.
+static int heads_to_a_block(int group) { return group > 8 && D <= 128 ? 16 : 8; }
+
+TAU_EXPORT int tau_decode8_passes(int group) { return (group + heads_to_a_block(group) - 1) / heads_to_a_block(group); }
+
+TAU_EXPORT int tau_decode8_most_clustered() { return kMostClustered; }
+
+TAU_EXPORT int tau_decode8_status() {
+    int flag = 0;
+    cudaDeviceSynchronize();
+    if (cudaMemcpyFromSymbol(&flag, wait_error, sizeof(flag)) != cudaSuccess) return -1;
+    return flag;
+}
+
+// bfloat16 queries and output [sequences, n_heads D]; pages [boxes / n_kv_heads, n_kv_heads, 64, D] of e4m3 codes with scales [boxes].  More than 8 splits need
+// scratch of n_seqs * n_heads * splits * (D + 2) floats.
+TAU_EXPORT int tau_decode8(const void* queries, const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* out, const int* seq_len,
+                           const int* page_rows, int page_stride, long long boxes, int n_seqs, int n_heads, int n_kv_heads, float scale, int window, int splits, float* scratch,
+                           long long scratch_floats, void* stream) {
+    if (n_seqs <= 0) return 0;
+    if (!queries || !key_pages || !value_pages || !key_scales || !value_scales || !out || !seq_len || !page_rows || page_stride <= 0 || boxes <= 0 || n_heads <= 0 || n_kv_heads <= 0 ||
+        n_heads % n_kv_heads != 0 || window < 0 || splits < 1 || splits > 256 || n_seqs > 65535 || boxes > 0x7fffffffll ||
+        (splits > kMostClustered && (!scratch || scratch_floats < static_cast<long long>(n_seqs) * n_heads * splits * (D + 2))))
+        return cudaErrorInvalidValue;
+    CUtensorMap key_map, value_map;
+    int status = page_map(&key_map, key_pages, boxes);
+    if (!status) status = page_map(&value_map, value_pages, boxes);
+    if (status) return status;
+    const int group = n_heads / n_kv_heads, passes = tau_decode8_passes(group);
+    if (n_kv_heads * passes > 65535) return cudaErrorInvalidValue;
+    float* partial_ml = scratch ? scratch + static_cast<size_t>(n_seqs) * n_heads * splits * D : nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if constexpr (D <= 128) {
+        if (heads_to_a_block(group) == 16) {
+            status = launch<2>(key_map, value_map, static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch, partial_ml, seq_len, page_rows, page_stride,
+                               n_seqs, n_heads, n_kv_heads, passes, scale, window, splits, s);
+            if (status || splits <= kMostClustered) return status;
+            tau_launch(join_kernel, dim3(n_heads, n_seqs), dim3(D < 128 ? D : 128), 0, s, scratch, partial_ml, static_cast<bf16*>(out), n_heads, splits);
+            return tau_launch_status();
+        }
+    }
+    status = launch<1>(key_map, value_map, static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch, partial_ml, seq_len, page_rows, page_stride, n_seqs, n_heads,
+                       n_kv_heads, passes, scale, window, splits, s);
+    if (status || splits <= kMostClustered) return status;
+    tau_launch(join_kernel, dim3(n_heads, n_seqs), dim3(D < 128 ? D : 128), 0, s, scratch, partial_ml, static_cast<bf16*>(out), n_heads, splits);
+    return tau_launch_status();
+}

@@ -88,7 +88,7 @@ _CLASS_OF = {
     "side_gate": "activation", "unit_add_mix": "norm", "norm_rows": "norm", "relu_squared": "activation",
     "short_conv": "recurrence", "delta_prepare": "recurrence", "delta_rule": "recurrence", "selective_scan": "recurrence",
     "masked_prepare": "attention", "masked_attention": "attention", "talking_decode": "attention", "shared_key_decode": "attention", "gated_rows": "attention",
-    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gate_groups": "activation", "cache8_store": "attention", "cache8_read": "attention",
+    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
     "token_shift": "recurrence", "tanh": "activation", "channel_decay": "recurrence", "wkv": "recurrence", "forget_gates": "recurrence", "turn_heads": "recurrence",
 }
 _timing = None     # while timing: [last event, [(class, event after the launch), ...]]
@@ -141,7 +141,7 @@ def _check(status: int, what: str, kernels_launched: int = 1) -> None:
 
 
 _STATUS = {"gemm_tc": "tau_gemm_tc_status", "gemm_f32_tc": "tau_gemm_f32_tc_status", "attention_f32_tc": "tau_attention_f32_tc_status", "attention_prefill_tc": "tau_attention_prefill_tc_status", "attention_prefill": "tau_attention_prefill_status",
-           "recurrence": "tau_recurrence_status", "delta_rule": "tau_delta_status"}
+           "recurrence": "tau_recurrence_status", "attention_decode8": "tau_decode8_status", "delta_rule": "tau_delta_status"}
 
 
 def waits_that_ran_out() -> list:
@@ -1018,11 +1018,29 @@ CODE_DTYPE = torch.float8_e4m3fn
 
 
 def _here(*tensors) -> None:
-    """`_on_device` for kernels that also refuse tensors of another device than the current one, whose stream they are launched on."""
-    _on_device(*tensors)
-    current = torch.cuda.current_device()
+    """Refuses tensors that do not lie on the current device, whose current stream the kernels are launched on."""
+    current = torch.cuda.current_device() if torch.cuda.is_initialized() else -2
     for tensor in tensors:
-        _require(tensor is None or tensor.device.index == current, "tensors must lie on the current CUDA device")
+        if tensor is not None and tensor.get_device() != current:
+            _require(False, "tensors must lie on the current CUDA device; there is no CPU path")
+
+
+_functions = {}
+
+
+def _function(source: str, name: str, signature: str, defines=()):
+    """A C symbol with its argument types (`p` pointer, `i` int, `l` long long, `f` float; the last one, the stream, is a pointer too), looked up once."""
+    key = (name, defines)
+    function = _functions.get(key)
+    if function is None:
+        function = getattr(build.load_library(source, defines), name)
+        function.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}[letter] for letter in signature] + [ctypes.c_void_p]
+        _functions[key] = function
+    return function
+
+
+def _address(tensor: Optional[torch.Tensor]):
+    return None if tensor is None else tensor.data_ptr()
 
 
 def _scale_blocks(count: int) -> int:
@@ -1043,9 +1061,8 @@ def quantize_blocks(weight):
     rows, columns = weight.shape
     codes = torch.empty((rows, columns), dtype=CODE_DTYPE, device=weight.device)
     scales = torch.empty((_scale_blocks(rows), _scale_blocks(columns)), dtype=torch.float32, device=weight.device)
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_quantize_blocks(_code(weight), _pointer(weight), ctypes.c_longlong(weight.stride(0)), _pointer(codes), _pointer(scales), ctypes.c_int(rows),
-                                       ctypes.c_int(columns), _stream()), "quantize_blocks")
+    run = _function("eight_bit.cu", "tau_quantize_blocks", "iplppii")
+    _check(run(_code(weight), weight.data_ptr(), weight.stride(0), codes.data_ptr(), scales.data_ptr(), rows, columns, _stream_handle()), "quantize_blocks")
     return codes, scales
 
 
@@ -1059,9 +1076,8 @@ def quantize_rows(values):
     rows, columns = values.shape
     codes = torch.empty((rows, columns), dtype=CODE_DTYPE, device=values.device)
     scales = torch.empty((_scale_blocks(columns), rows), dtype=torch.float32, device=values.device)
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_quantize_rows(_code(values), _pointer(values), ctypes.c_longlong(values.stride(0)), _pointer(codes), _pointer(scales), ctypes.c_int(rows),
-                                     ctypes.c_int(columns), _stream()), "quantize_rows")
+    run = _function("eight_bit.cu", "tau_quantize_rows", "iplppii")
+    _check(run(_code(values), values.data_ptr(), values.stride(0), codes.data_ptr(), scales.data_ptr(), rows, columns, _stream_handle()), "quantize_rows")
     return codes, scales
 
 
@@ -1086,9 +1102,9 @@ def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
 def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
     """The plain product of operands in 8 bits (`quantize_rows`, `quantize_blocks`), on the 32-bit pipes: every size, the kernel that the others are checked against."""
     rows, depth = x_codes.shape
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_gemm8_simt(_code(out), _pointer(x_codes), _pointer(x_scales), _pointer(codes), _pointer(scales), _pointer(bias), _pointer(out), ctypes.c_int(rows),
-                                  ctypes.c_int(codes.shape[0]), ctypes.c_int(depth), ctypes.c_longlong(out.stride(0)), _stream()), "gemm8_simt")
+    run = _function("eight_bit.cu", "tau_gemm8_simt", "ippppppiiil")
+    _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
+               _stream_handle()), "gemm8_simt")
 
 
 def linear8(values, codes, scales, bias, out) -> None:
@@ -1109,9 +1125,8 @@ def linear8_gated(values, codes, scales, out, limit: float = 0.0) -> None:
         return
     stacked = torch.empty((rows, features), dtype=torch.bfloat16, device=values.device)
     gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_gate_groups(_pointer(stacked), _pointer(out), ctypes.c_longlong(rows), ctypes.c_int(features // 2), ctypes.c_longlong(out.stride(0)),
-                                   ctypes.c_float(limit), _stream()), "gate_groups")
+    run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
+    _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
 
 
 def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows) -> None:
@@ -1153,13 +1168,11 @@ def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales,
     _here(keys, values, key_pages, value_pages, key_scales, value_scales, step.cu_seqlens, step.seq_start, page_rows, projected, queries, q_weight, k_weight, cos, sin)
     if step.n_tokens == 0:
         return
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_cache8_store(
-        _pointer(keys), ctypes.c_longlong(keys.stride(0)), _pointer(values), ctypes.c_longlong(values.stride(0)), _pointer(key_pages), _pointer(value_pages), _pointer(key_scales),
-        _pointer(value_scales), _pointer(step.cu_seqlens), _pointer(step.seq_start), _pointer(page_rows), ctypes.c_int(page_rows.shape[1]), ctypes.c_int(step.n_seqs),
-        ctypes.c_int(step.n_tokens), ctypes.c_int(1 if step.all_single else 0), ctypes.c_int(n_kv_heads), ctypes.c_int(head_dim), _pointer(projected),
-        ctypes.c_longlong(0 if projected is None else projected.stride(0)), _pointer(queries), ctypes.c_int(n_heads), _pointer(q_weight), _pointer(k_weight), ctypes.c_float(eps),
-        _pointer(cos), _pointer(sin), ctypes.c_int(rotary_dim), _stream()), "cache8_store")
+    run = _function("eight_bit.cu", "tau_cache8_store", "plplpppppppiiiiiiplpippfppi")
+    _check(run(keys.data_ptr(), keys.stride(0), values.data_ptr(), values.stride(0), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+               step.cu_seqlens.data_ptr(), step.seq_start.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], step.n_seqs, step.n_tokens, 1 if step.all_single else 0, n_kv_heads, head_dim,
+               _address(projected), 0 if projected is None else projected.stride(0), _address(queries), n_heads, _address(q_weight), _address(k_weight), eps, _address(cos), _address(sin),
+               rotary_dim, _stream_handle()), "cache8_store")
 
 
 def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int = 0, sparse: bool = False):
@@ -1172,12 +1185,35 @@ def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_row
     _require(step.n_seqs <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
     shape = (step.n_seqs * page_rows.shape[1], n_kv_heads, PAGE_TOKENS, head_dim)
     keys, values = (torch.empty(shape, dtype=torch.bfloat16, device=key_pages.device) for _ in range(2))
-    library = build.load_library("eight_bit.cu")
-    _check(library.tau_cache8_read(
-        _pointer(key_pages), _pointer(value_pages), _pointer(key_scales), _pointer(value_scales), _pointer(keys), _pointer(values), _pointer(step.seq_start), _pointer(step.seq_len),
-        _pointer(page_rows), ctypes.c_int(page_rows.shape[1]), ctypes.c_int(step.n_seqs), ctypes.c_int(n_kv_heads), ctypes.c_int(head_dim), ctypes.c_int(window),
-        ctypes.c_int(1 if sparse else 0), _stream()), "cache8_read")
+    run = _function("eight_bit.cu", "tau_cache8_read", "pppppppppiiiiii")
+    _check(run(key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(), values.data_ptr(), step.seq_start.data_ptr(),
+               step.seq_len.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], step.n_seqs, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
     return keys, values
+
+
+def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int] = None) -> int:
+    """Ranges that the pages of a sequence are cut into for `attention_decode8`: as many as keep all blocks (`kv_blocks` to a sequence and range) resident at once, three to an
+    SM, none without a page.  The length is rounded up to a power of two first, so that a captured graph serves a range of lengths."""
+    sms = sms or sm_count()
+    pages = max(1, (1 << max(0, (max_len - 1).bit_length())) // PAGE_TOKENS)
+    return max(1, min(pages, 3 * sms // max(1, n_seqs * kv_blocks), 64))
+
+
+def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
+    """One query token per sequence over its `seq_len` cached positions, read as they are held (`attention8` checks its arguments)."""
+    defines = (f"TAU_HEAD_DIM={head_dim}",)
+    n_seqs = step.n_seqs
+    group = n_heads // n_kv_heads
+    passes = -(-group // (16 if group > 8 and head_dim <= 128 else 8))
+    splits = min(step.decode_splits or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
+    scratch = torch.empty(n_seqs * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
+    run = _function("attention_decode8.cu", "tau_decode8", "ppppppppiliiifiipl", defines)
+    _check(run(queries.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.seq_len.data_ptr(),
+               page_rows.data_ptr(), page_rows.shape[1], key_pages.shape[0] * n_kv_heads, n_seqs, n_heads, n_kv_heads, scale, window, splits, _address(scratch),
+               0 if scratch is None else scratch.numel(), _stream_handle()), "attention_decode8", 1 if scratch is None else 2)
+
+
+DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 
 
 def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
@@ -1191,6 +1227,8 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
     if step.n_tokens == 0:
         return
+    if step.all_single and _prefer_optimized:
+        return attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     keys, values = cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, sparse=True)
     places = torch.arange(keys.shape[0], dtype=torch.int32, device=keys.device).view(step.n_seqs, -1)
     attention(queries, keys, values, out, step, places, n_heads, n_kv_heads, head_dim, scale, window)
