@@ -32,15 +32,21 @@ constexpr int kHalves = (D + 127) / 128;          // boxes of 128 bytes to a row
 constexpr int kBoxBytes = kPage * 128;
 constexpr int kTileBytes = kHalves * kBoxBytes;   // a page of a head's keys, or of its values
 constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kStages = kHalves == 1 ? 4 : 3;
+// Two pages ahead and four blocks to an SM where a page is 16 KB; three of 32 KB and two blocks for wider heads (64 sequences of 2,048 positions, 32 heads of 128 over 8: 54 us so,
+// 60 with four pages and three blocks, 61 with six and two).
+constexpr int kStages = kHalves == 1 ? 2 : 3;
 constexpr int kKeySteps = D / 16;                 // products of 16 head elements
 constexpr int kMostClustered = 8;
 constexpr float kLog2e = 1.4426950408889634f;
+// Weights are kept times 2^14: what f16 holds with all its bits then reaches down to 2^-28 of the greatest, and a long tail of small weights keeps its sum.
+constexpr float kWeightBits = 14.0f;
+constexpr float kLeastShare = 0.00390625f;      // 2^-8: a page whose value scale is smaller than this share of the accumulators' is added in 32 bits
 
 struct Shared {
     uint64_t full[kStages];
     uint64_t empty[kStages];
-    float key_scale[kStages], value_scale[kStages];
+    float key_scale[kStages], share[kStages], older[kStages];
+    float unit;
     int abort_flag;
 };
 
@@ -80,7 +86,7 @@ __device__ __forceinline__ int key_element(int step, int t, int i) {
 constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a lane holds 16 columns, 8 tiles of 16 rows
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 ? 4 : 2)
 decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
                const float* __restrict__ key_scales, const float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                const int* __restrict__ seq_len, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale, int window, int splits,
@@ -105,7 +111,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     volatile int* abort_flag = &shared->abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            barrier_init(&shared->full[s], 1);
+            barrier_init(&shared->full[s], 2);      // the copies', and the scales'
             barrier_init(&shared->empty[s], kWarps);
         }
         shared->abort_flag = 0;
@@ -119,7 +125,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     const int per_split = (max(0, pages_end - first_page) + splits - 1) / splits;
     const int page_lo = first_page + split * per_split, page_hi = min(pages_end, page_lo + per_split);
     const int count = max(0, page_hi - page_lo);
-    float running_max[NT][2], running_sum[NT][2];
+    float running_max[NT][2], running_sum[NT][2];      // log2 units; the sums and accumulators belong to weights exp2(score - max + 14)
+    float unit = 0.0f;      // producer: what one in the accumulators stands for, the greatest value scale of the pages so far
     float acc[NT][kValueRounds][8][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -145,7 +152,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             for (int i = 0; i < min(32, count - base); ++i) {
                 const int number = base + i, stage = number % kStages;
                 const int box = __shfl_sync(0xffffffffu, place, i);
-                const float k_of = __shfl_sync(0xffffffffu, k_scale, i), v_of = __shfl_sync(0xffffffffu, v_scale, i);
                 bool ready = true;
                 if (number >= kStages) ready = barrier_wait(&shared->empty[stage], (number / kStages - 1) & 1, abort_flag);
                 if (!__all_sync(0xffffffffu, ready)) {
@@ -153,8 +159,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     break;
                 }
                 if (lane == 0) {
-                    shared->key_scale[stage] = k_of;
-                    shared->value_scale[stage] = v_of;
                     barrier_expect_bytes(&shared->full[stage], kStageBytes);
                     uint8_t* tile = stages + stage * kStageBytes;
 #pragma unroll
@@ -162,10 +166,25 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h) tma_load_3d(tile + kTileBytes + h * kBoxBytes, &value_map, h * 128, 0, box, &shared->full[stage]);
                 }
-                __syncwarp();
                 asked = number + 1;
+                // The scales of the stages that were free from the start follow once all their copies are on their way.
+                if (number < kStages - 1 && number + 1 < count) continue;
+                for (int n = number < kStages ? 0 : number; n <= number; ++n) {
+                    const float k_of = __shfl_sync(0xffffffffu, k_scale, n - base), v_of = __shfl_sync(0xffffffffu, v_scale, n - base);
+                    // A page's value scale joins the weights as its share of the accumulators' unit (powers of two: exact), so a unit that grows rescales them.
+                    const float grown = fmaxf(unit, v_of);
+                    if (lane == 0) {
+                        shared->key_scale[n % kStages] = k_of;
+                        shared->share[n % kStages] = v_of / grown;
+                        shared->older[n % kStages] = unit / grown;
+                        barrier_arrive(&shared->full[n % kStages]);
+                    }
+                    unit = grown;
+                }
+                __syncwarp();
             }
         }
+        if (lane == 0) shared->unit = unit;
         if (!alive && lane == 0)      // giving up: the copies in flight own their stages until they have landed
             for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
     } else {
@@ -216,14 +235,14 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             if (base < length && base + 16 > first) {
                 const uint8_t* key_tile = stages + stage * kStageBytes;
                 const uint8_t* value_tile = key_tile + kTileBytes;
-                const float k_scale = shared->key_scale[stage], v_scale = shared->value_scale[stage];
+                const float k_scale = shared->key_scale[stage], share = shared->share[stage], older = shared->older[stage];
                 const bool whole = base >= first && base + 16 <= length;
                 // Scores of 16 keys and 8 heads: rows g and g + 8 are keys base + g and base + g + 8.
-                float score[NT][4];
+                float score[NT][4], score_odd[NT][4];      // two chains, so that consecutive products do not wait for each other
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) score[n][j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) score[n][j] = score_odd[n][j] = 0.0f;
                 const int row_lo = warp * 16 + g, row_hi = row_lo + 8;
                 constexpr int kGroups = D / 64;
 #pragma unroll
@@ -242,7 +261,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                         for (int j = 0; j < 8; ++j) {
                             const unsigned a0 = decode_half2(low[j]), a2 = decode_half2(low[j] >> 16), a1 = decode_half2(high[j]), a3 = decode_half2(high[j] >> 16);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
+                            for (int n = 0; n < NT; ++n) mma_f16(j & 1 ? score_odd[n] : score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
                         }
                     } else {
                         const unsigned low[4] = {lo.x, lo.y, lo.z, lo.w}, high[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -250,7 +269,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                         for (int j = 0; j < 4; ++j) {
                             const unsigned a0 = decode_half2(low[j]), a2 = decode_half2(low[j] >> 16), a1 = decode_half2(high[j]), a3 = decode_half2(high[j] >> 16);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
+                            for (int n = 0; n < NT; ++n) mma_f16(j & 1 ? score_odd[n] : score[n], a0, a1, a2, a3, q_frag[n][c * 4 + j][0], q_frag[n][c * 4 + j][1]);
                         }
                     }
                 }
@@ -259,9 +278,12 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     const unsigned low = page_word(key_tile, row_lo, step * 16 + t * 4), high = page_word(key_tile, row_hi, step * 16 + t * 4);
                     const unsigned a0 = decode_half2(low), a2 = decode_half2(low >> 16), a1 = decode_half2(high), a3 = decode_half2(high >> 16);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(score[n], a0, a1, a2, a3, q_frag[n][step][0], q_frag[n][step][1]);
+                    for (int n = 0; n < NT; ++n) mma_f16(step & 1 ? score_odd[n] : score[n], a0, a1, a2, a3, q_frag[n][step][0], q_frag[n][step][1]);
                 }
                 const bool live_lo = base + g >= first && base + g < length, live_hi = base + g + 8 >= first && base + g + 8 < length;
+                const bool apart = share < kLeastShare;      // a 16-bit weight would lose bits: the page's sums are taken apart and added in 32 bits
+                const float by_share = apart ? 1.0f : share;
+                bool moved = older != 1.0f;
                 float correction[NT][2];
                 unsigned pb0[NT], pb1[NT];
 #pragma unroll
@@ -270,22 +292,33 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float by = factor[n][h] * k_scale;
-                        const float low = live_lo ? score[n][h] * by : -INFINITY, high = live_hi ? score[n][2 + h] * by : -INFINITY;
+                        const float low = live_lo ? (score[n][h] + score_odd[n][h]) * by : -INFINITY, high = live_hi ? (score[n][2 + h] + score_odd[n][2 + h]) * by : -INFINITY;
                         float most = fmaxf(low, high);
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
                         const float new_max = fmaxf(running_max[n][h], most);      // finite: one of the 16 keys is visible
+                        moved |= new_max != running_max[n][h];
                         correction[n][h] = exp2f(running_max[n][h] - new_max);
                         running_max[n][h] = new_max;
-                        p[h] = exp2f(low - new_max);
-                        p[2 + h] = exp2f(high - new_max);
+                        p[h] = exp2f(low - new_max + kWeightBits);
+                        p[2 + h] = exp2f(high - new_max + kWeightBits);
                         running_sum[n][h] = running_sum[n][h] * correction[n][h] + p[h] + p[2 + h];
                     }
-                    pb0[n] = pack_half2(p[0], p[1]);
-                    pb1[n] = pack_half2(p[2], p[3]);
+                    pb0[n] = pack_half2(p[0] * by_share, p[1] * by_share);
+                    pb1[n] = pack_half2(p[2] * by_share, p[3] * by_share);
                     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb0[n]) : "r"(pb0[n]));
                     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb1[n]) : "r"(pb1[n]));
+                }
+                if (__any_sync(0xffffffffu, moved)) {      // in a long context almost never
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < kValueRounds; ++r)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) acc[n][r][i][j] *= correction[n][j & 1] * older;
                 }
                 // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9, columns 128 r + 16 g .. + 16.
 #pragma unroll
@@ -301,20 +334,47 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     }
                     const unsigned w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
                     const unsigned w8[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {      // columns 2 i (row g) and 2 i + 1 (row g + 8) of this lane's 16
+                    auto tile = [&](int i, unsigned (&a)[4]) {      // columns 2 i (row g) and 2 i + 1 (row g + 8) of this lane's 16
                         const unsigned pick = (i & 1) ? 0x7362u : 0x5140u;
                         const unsigned near = __byte_perm(w0[i >> 1], w1[i >> 1], pick), far = __byte_perm(w8[i >> 1], w9[i >> 1], pick);
-                        const unsigned a0 = decode_half2(near), a1 = decode_half2(near >> 16), a2 = decode_half2(far), a3 = decode_half2(far >> 16);
+                        a[0] = decode_half2(near);
+                        a[1] = decode_half2(near >> 16);
+                        a[2] = decode_half2(far);
+                        a[3] = decode_half2(far >> 16);
+                    };
+                    if (!apart) {
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(part, a0, a1, a2, a3, pb0[n], pb1[n]);
+                        for (int i = 0; i < 8; ++i) {
+                            unsigned a[4];
+                            tile(i, a);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) acc[n][r][i][j] = fmaf(acc[n][r][i][j], correction[n][j & 1], part[j] * v_scale);
+                            for (int n = 0; n < NT; ++n) mma_f16(acc[n][r][i], a[0], a[1], a[2], a[3], pb0[n], pb1[n]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            unsigned a[4];
+                            tile(i, a);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_f16(part, a[0], a[1], a[2], a[3], pb0[n], pb1[n]);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) acc[n][r][i][j] = fmaf(part[j], share, acc[n][r][i][j]);
+                            }
                         }
                     }
                 }
+            } else if (shared->older[stage] != 1.0f) {      // nothing of the page is this warp's, but its unit is
+                const float older = shared->older[stage];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < kValueRounds; ++r)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[n][r][i][j] *= older;
             }
             __syncwarp();
             if (lane == 0) barrier_arrive(&shared->empty[stage]);
@@ -330,6 +390,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     }
     __syncthreads();      // the stages are done with
     if (warp < kWarps) {
+        const float one = shared->unit;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -340,7 +401,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int column = 128 * r + 16 * g + 2 * i;
-                        if (column < D) *reinterpret_cast<float2*>(&merge_o[warp][head][column]) = make_float2(acc[n][r][i][h], acc[n][r][i][2 + h]);
+                        if (column < D) *reinterpret_cast<float2*>(&merge_o[warp][head][column]) = make_float2(acc[n][r][i][h] * one, acc[n][r][i][2 + h] * one);
                     }
                 if (g == 0) {
                     merge_ml[warp][head][0] = running_max[n][h];
