@@ -88,7 +88,7 @@ _CLASS_OF = {
     "side_gate": "activation", "unit_add_mix": "norm", "norm_rows": "norm", "relu_squared": "activation",
     "short_conv": "recurrence", "delta_prepare": "recurrence", "delta_rule": "recurrence", "selective_scan": "recurrence",
     "masked_prepare": "attention", "masked_attention": "attention", "talking_decode": "attention", "shared_key_decode": "attention", "gated_rows": "attention",
-    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
+    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gemm8_skinny": "product", "gemm8_tc": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
     "token_shift": "recurrence", "tanh": "activation", "channel_decay": "recurrence", "wkv": "recurrence", "forget_gates": "recurrence", "turn_heads": "recurrence",
 }
 _timing = None     # while timing: [last event, [(class, event after the launch), ...]]
@@ -141,7 +141,7 @@ def _check(status: int, what: str, kernels_launched: int = 1) -> None:
 
 
 _STATUS = {"gemm_tc": "tau_gemm_tc_status", "gemm_f32_tc": "tau_gemm_f32_tc_status", "attention_f32_tc": "tau_attention_f32_tc_status", "attention_prefill_tc": "tau_attention_prefill_tc_status", "attention_prefill": "tau_attention_prefill_status",
-           "recurrence": "tau_recurrence_status", "attention_decode8": "tau_decode8_status", "delta_rule": "tau_delta_status"}
+           "recurrence": "tau_recurrence_status", "attention_decode8": "tau_decode8_status", "gemm8_tc": "tau_gemm8_tc_status", "delta_rule": "tau_delta_status"}
 
 
 def waits_that_ran_out() -> list:
@@ -1107,26 +1107,64 @@ def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
                _stream_handle()), "gemm8_simt")
 
 
+SKINNY8_FUSED_ROWS = 8      # up to here the skinny kernel quantises the activations itself
+SKINNY8_MAX_ROWS = 32       # what it accepts quantised
+
+
+def gemm8_skinny(values, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
+    """The product for a few rows, bound by streaming the weight's codes once: bfloat16 rows (`x_scales` None, at most 8) or quantised ones (at most 32)."""
+    rows, depth = values.shape
+    _require(rows <= (SKINNY8_FUSED_ROWS if x_scales is None else SKINNY8_MAX_ROWS), "too many rows for the skinny kernel")
+    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "iplpppppiiilif")
+    _check(run(_code(out), values.data_ptr(), values.stride(0), _address(x_scales), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth,
+               out.stride(0), 1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
+
+
+def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
+    """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (64, 128, 256; 0: by the number of tiles) with K cut into `ranges`
+    (1 to 8; 0: as many as leave no SM without work)."""
+    rows, depth = x_codes.shape
+    run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
+    _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
+               1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
+
+
+def gemm8_tc_status() -> int:
+    """0 unless a bounded wait inside the 8-bit tensor-core product ran out (synchronises the device)."""
+    return build.load_library("gemm8_tc.cu").tau_gemm8_tc_status()
+
+
+def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> None:
+    rows, features = values.shape[0], codes.shape[0]
+    if rows == 0 or features == 0:
+        return
+    if not _prefer_optimized:
+        if not gated:
+            return gemm8_simt(*quantize_rows(values), codes, scales, bias, out)
+        stacked = torch.empty((rows, features), dtype=torch.bfloat16, device=values.device)
+        gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
+        run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
+        return _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
+    if rows <= SKINNY8_FUSED_ROWS and values.dtype == torch.bfloat16:
+        return gemm8_skinny(values, None, codes, scales, bias, out, gated, limit)
+    x_codes, x_scales = quantize_rows(values)
+    if rows <= SKINNY8_FUSED_ROWS:
+        return gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated, limit)
+    gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated, limit)
+
+
 def linear8(values, codes, scales, bias, out) -> None:
     """`out = values @ weight.T + bias` with the weight in 8 bits (`quantize_blocks`) and the activations brought to 8 bits within the call, a scale for each
     row and 128 columns; sums in 32 bits, one rounding to the output's type."""
     _check_linear8(values, codes, scales, bias, out, False)
-    if values.shape[0] == 0 or codes.shape[0] == 0:
-        return
-    gemm8_simt(*quantize_rows(values), codes, scales, bias, out)
+    _linear8(values, codes, scales, bias, out, False, 0.0)
 
 
 def linear8_gated(values, codes, scales, out, limit: float = 0.0) -> None:
     """`out = silu(values @ gate.T) * (values @ up.T)` with the stacked weight (groups of 8 gate rows followed by their 8 up rows) in 8 bits; `limit` > 0: the
     clamped form of `silu_mul`.  Gate and up values are rounded to bfloat16 as a product that is not gated would store them."""
     _check_linear8(values, codes, scales, None, out, True)
-    rows, features = values.shape[0], codes.shape[0]
-    if rows == 0 or features == 0:
-        return
-    stacked = torch.empty((rows, features), dtype=torch.bfloat16, device=values.device)
-    gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
-    run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
-    _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
+    _linear8(values, codes, scales, None, out, True, limit)
 
 
 def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows) -> None:

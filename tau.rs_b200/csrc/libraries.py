@@ -14,6 +14,8 @@ def all_libraries() -> List[Tuple[str, Sequence[str]]]:
         ("attention_f32_tc.cu", ()),
         ("attention_generic.cu", ()),
         ("eight_bit.cu", ()),
+        ("gemm8_skinny.cu", ()),
+        ("gemm8_tc.cu", ()),
         ("sampling.cu", ()),
         ("random_init.cu", ()),
         ("stream32.cu", ()),
