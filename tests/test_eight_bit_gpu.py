@@ -89,6 +89,34 @@ def test_gated_products(rows, depth, inner, limit):
     assert bool(((out.double() - exact).abs() <= bound).all()), float(((out.double() - exact).abs() / bound).max())
 
 
+@pytest.mark.parametrize("rows, depth, features", [(1, 16, 16), (100, 1040, 530), (300, 400, 272), (513, 1296, 800)])
+@pytest.mark.parametrize("tile, ranges", [(64, 1), (64, 3), (64, 8), (128, 1), (128, 2), (128, 7), (256, 1), (256, 2), (256, 5), (512, 1)])
+def test_every_tile_of_the_tensor_core_product(rows, depth, features, tile, ranges):
+    """Each width of tile, pairs of SMs, ranges of K (more than there are blocks of K too), ungated in both types and gated, into rows of a wider tensor."""
+    x, w = spread_values(rows, depth, seed=depth, outliers=False).to(torch.bfloat16), (spread_values(features, depth, seed=features, outliers=False) * depth ** -0.5).to(torch.bfloat16)
+    x_codes, x_scales = kernels.quantize_rows(x.cuda())
+    codes, scales = kernels.quantize_blocks(w.cuda())
+    held_x, held_w = plain.held_rows(x)[0].cuda(), plain.held_blocks(w)[0].cuda()
+    exact = held_x @ held_w.T
+    for out_dtype, apart in ((torch.float32, 8), (torch.bfloat16, 3)):
+        wide = torch.full((rows, features + apart), 7.0, device="cuda", dtype=out_dtype)
+        kernels.gemm8_tc(x_codes, x_scales, codes, scales, None, wide[:, :features], features=tile, ranges=ranges)
+        assert bool(((wide[:, :features].double() - exact).abs() <= product_bound(held_x, held_w, exact, out_dtype)).all()) and bool((wide[:, features:] == 7.0).all())
+    if features % 16 == 0:
+        stacked, out = torch.empty(rows, features, device="cuda", dtype=torch.bfloat16), torch.full((rows, features // 2 + 8), 7.0, device="cuda", dtype=torch.bfloat16)
+        kernels.gemm8_tc(x_codes, x_scales, codes, scales, None, stacked, features=tile, ranges=ranges)
+        kernels.gemm8_tc(x_codes, x_scales, codes, scales, None, out[:, : features // 2], gated=True, features=tile, ranges=ranges)
+        pairs = stacked.double().view(rows, -1, 2, 8)
+        gate, up = (pairs[:, :, i].reshape(rows, -1) for i in (0, 1))
+        wanted = torch.nn.functional.silu(gate) * up
+        # The same roundings before the activation.  __expf(x) is documented to be within 2 + 1.173 |x| units of 2^-23, the quotient within 2, the sum and the product are rounded once each
+        # (2^-24), and the quotient of a denominator above 2^126 may be 0 (a gate below -87: the result is smaller than 2^-126 |g u|).
+        bound = (2.0 ** -8 + 2.0 ** -23 * (6.0 + 1.173 * gate.abs())) * wanted.abs() + 2.0 ** -126 * (gate * up).abs() + 1e-37
+        assert bool(((out[:, : features // 2].double() - wanted).abs() <= bound).all()), float(((out[:, : features // 2].double() - wanted).abs() / bound).max())
+        assert bool((out[:, features // 2 :] == 7.0).all())
+    assert kernels.gemm8_tc_status() == 0
+
+
 def test_a_row_that_is_not_finite_stays_alone():
     """An infinity and a NaN in two rows make those rows' results NaN and leave the others as they are; so does a NaN in a weight's row for its feature."""
     for rows in (4, 40, 300):
