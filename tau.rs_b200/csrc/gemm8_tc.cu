@@ -48,7 +48,7 @@ __device__ __forceinline__ void mma_issue_e4m3(uint32_t sums, uint64_t a, uint64
 }
 
 constexpr int stage_bytes(int bn) { return (BM + bn) * BK; }
-constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
+constexpr int stages_of(int bn) { return bn == 256 ? 4 : 6; }
 constexpr int shared_bytes(int bn) { return static_cast<int>(sizeof(Shared)) + 1024 + stages_of(bn) * stage_bytes(bn); }
 
 // Adds a block's sums of this warp's 32 tokens and 64 features, times the token's factor; `Step` columns of tensor memory at a time: 32, or 16 where 18 warps leave a thread 100
@@ -313,189 +313,6 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
     }
 }
 
-// ---- pairs of SMs on one tile -----------------------------------------------------------------------------------------------------------
-// With many tokens the product is bound by what L2 delivers: a 128 x 256 tile brings 48 KB for each 128 columns of K.  Two blocks of a cluster share a tile of 256 tokens x 256
-// features instead: each brings 128 of the tokens and 128 of the weight's rows, 32 KB, one warp of the first block issues tcgen05.mma.cta_group::2, which reads
-// both blocks' weight rows, and each block's tensor memory receives its tokens' sums.  The first block's `full` barriers count the bytes of both blocks' copies, commits signal both
-// blocks, and the warps that add, of both blocks, release an accumulator at the first block's barrier.  No copy is multicast.
-__device__ __forceinline__ void tma_load_2d_pair(void* destination, const CUtensorMap* map, int inner, int outer, uint32_t cluster_barrier) {
-    if (operands_lost()) return;
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_address(destination)),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(inner), "r"(outer), "r"(cluster_barrier)
-                 : "memory");
-}
-
-__device__ __forceinline__ void mma_issue_e4m3_pair(uint32_t sums, uint64_t a, uint64_t b, uint32_t descriptor, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(sums),
-        "l"(a), "l"(b), "r"(descriptor), "r"(accumulate)
-        : "memory");
-}
-
-// Arrives, in both blocks of the pair, at the barrier that lies where `barrier` lies, once the products issued so far are done.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* barrier) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_address(barrier)), "h"(static_cast<uint16_t>(3)) : "memory");
-}
-
-__device__ __forceinline__ void barrier_arrive_cluster(uint32_t cluster_barrier) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_barrier) : "memory");
-}
-
-constexpr int kPairTokens = 256, kPairFeatures = 256;
-constexpr uint32_t kPairStages = 6, kPairStageBytes = 2 * 128 * BK;
-constexpr int kPairThreads = threads(kPairFeatures);
-constexpr int pair_shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + static_cast<int>(kPairStages * kPairStageBytes); }
-
-template <typename TOut, bool Gated>
-__global__ void __launch_bounds__(kPairThreads, 1)
-gemm8_tc_pair_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_constant__ CUtensorMap weight_map, const float* __restrict__ x_scales, const float* __restrict__ w_scales,
-                     const float* __restrict__ bias, TOut* __restrict__ out, int M, int N, int K, long long out_stride, int wide, float gate_limit) {
-    extern __shared__ uint8_t shared_raw[];
-    Shared* shared = reinterpret_cast<Shared*>(shared_raw);
-    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + sizeof(Shared) + 1023) & ~uintptr_t(1023));
-    constexpr uint32_t kColumns = 2 * kPairFeatures, kInputBytes = 128 * BK;      // all of tensor memory
-    static_assert(alone_on_an_sm(pair_shared_bytes()), "two blocks of an SM could wait for each other's tensor memory");
-    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
-    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-    const int token_tiles = (M + kPairTokens - 1) / kPairTokens, n_tiles = (N + kPairFeatures - 1) / kPairFeatures * token_tiles, k_blocks = (K + BK - 1) / BK;
-    volatile int* abort_flag = &shared->abort_flag;
-
-    if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < kPairStages; ++s) {
-            barrier_init(&shared->full[s], 1);
-            barrier_init(&shared->empty[s], 1);
-        }
-        for (int a = 0; a < 2; ++a) {
-            barrier_init(&shared->sums_full[a], 1);
-            barrier_init(&shared->sums_empty[a], 2 * adders(kPairFeatures));      // of both blocks (used in the first)
-        }
-        shared->abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&shared->tensor_memory_base)), "r"(kColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
-    tensor_fence_before_sync();
-    cluster_sync_all();      // both blocks' barriers exist before either signals the other's
-    tensor_fence_after_sync();
-    const uint32_t tensor_base = shared->tensor_memory_base;
-    grid_dependents_launch();
-
-    if (warp == 0) {
-        // ---- copies (both blocks): this block's 128 tokens and its 128 rows of the weight
-        if (lane == 0) {
-            grid_dependency_wait();
-            uint32_t stage = 0, phase = 0;
-            bool alive = true;
-            for (int tile = pair; tile < n_tiles && alive; tile += n_pairs) {
-                const int token0 = tile % token_tiles * kPairTokens + static_cast<int>(rank) * 128, feature0 = tile / token_tiles * kPairFeatures + static_cast<int>(rank) * 128;
-                for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!barrier_wait(&shared->empty[stage], phase ^ 1u, abort_flag)) { alive = false; break; }
-                    uint8_t* input_tile = tiles + stage * kPairStageBytes;
-                    const uint32_t first_full = cluster_address(&shared->full[stage], 0);
-                    if (rank == 0) barrier_expect_bytes(&shared->full[stage], 2 * kPairStageBytes);      // the bytes of both blocks
-                    tma_load_2d_pair(input_tile, &input_map, kb * BK, token0, first_full);
-                    tma_load_2d_pair(input_tile + kInputBytes, &weight_map, kb * BK, feature0, first_full);
-                    if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
-                }
-            }
-            // The last commits arrive at this block's barriers, and what the copies bring lies in its memory: nobody leaves before.
-            for (uint32_t s = 0; s < kPairStages; ++s) {
-                if (alive) alive = barrier_wait(&shared->empty[stage], phase ^ 1u, abort_flag);
-                else barrier_outlast(&shared->empty[stage], phase ^ 1u);
-                if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
-            }
-        }
-    } else if (warp == 1) {
-        // ---- products: one warp of the first block, for both
-        if (rank == 0) {
-            const bool leader = elect_one();
-            const uint32_t base = __shfl_sync(0xffffffffu, tensor_base, 0), first_tile = __shfl_sync(0xffffffffu, smem_address(tiles), 0);
-            auto warp_wait = [&](uint64_t* barrier, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(barrier, parity, abort_flag)) != 0; };
-            const uint32_t descriptor = descriptor_e4m3(kPairTokens, kPairFeatures);
-            uint32_t stage = 0, phase = 0, number = 0;
-            bool alive = true;
-            for (int tile = pair; tile < n_tiles && alive; tile += n_pairs) {
-                for (int kb = 0; kb < k_blocks; ++kb, ++number) {
-                    const uint32_t slot = number & 1u, use = number >> 1;
-                    if (use > 0 && !warp_wait(&shared->sums_empty[slot], (use - 1) & 1u)) { alive = false; break; }
-                    if (!warp_wait(&shared->full[stage], phase)) { alive = false; break; }
-                    tensor_fence_after_sync();
-                    const uint32_t input_address = first_tile + stage * kPairStageBytes, weight_address = input_address + kInputBytes;
-                    if (leader) {
-#pragma unroll
-                        for (int k = 0; k < BK / kMmaK; ++k)
-                            mma_issue_e4m3_pair(base + slot * kPairFeatures, tile_descriptor(input_address + k * kMmaK), tile_descriptor(weight_address + k * kMmaK), descriptor, k > 0 ? 1u : 0u);
-                        mma_commit_pair(&shared->empty[stage]);
-                        mma_commit_pair(&shared->sums_full[slot]);
-                    }
-                    __syncwarp();
-                    if (++stage == kPairStages) { stage = 0; phase ^= 1u; }
-                }
-            }
-        }
-    } else {
-        // ---- adders (both blocks): this block's 128 tokens, 64 of the tile's features to a warp
-        const int quarter = warp & 3, part = (warp - 2) >> 2;
-        uint32_t number = 0;
-        bool alive = true;
-        grid_dependency_wait();
-        for (int tile = pair; tile < n_tiles && alive; tile += n_pairs) {
-            const int feature0 = tile / token_tiles * kPairFeatures + part * kPart, token = tile % token_tiles * kPairTokens + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-            const float* x_scale = x_scales + min(token, M - 1);
-            const float* w_scale = w_scales + static_cast<size_t>(min(feature0, N - 1) / kScaleBlock) * k_blocks;
-            float sums[kPart];
-#pragma unroll
-            for (int c = 0; c < kPart; ++c) sums[c] = 0.0f;
-            float x_next[2], w_next[2];
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                x_next[a] = a < k_blocks ? x_scale[static_cast<size_t>(a) * M] : 0.0f;
-                w_next[a] = a < k_blocks ? w_scale[a] : 0.0f;
-            }
-            for (int kb = 0; kb < k_blocks; ++kb, ++number) {
-                const uint32_t slot = number & 1u, use = number >> 1;
-                const float factor = x_next[0] * w_next[0];
-                x_next[0] = x_next[1];
-                w_next[0] = w_next[1];
-                if (kb + 2 < k_blocks) {
-                    x_next[1] = x_scale[static_cast<size_t>(kb + 2) * M];
-                    w_next[1] = w_scale[kb + 2];
-                }
-                if (!__all_sync(0xffffffffu, barrier_wait(&shared->sums_full[slot], use & 1u, abort_flag))) { alive = false; break; }
-                tensor_fence_after_sync();
-                auto release = [&]() {
-                    if (lane == 0) barrier_arrive_cluster(cluster_address(&shared->sums_empty[slot], 0));
-                };
-                const uint32_t address = tensor_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * kPairFeatures + part * kPart;
-                if (token - lane < M && feature0 < N) add_block<16>(address, factor, sums, release);
-                else release();
-            }
-            if (!alive) break;
-            if (token < M) {
-                TOut* row = out + static_cast<size_t>(token) * out_stride;
-                constexpr int kStep = Gated ? 16 : 8;
-#pragma unroll
-                for (int c = 0; c < kPart; c += kStep)
-                    if (feature0 + c < N) finish_row<TOut, Gated>(sums + c, feature0 + c, N, bias, row, wide != 0, gate_limit);
-            }
-        }
-    }
-
-    // ---- both blocks meet (neither's shared or tensor memory is in use by the other), then free
-    tensor_fence_before_sync();
-    __syncthreads();
-    cluster_sync_all();
-    if (warp == 1) {
-        tensor_fence_after_sync();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tensor_base), "r"(kColumns) : "memory");
-    }
-}
-
 int code_map(CUtensorMap* map, const void* codes, long long rows, int K, int box_rows) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return cudaErrorNotSupported;
@@ -546,30 +363,6 @@ int launch(const Call& c, cudaStream_t stream) {
     return code ? code : tau_launch_status();
 }
 
-template <typename TOut, bool Gated>
-int launch_pairs(const Call& c, cudaStream_t stream) {
-    static bool ready[64] = {};
-    int device = 0;
-    cudaError_t status = cudaGetDevice(&device);
-    if (status != cudaSuccess) return static_cast<int>(status);
-    if (device >= 64 || !ready[device]) {
-        status = cudaFuncSetAttribute(gemm8_tc_pair_kernel<TOut, Gated>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_shared_bytes());
-        if (status != cudaSuccess) return static_cast<int>(status);
-        if (device < 64) ready[device] = true;
-    }
-    CUtensorMap input_map, weight_map;
-    int code = code_map(&input_map, c.x, c.M, c.K, 128);
-    if (!code) code = code_map(&weight_map, c.w, c.N, c.K, 128);
-    if (code) return code;
-    const long long tiles = static_cast<long long>((c.N + kPairFeatures - 1) / kPairFeatures) * ((c.M + kPairTokens - 1) / kPairTokens);
-    if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
-    const int wide = (c.out_stride * static_cast<long long>(sizeof(TOut))) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15) == 0;
-    const unsigned pairs = static_cast<unsigned>(tiles < c.sms / 2 ? tiles : c.sms / 2);
-    code = tau_launch_clusters(2, gemm8_tc_pair_kernel<TOut, Gated>, dim3(2 * pairs), dim3(kPairThreads), pair_shared_bytes(), stream, input_map, weight_map, c.x_scales, c.w_scales, c.bias,
-                               static_cast<TOut*>(c.out), c.M, c.N, c.K, c.out_stride, wide, c.gate_limit);
-    return code ? code : tau_launch_status();
-}
-
 template <int BN>
 int launch_typed(int out_dtype, int gated, const Call& c, cudaStream_t stream) {
     if (gated) return launch<BN, bf16, true>(c, stream);
@@ -586,34 +379,30 @@ TAU_EXPORT int tau_gemm8_tc_status() {
     return flag;
 }
 
-// x codes [M, K] with scales [blocks][M]; w codes [N, K] with scales [blocks of N][blocks].  `features`: 64, 128 or 256 to a tile of 128 tokens, 512: tiles of 256 x 256 on pairs of SMs;
-// `ranges`: 1 to 8 ranges of K to a tile (1 on pairs).  0: chosen.
+// x codes [M, K] with scales [blocks][M]; w codes [N, K] with scales [blocks of N][blocks].  `features`: 128 or 256 to a tile of 128 tokens; `ranges`: 1 to 8 ranges of K to a
+// tile.  0: chosen.
 TAU_EXPORT int tau_gemm8_tc(int out_dtype, const void* x, const float* x_scales, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K, long long out_stride,
                             int gated, float gate_limit, int features, int ranges, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !x_scales || !w || !w_scales || !out || K <= 0 || (K & 15) || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
-        (out_dtype != TAU_BF16 && out_dtype != TAU_F32) || (gated && ((N & 15) || out_dtype != TAU_BF16)) || (features != 0 && features != 64 && features != 128 && features != 256 && features != 512) ||
+        (out_dtype != TAU_BF16 && out_dtype != TAU_F32) || (gated && ((N & 15) || out_dtype != TAU_BF16)) || (features != 0 && features != 128 && features != 256) ||
         ranges < 0 || ranges > kMostRanges)
         return cudaErrorInvalidValue;
     int device = 0, sms = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return cudaErrorInvalidValue;
     const int k_blocks = (K + BK - 1) / BK, token_tiles = (M + BM - 1) / BM;
     auto tiles = [&](int bn) { return static_cast<long long>((N + bn - 1) / bn) * token_tiles; };
-    const Call pairs = {x, x_scales, w, w_scales, bias, out, M, N, K, out_stride, 1, sms, gate_limit};
-    if (features == 512) {
-        if (gated) return launch_pairs<bf16, true>(pairs, static_cast<cudaStream_t>(stream));
-        if (out_dtype == TAU_BF16) return launch_pairs<bf16, false>(pairs, static_cast<cudaStream_t>(stream));
-        return launch_pairs<float, false>(pairs, static_cast<cudaStream_t>(stream));
-    }
-    if (features == 0) features = tiles(256) >= sms ? 256 : tiles(128) * 4 >= sms ? 128 : 64;
+    // Wide tiles where they give three of five SMs work (64 x 4,096 x 24,576: 96 wide tiles 23 us, 192 narrow ones 29) or where narrow ones would take a second round (512 x 4,096 x
+    // 6,144: 22 and 30).  Else narrow ones, K cut into ranges of four blocks and more as long as their clusters fit the machine at once, whose groups of SMs hold about 72 clusters of two,
+    // 32 of four and 12 of eight (64 x 12,288 x 4,096: 32 tiles in four ranges 16 us, in two 23, in one 38; 333 x 2,000 x 1,500: 36 tiles in two ranges 10 us, in four 16).
+    if (features == 0) features = tiles(256) * 5 >= sms * 3 || tiles(128) > sms ? 256 : 128;
     if (ranges == 0) {
-        ranges = 1;
-        while (ranges < kMostRanges && tiles(features) * (ranges + 1) <= sms && (ranges + 1) * 2 <= k_blocks) ++ranges;
+        const long long n = tiles(features);
+        ranges = n <= 12 && k_blocks >= 32 ? 8 : n <= 32 && k_blocks >= 16 ? 4 : n <= 72 && k_blocks >= 8 ? 2 : 1;
     }
     if (ranges > k_blocks) ranges = k_blocks;
     const Call call = {x, x_scales, w, w_scales, bias, out, M, N, K, out_stride, ranges, sms, gate_limit};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (features == 256) return launch_typed<256>(out_dtype, gated, call, s);
-    if (features == 128) return launch_typed<128>(out_dtype, gated, call, s);
-    return launch_typed<64>(out_dtype, gated, call, s);
+    return launch_typed<128>(out_dtype, gated, call, s);
 }

@@ -1107,8 +1107,11 @@ def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
                _stream_handle()), "gemm8_simt")
 
 
-SKINNY8_FUSED_ROWS = 8      # up to here the skinny kernel quantises the activations itself
+SKINNY8_FUSED_ROWS = 8      # up to here the skinny kernel can quantise the activations itself ...
+SKINNY8_FUSED_WEIGHT = 8 << 20   # ... and does where the weight is small: a launch less (1 x 1,024 x 4,096 2.8 us against 2.1 and 1.3), but each block quantises for itself (8 x
+                            # 4,096 x 6,144 8.6 us against 6.2 and 1.4, 24,576 26.9 against 22.4 and 1.4)
 SKINNY8_MAX_ROWS = 32       # what it accepts quantised
+SKINNY8_SMALL_ROWS = 16     # up to here it beats the tensor-core product where the weight is small (16 x 1,024 x 4,096 2.5 us against 5.2; 16 x 4,096 x 24,576 30 against 27)
 
 
 def gemm8_skinny(values, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
@@ -1121,7 +1124,7 @@ def gemm8_skinny(values, x_scales, codes, scales, bias, out, gated: bool = False
 
 
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
-    """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (64, 128, 256; 0: by the number of tiles) with K cut into `ranges`
+    """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 256; 0: by the number of tiles) with K cut into `ranges`
     (1 to 8; 0: as many as leave no SM without work)."""
     rows, depth = x_codes.shape
     run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
@@ -1145,10 +1148,11 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
         gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
         run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
         return _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
-    if rows <= SKINNY8_FUSED_ROWS and values.dtype == torch.bfloat16:
+    small = codes.numel() <= SKINNY8_FUSED_WEIGHT
+    if small and rows <= SKINNY8_FUSED_ROWS and values.dtype == torch.bfloat16:
         return gemm8_skinny(values, None, codes, scales, bias, out, gated, limit)
     x_codes, x_scales = quantize_rows(values)
-    if rows <= SKINNY8_FUSED_ROWS:
+    if rows <= SKINNY8_FUSED_ROWS or (small and rows <= SKINNY8_SMALL_ROWS):
         return gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated, limit)
     gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated, limit)
 
