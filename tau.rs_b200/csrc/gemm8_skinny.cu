@@ -120,30 +120,51 @@ gemm8_skinny_kernel(const void* __restrict__ x_any, long long x_stride, const fl
             held[2 * p + 1] = live ? __ldg(reinterpret_cast<const uint4*>(row + column + 64 * p) + 1) : zero;
         }
     };
-    if constexpr (!Codes) fetch(0);
+    // Quantised rows: the next chunk's codes and scales likewise.
+    uint4 code_next[NB][2];
+    float factor_next[NB][2];
+    auto fetch_codes = [&](int index) {
+        const uint8_t* x = static_cast<const uint8_t*>(x_any);
+        const int block = warp + index * kWarps;
+        const bool there = index < n_chunks;
+        const float w_scale = there ? __ldg(w_scale_row + block) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int token = j * 8 + g;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int column = block * kChunk + 64 * p + t * 16;
+                code_next[j][p] = there && token < M && column < K ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(token) * K + column)) : zero;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) factor_next[j][h] = there && j * 8 + 2 * t + h < M ? __ldg(x_scales + static_cast<size_t>(block) * M + j * 8 + 2 * t + h) * w_scale : 0.0f;
+        }
+    };
+    if constexpr (Codes) fetch_codes(0);
+    else fetch(0);
     for (int index = 0; index < n_chunks; ++index) {
         copy_async_wait<kDepth - 2>();      // chunk `index` has landed, and every lane is done with the slot that is written next
         __syncwarp();
         issue(index + kDepth - 1);
-        const int block = warp + index * kWarps;
-        const float w_scale_here = w_scale;
-        if (index + 1 < n_chunks) w_scale = w_scale_row[block + kWarps];
         unsigned codes[NB][8];
         float factor[NB][2];      // of tokens 2t and 2t + 1
         if constexpr (Codes) {
-            const uint8_t* x = static_cast<const uint8_t*>(x_any);
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
-                const int token = j * 8 + g;
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    const int column = block * kChunk + 64 * p + t * 16;
-                    *reinterpret_cast<uint4*>(&codes[j][4 * p]) = token < M && column < K ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(token) * K + column)) : zero;
+                    codes[j][4 * p] = code_next[j][p].x;
+                    codes[j][4 * p + 1] = code_next[j][p].y;
+                    codes[j][4 * p + 2] = code_next[j][p].z;
+                    codes[j][4 * p + 3] = code_next[j][p].w;
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) factor[j][h] = j * 8 + 2 * t + h < M ? __ldg(x_scales + static_cast<size_t>(block) * M + j * 8 + 2 * t + h) * w_scale_here : 0.0f;
+                factor[j][0] = factor_next[j][0];
+                factor[j][1] = factor_next[j][1];
             }
+            fetch_codes(index + 1);
         } else {
+            const float w_scale_here = w_scale;
+            if (index + 1 < n_chunks) w_scale = w_scale_row[warp + (index + 1) * kWarps];
             const float scale = quantize_chunk(held, codes[0]);
             fetch(index + 1);
 #pragma unroll

@@ -4,7 +4,7 @@
 //
 // The scales change every 128 columns of K, so the accumulator in tensor memory holds one such block at a time (four tcgen05.mma of kind f8f6f4, 32 columns each)
 // and the sums over blocks are kept in registers: four warps for each 64 features read a block's sums with tcgen05.ld and add them times both scales, while
-// the next block's products fill the other accumulator.  Rows (tokens) are the lanes of tensor memory and features its columns, so a thread's factor
+// the next blocks' products fill the other accumulators (two of 256 features, four of 128).  Rows (tokens) are the lanes of tensor memory and features its columns, so a thread's factor
 // is one number for each 128 features: 64 multiply-adds a thread and block, 256 on each quarter of an SM, against the 512 clocks that the products of a 128 x 256 block take.
 //
 // Operands come by TMA (128-byte swizzle, no multicast): a stage is 128 bytes of K of 128 rows of x and BN of w.  One warp asks for tiles, one issues products,
@@ -29,8 +29,8 @@ constexpr int kMostRanges = 8;
 struct Shared {
     uint64_t full[8];
     uint64_t empty[8];
-    uint64_t sums_full[2];
-    uint64_t sums_empty[2];
+    uint64_t sums_full[4];
+    uint64_t sums_empty[4];
     uint32_t tensor_memory_base;
     int abort_flag;
 };
@@ -74,48 +74,63 @@ __device__ __forceinline__ void add_block(uint32_t address, float factor, float 
     }
 }
 
-// Stores eight neighbouring results of a row, those below `left` of them; `wide`: rows are on borders of eight results.
+// Stores eight neighbouring results of a row, those below `left` of them; `border`: rows (and every eighth result) begin on so many bytes, up to 16.
 template <typename TOut>
-__device__ __forceinline__ void store_eight(TOut* target, const float (&v)[8], int left, bool wide) {
-    if (wide && left >= 8) {
-        if constexpr (sizeof(TOut) == 2) {
-            *reinterpret_cast<uint4*>(target) = make_uint4(pack_bf16_pair(v[0], v[1]), pack_bf16_pair(v[2], v[3]), pack_bf16_pair(v[4], v[5]), pack_bf16_pair(v[6], v[7]));
-        } else {
+__device__ __forceinline__ void store_eight(TOut* target, const float (&v)[8], int left, int border) {
+    if constexpr (sizeof(TOut) == 2) {
+        const unsigned words[4] = {pack_bf16_pair(v[0], v[1]), pack_bf16_pair(v[2], v[3]), pack_bf16_pair(v[4], v[5]), pack_bf16_pair(v[6], v[7])};
+        if (left >= 8 && border >= 4) {
+            if (border == 16) {
+                *reinterpret_cast<uint4*>(target) = make_uint4(words[0], words[1], words[2], words[3]);
+            } else if (border == 8) {
+                reinterpret_cast<uint2*>(target)[0] = make_uint2(words[0], words[1]);
+                reinterpret_cast<uint2*>(target)[1] = make_uint2(words[2], words[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) reinterpret_cast<unsigned*>(target)[i] = words[i];
+            }
+            return;
+        }
+    } else if (left >= 8 && border >= 8) {
+        if (border == 16) {
             reinterpret_cast<float4*>(target)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4*>(target)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) target[i] = from_float<TOut>(v[i]);
+            for (int i = 0; i < 4; ++i) reinterpret_cast<float2*>(target)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+        }
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left) target[i] = from_float<TOut>(v[i]);
 }
 
 // Eight or, gated, sixteen sums of a row from feature `feature` on, finished and stored.
 template <typename TOut, bool Gated>
-__device__ __forceinline__ void finish_row(const float* v, int feature, int N, const float* __restrict__ bias, TOut* row, bool wide, float gate_limit) {
+__device__ __forceinline__ void finish_row(const float* v, int feature, int N, const float* __restrict__ bias, TOut* row, int border, float gate_limit) {
     if constexpr (Gated) {      // 8 gate columns, their 8 up columns; both rounded as a product that is not gated would store them
         float result[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) result[i] = gated_value(round_through<bf16>(v[i]), round_through<bf16>(v[8 + i]), gate_limit);
-        store_eight(row + (feature >> 1), result, N - feature > 0 ? 8 : 0, wide);      // N is a multiple of 16
+        store_eight(row + (feature >> 1), result, N - feature > 0 ? 8 : 0, border);      // N is a multiple of 16
     } else {
         float result[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) result[i] = v[i] + ((bias != nullptr && feature + i < N) ? bias[feature + i] : 0.0f);
-        store_eight(row + feature, result, N - feature, wide);
+        store_eight(row + feature, result, N - feature, border);
     }
 }
 
 template <int BN, typename TOut, bool Gated>
 __global__ void __launch_bounds__(threads(BN), 1)
 gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_constant__ CUtensorMap weight_map, const float* __restrict__ x_scales, const float* __restrict__ w_scales,
-                const float* __restrict__ bias, TOut* __restrict__ out, int M, int N, int K, long long out_stride, int ranges, int wide, float gate_limit) {
+                const float* __restrict__ bias, TOut* __restrict__ out, int M, int N, int K, long long out_stride, int ranges, int border, float gate_limit) {
     extern __shared__ uint8_t shared_raw[];
     Shared* shared = reinterpret_cast<Shared*>(shared_raw);
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + sizeof(Shared) + 1023) & ~uintptr_t(1023));
     constexpr uint32_t kStages = stages_of(BN), kInputBytes = BM * BK, kStageBytes = stage_bytes(BN);
-    constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;      // two accumulators
+    constexpr uint32_t kSlots = 512 / BN, kColumns = 512;      // all of tensor memory: two or four accumulators
     constexpr int kAdders = adders(BN), kThreads = threads(BN);
     constexpr int kPartialStride = BN + 4;                        // floats to a row of the sums that a cluster shares: 16-byte loads of neighbouring rows fall on different banks
     static_assert(BM * kPartialStride * 4 <= static_cast<int>(kStages * kStageBytes), "the shared sums must fit the stages");
@@ -132,7 +147,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
             barrier_init(&shared->full[s], 1);
             barrier_init(&shared->empty[s], 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (uint32_t a = 0; a < kSlots; ++a) {
             barrier_init(&shared->sums_full[a], 1);
             barrier_init(&shared->sums_empty[a], kAdders);
         }
@@ -198,7 +213,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
             const int range = item % ranges;
             const int count = k_blocks * (range + 1) / ranges - k_blocks * range / ranges;
             for (int i = 0; i < count; ++i, ++number) {
-                const uint32_t slot = number & 1u, use = number >> 1;
+                const uint32_t slot = number % kSlots, use = number / kSlots;
                 if (use > 0 && !warp_wait(&shared->sums_empty[slot], (use - 1) & 1u)) { alive = false; break; }
                 if (!warp_wait(&shared->full[stage], phase)) { alive = false; break; }
                 tensor_fence_after_sync();
@@ -237,7 +252,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
                 w_next[a] = a < count ? w_scale[a] : 0.0f;
             }
             for (int i = 0; i < count; ++i, ++number) {
-                const uint32_t slot = number & 1u, use = number >> 1;
+                const uint32_t slot = number % kSlots, use = number / kSlots;
                 const float factor = x_next[0] * w_next[0];
                 x_next[0] = x_next[1];
                 w_next[0] = w_next[1];
@@ -261,7 +276,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
                     constexpr int kStep = Gated ? 16 : 8;
 #pragma unroll
                     for (int c = 0; c < kPart; c += kStep)
-                        if (feature0 + c < N) finish_row<TOut, Gated>(sums + c, feature0 + c, N, bias, row, wide != 0, gate_limit);
+                        if (feature0 + c < N) finish_row<TOut, Gated>(sums + c, feature0 + c, N, bias, row, border, gate_limit);
                 }
             } else {
                 // One item to a block here.  The stages are free: every product has read them (the sums are complete) and no copy is left.
@@ -302,7 +317,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
                         sum[i] += part.x; sum[i + 1] += part.y; sum[i + 2] += part.z; sum[i + 3] += part.w;
                     }
                 }
-                finish_row<TOut, Gated>(sum, feature0 + c, N, bias, out + static_cast<size_t>(token0 + row) * out_stride, wide != 0, gate_limit);
+                finish_row<TOut, Gated>(sum, feature0 + c, N, bias, out + static_cast<size_t>(token0 + row) * out_stride, border, gate_limit);
             }
         }
         cluster_sync_all();      // nobody leaves while another still reads its sums
@@ -353,13 +368,14 @@ int launch(const Call& c, cudaStream_t stream) {
     if (code) return code;
     const long long tiles = static_cast<long long>((c.N + BN - 1) / BN) * ((c.M + BM - 1) / BM);
     if (tiles * c.ranges > 0x7fffffffll) return cudaErrorInvalidValue;
-    const int wide = (c.out_stride * static_cast<long long>(sizeof(TOut))) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 15) == 0;
+    const unsigned long long bits = static_cast<unsigned long long>(c.out_stride) * sizeof(TOut) | reinterpret_cast<uintptr_t>(c.out) | 16u;
+    const int border = static_cast<int>(bits & (~bits + 1));
     if (c.ranges > 1)
         code = tau_launch_clusters(c.ranges, gemm8_tc_kernel<BN, TOut, Gated>, dim3(static_cast<unsigned>(tiles * c.ranges)), dim3(threads(BN)), shared_bytes(BN), stream, input_map, weight_map,
-                                   c.x_scales, c.w_scales, c.bias, static_cast<TOut*>(c.out), c.M, c.N, c.K, c.out_stride, c.ranges, wide, c.gate_limit);
+                                   c.x_scales, c.w_scales, c.bias, static_cast<TOut*>(c.out), c.M, c.N, c.K, c.out_stride, c.ranges, border, c.gate_limit);
     else
         code = tau_launch(gemm8_tc_kernel<BN, TOut, Gated>, dim3(static_cast<unsigned>(tiles < c.sms ? tiles : c.sms)), dim3(threads(BN)), shared_bytes(BN), stream, input_map, weight_map, c.x_scales,
-                          c.w_scales, c.bias, static_cast<TOut*>(c.out), c.M, c.N, c.K, c.out_stride, 1, wide, c.gate_limit);
+                          c.w_scales, c.bias, static_cast<TOut*>(c.out), c.M, c.N, c.K, c.out_stride, 1, border, c.gate_limit);
     return code ? code : tau_launch_status();
 }
 
