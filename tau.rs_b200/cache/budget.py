@@ -33,11 +33,14 @@ def headroom(total_bytes: int) -> int:
 
 
 def kv_bytes_per_token(groups: Dict[str, Tuple[object, int]], element_bytes: int) -> int:
-    """Bytes that one cached position takes over all kv groups (keys and values of every cache layer)."""
+    """Bytes that one cached position takes over all kv groups (keys and values of every cache layer).  At one byte an element a position's share of
+    its page's scales is counted with it, rounded up."""
     total = 0
     for need, layers in groups.values():
         if need.kind == "kv":
             total += 2 * layers * need.n_kv_heads * need.head_dim * element_bytes
+            if element_bytes == 1:
+                total += -(-2 * layers * need.n_kv_heads * 4 // PAGE_TOKENS)
         elif need.kind == "rows":
             total += layers * need.row_width * element_bytes
     return total

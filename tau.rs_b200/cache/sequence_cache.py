@@ -55,6 +55,8 @@ class KVLayerView:
     group: str                # key of the step's page rows (`StepContext.page_rows[group]`)
     window: Optional[int]
     extra: Dict[str, object] = field(default_factory=dict)   # role -> view of what the block keeps beside this (`ScheduleEntry.extra_cache`)
+    key_scales: Optional[torch.Tensor] = None     # [pages, kv_heads] float32 where keys and values are held in 8 bits (float8_e4m3fn codes)
+    value_scales: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -72,8 +74,12 @@ class StateLayerView:
 
 
 class _KVGroup:
-    def __init__(self, need: CacheNeed, layers: int, pages: int, slots: int, pages_per_sequence: int, dtype, device):
+    def __init__(self, need: CacheNeed, layers: int, pages: int, slots: int, pages_per_sequence: int, dtype, device, eight_bit: bool = False):
         self.need, self.layers = need, layers
+        self.key_scales = self.value_scales = None
+        if eight_bit:
+            dtype = torch.float8_e4m3fn
+            self.key_scales, self.value_scales = (torch.ones((layers, pages, need.n_kv_heads), dtype=torch.float32, device=device) for _ in range(2))
         if need.kind == "rows":     # one row per position: the pages of a kv group without heads, and nothing beside them
             self.keys = torch.empty((layers, pages, PAGE_TOKENS, need.row_width), dtype=dtype, device=device)
             self.values = None
@@ -101,7 +107,8 @@ class _KVGroup:
     def bytes_per_token(self) -> int:
         if self.need.kind == "rows":
             return self.layers * self.need.row_width * self.keys.element_size()
-        return 2 * self.layers * self.need.n_kv_heads * self.need.head_dim * self.keys.element_size()
+        scales = 0 if self.key_scales is None else 2 * self.layers * self.need.n_kv_heads * 4 // PAGE_TOKENS      # a position's share of its page's scales, rounded down
+        return 2 * self.layers * self.need.n_kv_heads * self.need.head_dim * self.keys.element_size() + scales
 
 
 class _StateGroup:
@@ -110,15 +117,33 @@ class _StateGroup:
         self.state = torch.zeros((layers, slots, *need.state_shape), dtype=need.state_dtype, device=device)
 
 
+def check_cache_format(groups: Dict[str, Tuple[CacheNeed, int]], cache_format: str, dtype: torch.dtype) -> None:
+    if cache_format not in ("", "fp8"):
+        raise ValueError(f"unknown cache format {cache_format!r}; use fp8, or nothing for the run's dtype")
+    if not cache_format:
+        return
+    if dtype != torch.bfloat16:
+        raise ValueError(f"a cache in 8 bits serves bfloat16 runs; this one is in {dtype}")
+    for name, (need, _) in groups.items():
+        if need.kind in ("kv", "rows") and not need.eight_bit:
+            raise ValueError(f"cache group {name!r} cannot be held in 8 bits: its mixer reads it in the run's dtype")
+    if not any(need.kind == "kv" for need, _ in groups.values()):
+        raise ValueError("the model keeps no keys and values that could be held in 8 bits")
+
+
 class SequenceCache:
     """`groups`: name -> (`CacheNeed`, number of cache layers), as `DecoderModel.cache_groups()` gives it.
 
     `max_tokens` is the most tokens that live sequences may hold together, each
-    sequence's count rounded up to a multiple of `PAGE_TOKENS`.
+    sequence's count rounded up to a multiple of `PAGE_TOKENS`.  `cache_format` "fp8": keys and
+    values are held as e4m3 codes with a scale for each page and head (about half of the bytes);
+    refused unless every group that keeps something by position can be held so.
     """
 
     def __init__(self, groups: Dict[str, Tuple[CacheNeed, int]], max_tokens: int, max_sequence_tokens: int,
-                 dtype: torch.dtype, device, max_slots: Optional[int] = None):
+                 dtype: torch.dtype, device, max_slots: Optional[int] = None, cache_format: str = ""):
+        check_cache_format(groups, cache_format, dtype)
+        self.cache_format = cache_format
         if max_tokens <= 0:
             raise ValueError("the cache must hold at least one token")
         self.device, self.dtype = device, dtype
@@ -140,7 +165,8 @@ class SequenceCache:
         self.states: Dict[str, _StateGroup] = {}
         for name, (need, layers) in groups.items():
             if need.kind in ("kv", "rows"):
-                self.kv[name] = _KVGroup(need, layers, self.n_pages, self.n_slots, self.pages_per_sequence, dtype, device)
+                self.kv[name] = _KVGroup(need, layers, self.n_pages, self.n_slots, self.pages_per_sequence, dtype, device,
+                                          eight_bit=cache_format == "fp8")
             elif need.kind == "state":
                 self.states[name] = _StateGroup(need, layers, self.n_slots, device)
             else:
@@ -224,6 +250,8 @@ class SequenceCache:
             entry = self.kv[group]
             if entry.need.kind == "rows":
                 return RowsLayerView(entry.keys[layer], group, entry.need.window)
+            if entry.key_scales is not None:
+                return KVLayerView(entry.keys[layer], entry.values[layer], group, entry.need.window, key_scales=entry.key_scales[layer], value_scales=entry.value_scales[layer])
             return KVLayerView(entry.keys[layer], entry.values[layer], group, entry.need.window)
         return StateLayerView(self.states[group].state[layer])
 

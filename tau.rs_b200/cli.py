@@ -39,6 +39,10 @@ def build_parser() -> argparse.ArgumentParser:
     execution = parser.add_argument_group("Execution options")
     execution.add_argument("--optimize-kernel", default="true", choices=["true", "false"],
                            help="Prefer optimized kernels. [default: true] false: the plain kernels that the others are checked against.")
+    execution.add_argument("--weights", default="auto", choices=["auto", "fp8"],
+                           help="How the products' weights are held. [default: auto] auto: the run's dtype; fp8: 8 bits with a scale for each 128 x 128 (BF16 runs).")
+    execution.add_argument("--cache", default="auto", choices=["auto", "fp8"],
+                           help="How cached keys and values are held. [default: auto] auto: the run's dtype; fp8: 8 bits with a scale for each 64 positions and head (BF16 runs).")
     execution.add_argument("--cuda-graph", default="full", choices=["none", "full"], help="CUDA graph policy for decode steps. [default: full]")
     execution.add_argument("--attention-block-size", type=int, default=None, choices=[32, 64, 128, 256], metavar="32|64|128|256",
                            help="Context tokens per block of decode attention. [default: chosen from the batch and the context]")
@@ -163,7 +167,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     from .csrc import kernels
 
     kernels.prefer_optimized(args.optimize_kernel == "true")
-    model = load_model(args.model, args.dtype, args.device)
+    model = load_model(args.model, args.dtype, args.device, weights=args.weights)
     settings: GenerationConfig = model.generation_config
     limit = args.max_tokens if args.max_tokens is not None else settings.max_new_tokens
     stop = _ids(args.stop_ids) if args.stop_ids is not None else settings.eos_token_ids
@@ -171,7 +175,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     if cache_tokens is None:
         needs = sorted((-(-(len(prompt) + limit) // 64) * 64 for prompt in prompts), reverse=True)
         cache_tokens = max(64, sum(needs[: args.max_batch]))
-    engine = Engine(model, cache_tokens)
+    engine = Engine(model, cache_tokens, cache_format="fp8" if args.cache == "fp8" else "")
     engine.use_graphs = engine.use_graphs and args.cuda_graph == "full"
     engine.attention_block_size = args.attention_block_size
     select = Sampler(SamplingParams(args.temperature, args.seed))   # the object, not its method: the loop then decodes one step ahead

@@ -9,7 +9,7 @@ kind of token mixer and its own state).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Optional, Tuple
 
 
@@ -53,6 +53,7 @@ class AttentionSpec:
     position: Optional[PositionSpec] = None
     window: Optional[int] = None
     kind: str = "attention"
+    weight_format: str = ""      # "fp8": the products' weights are held in 8 bits (`with_weight_format`)
 
 
 @dataclass(frozen=True)
@@ -71,6 +72,7 @@ class SwiGLUSpec:
     activation: str = "silu"
     limit: float = 0.0
     wide_result: bool = False
+    weight_format: str = ""      # as in `AttentionSpec`
 
 
 @dataclass(frozen=True)
@@ -482,3 +484,26 @@ class ModelSpec:
     logit_scale: float = 1.0
     # With a cap c > 0 the logits l leave as c * tanh(l / c).
     logit_cap: float = 0.0
+
+
+def with_weight_format(spec: "ModelSpec", weight_format: str) -> "ModelSpec":
+    """The same model with the weights of its attention and feed-forward products held in `weight_format` ("" as the run's dtype, or "fp8": e4m3 codes with a scale for each
+    128 x 128).  The embedding and the head stay as they are.  Refused where a layer has a mixer or a feed-forward whose products are not served in 8 bits."""
+    if not weight_format:
+        return spec
+    if weight_format != "fp8":
+        raise ValueError(f"unknown weight format {weight_format!r}; use fp8")
+
+    def changed(part):
+        if part is None:
+            return None
+        if not hasattr(part, "weight_format"):
+            raise ValueError(f"weights in 8 bits are served by attention and gated feed-forwards; a layer of {spec.architecture} has a part of kind {part.kind!r}")
+        return replace(part, weight_format=weight_format)
+
+    blocks = []
+    for block in spec.blocks:
+        if not hasattr(block, "mixer"):
+            raise ValueError(f"weights in 8 bits are not served by blocks of kind {getattr(block, 'kind', '?')!r}")
+        blocks.append(replace(block, mixer=changed(block.mixer), feed_forward=changed(block.feed_forward)))
+    return replace(spec, blocks=tuple(blocks))

@@ -1217,6 +1217,13 @@ def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales,
                rotary_dim, _stream_handle()), "cache8_store")
 
 
+def attention8_queries(projected, queries, q_weight, eps: float, cos, sin, rotary_dim: int, step, n_heads: int, head_dim: int) -> None:
+    """The queries alone, normalised per head and rotated: what a run needs that reads keys and values which another run stored."""
+    nothing = torch.empty((0, 1, PAGE_TOKENS, head_dim), dtype=projected.dtype, device=projected.device)
+    places = torch.zeros((step.n_seqs, 1), dtype=torch.int32, device=projected.device)
+    attention_prepare(projected, queries, nothing, nothing, False, q_weight, None, eps, cos, sin, rotary_dim, step.positions, step.token_seq, places, n_heads, 1, head_dim)
+
+
 def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int = 0, sparse: bool = False):
     """The pages of the step's sequences as the bfloat16 values that they stand for: keys and values [sequences * stride, n_kv_heads, 64, head_dim], page `j` of
     sequence `i` at `i * stride + j`; zeros where a sequence has no position.  `sparse`: pages that no query of the step sees (behind the sequence's end, or wholly before

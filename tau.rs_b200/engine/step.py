@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from ..cache.allocator import CacheFull
-from ..cache.sequence_cache import PAGE_TOKENS, SequenceCache, pages_for
+from ..cache.sequence_cache import PAGE_TOKENS, SequenceCache, check_cache_format, pages_for
 from .batch import StepContext, StepEntry, StepLayout, fill_step, step_views
 from .staging import PinnedRing
 
@@ -34,10 +34,12 @@ class Engine:
     """A model, its cache and the step function over both."""
 
     def __init__(self, model, max_tokens: int, max_sequence_tokens: Optional[int] = None, max_slots: Optional[int] = None,
-                 headroom_bytes: Optional[int] = None):
+                 headroom_bytes: Optional[int] = None, cache_format: str = ""):
         """`max_tokens` sizes the cache: the most tokens that live sequences hold together, each rounded up to 64.
         On a CUDA device a cache that does not fit the free memory (less `headroom_bytes` for activations; default: the
-        larger of 2 GiB and 1/32 of the device) is refused with `CacheDoesNotFit` before anything is allocated."""
+        larger of 2 GiB and 1/32 of the device) is refused with `CacheDoesNotFit` before anything is allocated.
+        `cache_format` "fp8" holds keys and values in 8 bits (see `SequenceCache`); a model that cannot work on them so is refused."""
+        check_cache_format(model.cache_groups(), cache_format, model.dtype)
         self.model = model
         self.device = torch.device(model.device)
         limit = model.spec.max_positions
@@ -50,8 +52,8 @@ class Engine:
             free_bytes += torch.cuda.memory_reserved(self.device) - torch.cuda.memory_allocated(self.device)   # what torch holds unused
             pages = -(-max_tokens // PAGE_TOKENS)
             check_fits(model.cache_groups(), max_tokens, min(pages, max_slots) if max_slots else pages,
-                       torch.empty((), dtype=model.dtype).element_size(), free_bytes, total_bytes, headroom_bytes)
-        self.cache = SequenceCache(model.cache_groups(), max_tokens, limit, model.dtype, self.device, max_slots)
+                       1 if cache_format else torch.empty((), dtype=model.dtype).element_size(), free_bytes, total_bytes, headroom_bytes)
+        self.cache = SequenceCache(model.cache_groups(), max_tokens, limit, model.dtype, self.device, max_slots, cache_format)
         self._ring: Optional[PinnedRing] = None
         self._graphs: Dict = {}
         self._graph_stream = None
@@ -70,7 +72,7 @@ class Engine:
         if self.attention_block_size:
             bucket = 1 << max(0, (max_len - 1).bit_length())   # as the graphs are keyed: a power of two of positions
             return max(1, min(-(-bucket // self.attention_block_size), MAX_DECODE_SPLITS))
-        return self.model.decode_splits(n_seqs, max_len)
+        return self.model.decode_splits(n_seqs, max_len, eight_bit=bool(self.cache.cache_format))
 
     def ring(self, ints: int) -> PinnedRing:
         """The pinned staging ring, grown if a step needs more room."""

@@ -33,9 +33,9 @@ class Attention(Mixer):
         self.q_width, self.kv_width = q_width, kv_width
         self.qkv = StackedLinear(
             [(f"{prefix}.q_proj", q_width), (f"{prefix}.k_proj", kv_width), (f"{prefix}.v_proj", kv_width)],
-            spec.hidden, spec.bias, dtype, device,
+            spec.hidden, spec.bias, dtype, device, weight_format=spec.weight_format,
         )
-        self.out = StackedLinear([(f"{prefix}.o_proj", spec.hidden)], q_width, spec.bias, dtype, device)
+        self.out = StackedLinear([(f"{prefix}.o_proj", spec.hidden)], q_width, spec.bias, dtype, device, weight_format=spec.weight_format)
         self.q_norm = self.k_norm = None
         if spec.qk_norm is not None:
             if spec.qk_norm.width != spec.head_dim:
@@ -54,7 +54,10 @@ class Attention(Mixer):
         self._children = [part for part in (self.qkv, self.out, self.q_norm, self.k_norm, self.position) if part is not None]
 
     def cache_need(self):
-        return CacheNeed("kv", n_kv_heads=self.spec.n_kv_heads, head_dim=self.spec.head_dim, window=self.spec.window)
+        return CacheNeed("kv", n_kv_heads=self.spec.n_kv_heads, head_dim=self.spec.head_dim, window=self.spec.window, eight_bit=True)
+
+    def bytes_read_per_step(self, dtype) -> int:
+        return super().bytes_read_per_step(dtype) - self.qkv.bytes_saved_per_step() - self.out.bytes_saved_per_step()
 
     def decode_blocks(self) -> int:
         """Blocks that the decode kernel launches per sequence and context split."""
@@ -92,6 +95,8 @@ class Attention(Mixer):
             None if self.position is None else self.position.sin,
             0 if self.position is None else spec.position.rotary_dim,
         )
+        if cache.key_scales is not None:
+            return self.out.forward(self._forward_eight_bit(projected, context, step, cache, pages, writes_cache, prepare))
         # One token per sequence in bfloat16: norm, rotation, cache write and attention are one kernel.
         if kernels.attention_decode_fused(projected, cache.keys, cache.values, context, step, pages, writes_cache, *prepare,
                                           spec.n_heads, spec.n_kv_heads, spec.head_dim, spec.softmax_scale, spec.window or 0):
@@ -102,3 +107,18 @@ class Attention(Mixer):
         kernels.attention(queries, cache.keys, cache.values, context, step, pages, spec.n_heads, spec.n_kv_heads, spec.head_dim,
                           spec.softmax_scale, spec.window or 0)
         return self.out.forward(context)
+
+    def _forward_eight_bit(self, projected, context, step, cache, pages, writes_cache: bool, prepare):
+        """The same over pages held in 8 bits: norm, rotation and the store, or the queries alone where another run stored keys and values, then attention."""
+        spec = self.spec
+        q_weight, k_weight, eps, cos, sin, rotary_dim = prepare
+        queries = torch.empty_like(context)
+        held = (cache.keys, cache.values, cache.key_scales, cache.value_scales)
+        if writes_cache:
+            keys = projected[:, self.q_width : self.q_width + self.kv_width].unflatten(1, (spec.n_kv_heads, spec.head_dim))
+            values = projected[:, self.q_width + self.kv_width :].unflatten(1, (spec.n_kv_heads, spec.head_dim))
+            kernels.cache8_store(keys, values, *held, step, pages, prepare=(projected, queries, q_weight, k_weight, eps, cos, sin, rotary_dim, spec.n_heads))
+        else:
+            kernels.attention8_queries(projected, queries, q_weight, eps, cos, sin, rotary_dim, step, spec.n_heads, spec.head_dim)
+        kernels.attention8(queries, *held, context, step, pages, spec.n_heads, spec.n_kv_heads, spec.head_dim, spec.softmax_scale, spec.window or 0)
+        return context

@@ -27,7 +27,9 @@ class CacheNeed:
     position 0), so that what lies before the newest chunk need not be kept.  `kind == "state"`:
     one tensor of `state_shape` and `state_dtype` for each sequence, zero when the sequence
     starts, whatever its length.  `keep_first` (beside a window): the first that many positions
-    are read by every query and kept as long as the sequence lives.
+    are read by every query and kept as long as the sequence lives.  `eight_bit` (kind "kv"): the
+    mixer can also work on keys and values held in 8 bits with a scale for each page and head, if the
+    engine keeps its cache so.
     """
 
     kind: str
@@ -39,6 +41,7 @@ class CacheNeed:
     row_width: int = 0
     chunk: Optional[int] = None
     keep_first: int = 0
+    eight_bit: bool = False
 
 
 class Pending(tuple):

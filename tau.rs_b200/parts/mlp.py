@@ -29,14 +29,20 @@ class SwiGLU(FeedForward):
         self.result_dtype = torch.float32 if getattr(spec, "wide_result", False) else None
         # Where the gated product exists (bfloat16, aligned sizes; its epilogue is SiLU or the clamped gate) gate and up rows are interleaved for it and
         # the activation is its epilogue; otherwise the two are stacked and the activation is a kernel of its own.
-        self.fused = self.activation != "relu" and kernels.gated_fits(spec.hidden, spec.intermediate, dtype)
+        self.weight_format = getattr(spec, "weight_format", "")
+        fits = kernels.linear8_fits(spec.hidden, spec.intermediate, dtype, gated=True) if self.weight_format else kernels.gated_fits(spec.hidden, spec.intermediate, dtype)
+        self.fused = self.activation != "relu" and fits
         gate, up, down = (getattr(spec, key, default) for key, default in (("gate_name", "gate_proj"), ("up_name", "up_proj"), ("down_name", "down_proj")))
         suffix = getattr(spec, "weight_suffix", ".weight")
         self.gate_up = StackedLinear(
             [(f"{prefix}.{gate}", spec.intermediate), (f"{prefix}.{up}", spec.intermediate)],
             spec.hidden, False, dtype, device, interleave=kernels.GATE_GROUP if self.fused else 0, weight_suffix=suffix,
+            weight_format=self.weight_format,
         )
-        self.down = StackedLinear([(f"{prefix}.{down}", spec.hidden)], spec.intermediate, False, dtype, device, weight_suffix=suffix)
+        self.down = StackedLinear([(f"{prefix}.{down}", spec.hidden)], spec.intermediate, False, dtype, device, weight_suffix=suffix, weight_format=self.weight_format)
+
+    def bytes_read_per_step(self, dtype) -> int:
+        return super().bytes_read_per_step(dtype) - self.gate_up.bytes_saved_per_step() - self.down.bytes_saved_per_step()
 
     def tensor_specs(self):
         return {**self.gate_up.tensor_specs(), **self.down.tensor_specs()}

@@ -260,7 +260,7 @@ def test_the_store_reads_keys_and_values_inside_wider_rows_and_leaves_other_page
         assert bool((cache.keys[page].view(torch.uint8) == 0x7F).all()) and bool(cache.key_scales[page].isnan().all())
 
 
-@pytest.mark.parametrize("n_heads, n_kv_heads, dim, rotary, normed", [(4, 2, 32, 32, True), (6, 2, 80, 40, True), (8, 8, 128, 128, True), (2, 1, 64, 0, False), (9, 3, 256, 256, False)])
+@pytest.mark.parametrize("n_heads, n_kv_heads, dim, rotary, normed", [(4, 2, 32, 32, True), (6, 2, 80, 40, True), (8, 8, 128, 128, True), (2, 1, 64, 0, False), (9, 3, 256, 256, False), (4, 4, 64, 64, True), (4, 2, 96, 96, True), (2, 2, 256, 256, True)])
 def test_preparing_and_storing_equals_the_prepare_kernel_and_a_store(n_heads, n_kv_heads, dim, rotary, normed):
     runs = [(0, 75), (30, 1), (64, 2), (100, 60)]
     tokens = sum(new for _, new in runs)

@@ -102,3 +102,116 @@ def test_attention_refuses(change):
     with pytest.raises(kernels.KernelError):
         kernels.attention8(operands["queries"], operands["key_pages"], operands["value_pages"], operands["key_scales"], operands["value_scales"], operands["out"], operands["step"],
                            operands["page_rows"], operands["heads"], operands["kv_heads"], operands["head_dim"], 1.0, operands["window"])
+
+
+# ---- configuration, cache and budget: host logic ---------------------------------------------------------------------------------
+def tiny_spec(which="B"):
+    import tiny_configs
+    from tau_rs_b200.config.registry import architecture_for
+
+    entry = architecture_for(tiny_configs.CONFIGS[which])
+    return entry.build_spec(entry.parse_config(tiny_configs.CONFIGS[which]))
+
+
+def test_a_model_names_the_parts_whose_weights_are_held_in_8_bits():
+    from tau_rs_b200 import DecoderModel
+    from tau_rs_b200.config.specs import with_weight_format
+
+    spec = tiny_spec("B")
+    assert with_weight_format(spec, "") is spec
+    changed = with_weight_format(spec, "fp8")
+    assert all(block.mixer.weight_format == block.feed_forward.weight_format == "fp8" for block in changed.blocks) and spec.blocks[0].mixer.weight_format == ""
+    model = DecoderModel(changed, torch.bfloat16, "cpu")
+    assert model.tensor_specs() == DecoderModel(spec, torch.bfloat16, "cpu").tensor_specs()      # the folder is the same
+    block = model.blocks[0]
+    assert block.feed_forward.fused and block.mixer.qkv.weight_format == block.feed_forward.down.weight_format == "fp8"
+    # 96 wide, 8 heads of 32 over one, 224 inner: bytes of codes and scales in the place of two bytes an element.
+    held = [(320, 96), (96, 256), (448, 96), (96, 224)]
+    saved = sum(rows * columns - 4 * -(-rows // 128) * -(-columns // 128) for rows, columns in held)
+    plain = DecoderModel(spec, torch.bfloat16, "cpu")
+    assert plain.weight_bytes() - model.weight_bytes() == 3 * saved
+    with pytest.raises(ValueError, match="fp4"):
+        with_weight_format(spec, "fp4")
+
+
+def test_weights_in_8_bits_are_refused_where_they_are_not_served():
+    import fasesun_models
+    from tau_rs_b200 import DecoderModel
+    from tau_rs_b200.api import random_model
+    from tau_rs_b200.config.errors import UnsupportedDType
+    from tau_rs_b200.config.specs import with_weight_format
+    import tiny_configs
+
+    with pytest.raises(ValueError, match="multiples of 16"):
+        DecoderModel(with_weight_format(tiny_spec("C"), "fp8"), torch.bfloat16, "cpu")      # 120 wide
+    with pytest.raises(ValueError, match="8 bits"):
+        DecoderModel(with_weight_format(tiny_spec("B"), "fp8"), torch.float32, "cpu")
+    with pytest.raises(UnsupportedDType, match="float32"):
+        random_model(tiny_configs.TINY_B, dtype="float32", device=torch.device("cpu"), weights="fp8")
+    with pytest.raises(UnsupportedDType, match="fp16"):
+        random_model(tiny_configs.TINY_B, device=torch.device("cpu"), weights="fp16")
+    with pytest.raises(UnsupportedDType, match="latent_attention|served"):
+        random_model(fasesun_models.MIXED, device=torch.device("cpu"), weights="fp8")
+
+
+def test_a_cache_in_8_bits_holds_codes_and_scales():
+    from tau_rs_b200 import SequenceCache
+    from tau_rs_b200.parts.base import CacheNeed
+
+    groups = {"attention": (CacheNeed("kv", n_kv_heads=2, head_dim=32, eight_bit=True), 3), "state": (CacheNeed("state", state_shape=(4,)), 1)}
+    cache = SequenceCache(groups, 64 * 5, 1024, torch.bfloat16, "cpu", cache_format="fp8")
+    view = cache.layer_view("attention", 1)
+    assert view.keys.dtype == view.values.dtype == CODES and view.keys.shape == (5, 2, 64, 32) and view.key_scales.shape == view.value_scales.shape == (5, 2)
+    assert view.key_scales.dtype == torch.float32 and cache.layer_view("attention", 2).key_scales.data_ptr() != view.key_scales.data_ptr()
+    assert cache.bytes_per_token() == 2 * 3 * 2 * 32 + 2 * 3 * 2 * 4 // 64
+    wide = SequenceCache(groups, 64 * 5, 1024, torch.bfloat16, "cpu")
+    assert wide.layer_view("attention", 1).key_scales is None and wide.layer_view("attention", 1).keys.dtype == torch.bfloat16
+    slot = cache.open()
+    cache.reserve(slot, 130)
+    cache.advance(slot, 130)
+    cache.check()
+
+
+@pytest.mark.parametrize("need, dtype, cache_format, message", [
+    (dict(kind="kv", n_kv_heads=2, head_dim=32), torch.bfloat16, "fp8", "run's dtype"),
+    (dict(kind="rows", row_width=32), torch.bfloat16, "fp8", "run's dtype"),
+    (dict(kind="state", state_shape=(4,)), torch.bfloat16, "fp8", "no keys"),
+    (dict(kind="kv", n_kv_heads=2, head_dim=32, eight_bit=True), torch.float32, "fp8", "bfloat16 runs"),
+    (dict(kind="kv", n_kv_heads=2, head_dim=32, eight_bit=True), torch.bfloat16, "int8", "unknown"),
+])
+def test_caches_in_8_bits_are_refused_where_they_are_not_served(need, dtype, cache_format, message):
+    from tau_rs_b200 import SequenceCache
+    from tau_rs_b200.parts.base import CacheNeed
+
+    with pytest.raises(ValueError, match=message):
+        SequenceCache({"g": (CacheNeed(**need), 1)}, 256, 256, dtype, "cpu", cache_format=cache_format)
+
+
+def test_the_budget_counts_a_byte_an_element_and_the_scales():
+    from tau_rs_b200.cache.budget import kv_bytes_per_token
+    from tau_rs_b200.parts.base import CacheNeed
+
+    groups = {"kv": (CacheNeed("kv", n_kv_heads=8, head_dim=128, eight_bit=True), 36)}
+    assert kv_bytes_per_token(groups, 2) == 2 * 36 * 8 * 128 * 2
+    assert kv_bytes_per_token(groups, 1) == 2 * 36 * 8 * 128 + 36      # 2 x 36 x 8 scales of 4 bytes to 64 positions
+
+
+def test_the_command_line_names_both_formats():
+    from tau_rs_b200.cli import build_parser
+
+    parser = build_parser()
+    assert parser.parse_args([]).weights == parser.parse_args([]).cache == "auto"
+    assert parser.parse_args(["--weights", "fp8", "--cache", "fp8"]).weights == "fp8"
+    with pytest.raises(SystemExit):
+        parser.parse_args(["--cache", "fp4"])
+
+
+def test_ranges_of_a_decode_over_8_bit_pages():
+    """The rule's corners: never more ranges than pages, one where sequences fill the machine, numbers just above a cluster's eight become eight."""
+    splits = kernels.decode8_splits
+    assert splits(1, 1, 8, 148) == 1 and splits(1, 64, 8, 148) == 1 and splits(1, 300, 8, 148) == 8 and splits(8, 2048, 8, 148) == 4
+    assert splits(64, 2048, 8, 148) == 1 and splits(40, 6000, 8, 148) == 2 and splits(2, 120000, 8, 148) == 37 and splits(4, 1000, 8, 148) == 8
+    for n_seqs in (1, 3, 17, 64, 500):
+        for length in (1, 65, 1000, 33000, 1 << 20):
+            found = splits(n_seqs, length, 8, 148)
+            assert 1 <= found <= 64 and found <= max(1, (1 << (length - 1).bit_length()) // 64)
