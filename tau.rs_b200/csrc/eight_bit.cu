@@ -330,16 +330,17 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
 
 // Pages of the step's sequences as the bfloat16 values that they stand for (exact: 4 significant bits times a power of two).
 // grid (page of a sequence, sequence, 2 n_kv_heads).  Positions that a sequence does not have are zeros; with `sparse` only pages that a query sees
-// are written at all, and positions that none sees are zeros: what a window left behind may be NaN, and a weight of zero would not hide that.
+// are written at all (and `places` gets the numbers that the pages have in the result), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of zero would not hide that.
 __global__ void __launch_bounds__(256)
 read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
-            bf16* __restrict__ keys, bf16* __restrict__ values, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
+            bf16* __restrict__ keys, bf16* __restrict__ values, int* __restrict__ places, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
             int page_stride, int n_kv_heads, int D, int window, int sparse) {
     grid_dependents_launch();
     grid_dependency_wait();
     const int page = blockIdx.x, seq = blockIdx.y;
     const bool is_key = static_cast<int>(blockIdx.z) < n_kv_heads;
     const int head = is_key ? blockIdx.z : blockIdx.z - n_kv_heads;
+    if (places != nullptr && blockIdx.z == 0 && threadIdx.x == 0) places[static_cast<size_t>(seq) * page_stride + page] = seq * page_stride + page;
     const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
     const int first = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) - page * kPage : 0;      // the first position of this page that a query sees
     if (sparse && (live <= 0 || first >= kPage)) return;
@@ -433,7 +434,7 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
                                 int n_kv_heads, int D, const void* query_rows, long long query_stride, void* queries, int n_heads, const float* q_weight, const float* k_weight,
                                 float eps, const float* cos_table, const float* sin_table, int rotary_dim, void* stream) {
     if (tokens <= 0 || n_seqs <= 0) return 0;
-    if (!keys || !values || !key_pages || !value_pages || !key_scales || !value_scales || !cu_seqlens || !seq_start || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 ||
+    if (!keys || !values || !key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !cu_seqlens || !seq_start || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 ||
         D > 256 || (D & 15) || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) || (rotary_dim > 0 && (!cos_table || !sin_table)) || (query_rows && (!queries || n_heads <= 0)))
         return cudaErrorInvalidValue;
     const StoreSource source = {static_cast<const bf16*>(keys), static_cast<const bf16*>(values), key_stride, value_stride, static_cast<const bf16*>(query_rows), query_stride,
@@ -449,14 +450,15 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
     return tau_launch_status();
 }
 
-TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* keys, void* values, const int* seq_start,
+TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* keys, void* values, int* places, const int* seq_start,
                                const int* seq_len, const int* page_rows, int page_stride, int n_seqs, int n_kv_heads, int D, int window, int sparse, void* stream) {
     if (n_seqs <= 0) return 0;
-    if (!key_pages || !value_pages || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
+    if (!key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len ||
+        !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || 2 * n_kv_heads > 65535)
         return cudaErrorInvalidValue;
     tau_launch(read_kernel, dim3(page_stride, n_seqs, 2 * n_kv_heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
-               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), seq_start, seq_len, page_rows, page_stride, n_kv_heads, D,
+               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, n_kv_heads, D,
                window, sparse);
     return tau_launch_status();
 }

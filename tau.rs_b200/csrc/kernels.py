@@ -471,6 +471,10 @@ _sm_counts = {}
 def sm_count(device=None) -> int:
     """Streaming multiprocessors of the device (of the current one if none is named; 148, a B200's, where there is no GPU
     to ask, which only the host-side tests of the rules below meet)."""
+    if device is None and _sm_counts and _raw_device is not None:      # asked before: `is_available` takes longer than the rest of a launch's rule
+        known = _sm_counts.get(_raw_device())
+        if known is not None:
+            return known
     if not torch.cuda.is_available():
         return 148
     index = torch.cuda.current_device() if device is None or torch.device(device).index is None else torch.device(device).index
@@ -1019,10 +1023,10 @@ CODE_DTYPE = torch.float8_e4m3fn
 
 def _here(*tensors) -> None:
     """Refuses tensors that do not lie on the current device, whose current stream the kernels are launched on."""
-    current = torch.cuda.current_device() if torch.cuda.is_initialized() else -2
+    current = _raw_device() if _raw_device is not None and torch.cuda.is_initialized() else torch.cuda.current_device() if torch.cuda.is_initialized() else -2
     for tensor in tensors:
         if tensor is not None and tensor.get_device() != current:
-            _require(False, "tensors must lie on the current CUDA device; there is no CPU path")
+            raise KernelError("tensors must lie on the current CUDA device; there is no CPU path")
 
 
 _functions = {}
@@ -1082,21 +1086,33 @@ def quantize_rows(values):
 
 
 def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
-    _require(values.dim() == 2 and codes.dim() == 2 and values.shape[1] == codes.shape[1], "shapes must be [M,K] x [N,K] -> [M,N]")
-    rows, depth = values.shape
-    features = codes.shape[0]
-    _require(codes.dtype == CODE_DTYPE and codes.is_contiguous() and codes.data_ptr() % 16 == 0, "the weight must be contiguous float8_e4m3fn codes on a 16-byte border")
-    _require(depth > 0 and depth % 16 == 0, "the depth must be a multiple of 16")
-    _require(scales.dtype == torch.float32 and scales.shape == (_scale_blocks(features), _scale_blocks(depth)) and scales.is_contiguous(),
-             "the weight's scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)]")
-    _require(values.dtype in (torch.bfloat16, torch.float32) and values.stride(1) == 1 and values.stride(0) % 8 == 0 and values.data_ptr() % 16 == 0,
-             "activations must be bfloat16 or float32 with rows on 16-byte borders")
-    _require(out.shape == (rows, features // 2 if gated else features) and (out.stride(1) == 1 or out.shape[1] == 1) and (rows < 2 or out.stride(0) >= out.shape[1]),
-             "the output must be [M, N], or [M, N / 2] of a gated product")
-    _require(out.dtype == torch.bfloat16 if gated else out.dtype in (torch.bfloat16, torch.float32), "the output must be bfloat16 (or float32 where nothing is gated)")
-    _require(not gated or features % (2 * GATE_GROUP) == 0, "a gated product needs a multiple of 16 weight rows")
-    _f32_vector(bias, features, "the bias")
+    (rows, depth), (features, weight_depth) = _two(values, codes)
+    if depth != weight_depth:
+        raise KernelError("shapes must be [M,K] x [N,K] -> [M,N]")
+    if codes.dtype is not CODE_DTYPE or not codes.is_contiguous():
+        raise KernelError("the weight must be contiguous float8_e4m3fn codes")
+    if depth % 16 or not depth:
+        raise KernelError("the depth must be a multiple of 16")
+    if scales.dtype is not torch.float32 or scales.shape != (-(-features // SCALE_BLOCK), -(-depth // SCALE_BLOCK)) or not scales.is_contiguous():
+        raise KernelError("the weight's scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)]")
+    if values.dtype not in _DTYPE_CODE or values.stride(1) != 1 or values.stride(0) % 8 or values.data_ptr() % 16:
+        raise KernelError("activations must be bfloat16 or float32 with rows on 16-byte borders")
+    columns = features // 2 if gated else features
+    if out.shape != (rows, columns) or (columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns):
+        raise KernelError("the output must be [M, N], or [M, N / 2] of a gated product")
+    if out.dtype is not torch.bfloat16 and (gated or out.dtype is not torch.float32):
+        raise KernelError("the output must be bfloat16 (or float32 where nothing is gated)")
+    if gated and features % (2 * GATE_GROUP):
+        raise KernelError("a gated product needs a multiple of 16 weight rows")
+    if bias is not None:
+        _f32_vector(bias, features, "the bias")
     _here(values, codes, scales, bias, out)
+
+
+def _two(values, codes):
+    if values.dim() != 2 or codes.dim() != 2:
+        raise KernelError("shapes must be [M,K] x [N,K] -> [M,N]")
+    return values.shape, codes.shape
 
 
 def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
@@ -1114,22 +1130,29 @@ SKINNY8_MAX_ROWS = 32       # what it accepts quantised
 SKINNY8_SMALL_ROWS = 16     # up to here it beats the tensor-core product where the weight is small (16 x 1,024 x 4,096 2.5 us against 5.2; 16 x 4,096 x 24,576 30 against 27)
 
 
+def _skinny8(x: int, x_stride: int, x_scales, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
+    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "iplpppppiiilif")
+    features, depth = codes.shape
+    _check(run(_DTYPE_CODE[out.dtype], x, x_stride, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, features, depth, out.stride(0),
+               1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
+
+
+def _tc8(x: int, x_scales: int, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float, features: int, ranges: int) -> None:
+    run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
+    _check(run(_DTYPE_CODE[out.dtype], x, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], codes.shape[1], out.stride(0),
+               1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
+
+
 def gemm8_skinny(values, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
     """The product for a few rows, bound by streaming the weight's codes once: bfloat16 rows (`x_scales` None, at most 8) or quantised ones (at most 32)."""
-    rows, depth = values.shape
-    _require(rows <= (SKINNY8_FUSED_ROWS if x_scales is None else SKINNY8_MAX_ROWS), "too many rows for the skinny kernel")
-    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "iplpppppiiilif")
-    _check(run(_code(out), values.data_ptr(), values.stride(0), _address(x_scales), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth,
-               out.stride(0), 1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
+    _require(values.shape[0] <= (SKINNY8_FUSED_ROWS if x_scales is None else SKINNY8_MAX_ROWS), "too many rows for the skinny kernel")
+    _skinny8(values.data_ptr(), values.stride(0), _address(x_scales), values.shape[0], codes, scales, bias, out, gated, gate_limit)
 
 
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
     """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 256; 0: by the number of tiles) with K cut into `ranges`
     (1 to 8; 0: as many as leave no SM without work)."""
-    rows, depth = x_codes.shape
-    run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
-    _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
-               1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
+    _tc8(x_codes.data_ptr(), x_scales.data_ptr(), x_codes.shape[0], codes, scales, bias, out, gated, gate_limit, features, ranges)
 
 
 def gemm8_tc_status() -> int:
@@ -1138,7 +1161,8 @@ def gemm8_tc_status() -> int:
 
 
 def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> None:
-    rows, features = values.shape[0], codes.shape[0]
+    rows, depth = values.shape
+    features = codes.shape[0]
     if rows == 0 or features == 0:
         return
     if not _prefer_optimized:
@@ -1148,13 +1172,18 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
         gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
         run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
         return _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
-    small = codes.numel() <= SKINNY8_FUSED_WEIGHT
-    if small and rows <= SKINNY8_FUSED_ROWS and values.dtype == torch.bfloat16:
-        return gemm8_skinny(values, None, codes, scales, bias, out, gated, limit)
-    x_codes, x_scales = quantize_rows(values)
+    small = features * depth <= SKINNY8_FUSED_WEIGHT
+    if small and rows <= SKINNY8_FUSED_ROWS and values.dtype is torch.bfloat16:
+        return _skinny8(values.data_ptr(), values.stride(0), None, rows, codes, scales, bias, out, gated, limit)
+    # The activations' codes and, behind them, their scales, in one piece of memory.
+    held = torch.empty(rows * (depth + 4 * -(-depth // SCALE_BLOCK)), dtype=torch.uint8, device=values.device)
+    x = held.data_ptr()
+    x_scales = x + rows * depth
+    run = _function("eight_bit.cu", "tau_quantize_rows", "iplppii")
+    _check(run(_DTYPE_CODE[values.dtype], values.data_ptr(), values.stride(0), x, x_scales, rows, depth, _stream_handle()), "quantize_rows")
     if rows <= SKINNY8_FUSED_ROWS or (small and rows <= SKINNY8_SMALL_ROWS):
-        return gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated, limit)
-    gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated, limit)
+        return _skinny8(x, depth, x_scales, rows, codes, scales, bias, out, gated, limit)
+    _tc8(x, x_scales, rows, codes, scales, bias, out, gated, limit, 0, 0)
 
 
 def linear8(values, codes, scales, bias, out) -> None:
@@ -1172,16 +1201,21 @@ def linear8_gated(values, codes, scales, out, limit: float = 0.0) -> None:
 
 
 def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows) -> None:
-    _require(key_pages.dtype == CODE_DTYPE == value_pages.dtype and key_pages.dim() == 4 and key_pages.shape[2] == PAGE_TOKENS and key_pages.shape == value_pages.shape
-             and key_pages.is_contiguous() and value_pages.is_contiguous() and key_pages.data_ptr() % 16 == 0 and value_pages.data_ptr() % 16 == 0,
-             "cache pages must be float8_e4m3fn [pages, n_kv_heads, 64, head_dim]")
-    _require(key_pages.shape[3] % 16 == 0 and 16 <= key_pages.shape[3] <= 256, "head_dim must be a multiple of 16 between 16 and 256")
+    shape = key_pages.shape
+    if (key_pages.dtype is not CODE_DTYPE or value_pages.dtype is not CODE_DTYPE or len(shape) != 4 or shape[2] != PAGE_TOKENS or value_pages.shape != shape
+            or not key_pages.is_contiguous() or not value_pages.is_contiguous()):
+        raise KernelError("cache pages must be float8_e4m3fn [pages, n_kv_heads, 64, head_dim]")
+    if shape[3] % 16 or not 16 <= shape[3] <= 256:
+        raise KernelError("head_dim must be a multiple of 16 between 16 and 256")
     for scales in (key_scales, value_scales):
-        _require(scales.dtype == torch.float32 and scales.shape == key_pages.shape[:2] and scales.is_contiguous(), "the pages' scales must be float32 [pages, n_kv_heads]")
-    _require(page_rows.dtype == torch.int32 and page_rows.dim() == 2 and page_rows.is_contiguous() and page_rows.shape[0] == step.n_seqs, "page rows must be int32 [sequences, stride]")
-    for what, tensor, count in (("cu_seqlens", step.cu_seqlens, step.n_seqs + 1), ("seq_start", step.seq_start, step.n_seqs), ("seq_len", step.seq_len, step.n_seqs)):
-        _int_vector(tensor, what)
-        _require(tensor.numel() == count, f"{what} must have {count} elements")
+        if scales.dtype is not torch.float32 or scales.shape != shape[:2] or not scales.is_contiguous():
+            raise KernelError("the pages' scales must be float32 [pages, n_kv_heads]")
+    sequences = step.n_seqs
+    if page_rows.dtype is not torch.int32 or page_rows.dim() != 2 or page_rows.shape[0] != sequences or not page_rows.is_contiguous():
+        raise KernelError("page rows must be int32 [sequences, stride]")
+    for tensor, count in ((step.cu_seqlens, sequences + 1), (step.seq_start, sequences), (step.seq_len, sequences)):
+        if tensor.dtype is not torch.int32 or tensor.numel() != count or tensor.stride(0) != 1:
+            raise KernelError("a step's cu_seqlens, seq_start and seq_len must be int32, one (and one more bound) to a sequence")
 
 
 def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales, step, page_rows, prepare=None) -> None:
@@ -1224,20 +1258,25 @@ def attention8_queries(projected, queries, q_weight, eps: float, cos, sin, rotar
     attention_prepare(projected, queries, nothing, nothing, False, q_weight, None, eps, cos, sin, rotary_dim, step.positions, step.token_seq, places, n_heads, 1, head_dim)
 
 
-def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int = 0, sparse: bool = False):
+def _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int, sparse: bool):
+    sequences, stride = page_rows.shape
+    n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
+    _require(sequences <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
+    pages = torch.empty((2, sequences * stride, n_kv_heads, PAGE_TOKENS, head_dim), dtype=torch.bfloat16, device=key_pages.device)
+    places = torch.empty((sequences, stride), dtype=torch.int32, device=key_pages.device) if sparse else None
+    run = _function("eight_bit.cu", "tau_cache8_read", "ppppppppppiiiiii")
+    keys, values = pages.unbind()
+    _check(run(key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(places), step.seq_start.data_ptr(),
+               step.seq_len.data_ptr(), page_rows.data_ptr(), stride, sequences, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
+    return keys, values, places
+
+
+def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows):
     """The pages of the step's sequences as the bfloat16 values that they stand for: keys and values [sequences * stride, n_kv_heads, 64, head_dim], page `j` of
-    sequence `i` at `i * stride + j`; zeros where a sequence has no position.  `sparse`: pages that no query of the step sees (behind the sequence's end, or wholly before
-    the `window` of its first new token) are left unwritten."""
+    sequence `i` at `i * stride + j`; zeros where a sequence has no position."""
     _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
     _here(key_pages, value_pages, key_scales, value_scales, step.seq_start, step.seq_len, page_rows)
-    n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
-    _require(step.n_seqs <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
-    shape = (step.n_seqs * page_rows.shape[1], n_kv_heads, PAGE_TOKENS, head_dim)
-    keys, values = (torch.empty(shape, dtype=torch.bfloat16, device=key_pages.device) for _ in range(2))
-    run = _function("eight_bit.cu", "tau_cache8_read", "pppppppppiiiiii")
-    _check(run(key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(), values.data_ptr(), step.seq_start.data_ptr(),
-               step.seq_len.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], step.n_seqs, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
-    return keys, values
+    return _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, 0, False)[:2]
 
 
 def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int] = None) -> int:
@@ -1257,36 +1296,40 @@ def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int]
 
 def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
     """One query token per sequence over its `seq_len` cached positions, read as they are held (`attention8` checks its arguments)."""
-    defines = (f"TAU_HEAD_DIM={head_dim}",)
     n_seqs = step.n_seqs
     group = n_heads // n_kv_heads
     passes = -(-group // (16 if group > 8 and head_dim <= 128 else 8))
     splits = min(step.decode_splits or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
     scratch = torch.empty(n_seqs * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
-    run = _function("attention_decode8.cu", "tau_decode8", "ppppppppiliiifiipl", defines)
+    run = _decode8_functions.get(head_dim)
+    if run is None:
+        run = _decode8_functions[head_dim] = _function("attention_decode8.cu", "tau_decode8", "ppppppppiliiifiipl", (f"TAU_HEAD_DIM={head_dim}",))
     _check(run(queries.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.seq_len.data_ptr(),
                page_rows.data_ptr(), page_rows.shape[1], key_pages.shape[0] * n_kv_heads, n_seqs, n_heads, n_kv_heads, scale, window, splits, _address(scratch),
                0 if scratch is None else scratch.numel(), _stream_handle()), "attention_decode8", 1 if scratch is None else 2)
 
 
+_decode8_functions = {}
 DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 
 
 def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
     """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
     _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
-    _require(key_pages.shape[1] == n_kv_heads and key_pages.shape[3] == head_dim and n_kv_heads > 0 and n_heads % n_kv_heads == 0,
-             "the pages must be [pages, n_kv_heads, 64, head_dim] and n_heads a multiple of n_kv_heads")
-    _require(queries.dtype == torch.bfloat16 == out.dtype and queries.shape == (step.n_tokens, n_heads * head_dim) and out.shape == queries.shape and queries.is_contiguous()
-             and out.is_contiguous(), "queries and output must be bfloat16 [tokens, n_heads * head_dim]")
-    _require(window >= 0, "a window must not be negative")
+    if key_pages.shape[1] != n_kv_heads or key_pages.shape[3] != head_dim or n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads <= 0:
+        raise KernelError("the pages must be [pages, n_kv_heads, 64, head_dim] and n_heads a multiple of n_kv_heads")
+    if (queries.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or queries.shape != (step.n_tokens, n_heads * head_dim) or out.shape != queries.shape
+            or not queries.is_contiguous() or not out.is_contiguous()):
+        raise KernelError("queries and output must be bfloat16 [tokens, n_heads * head_dim]")
+    if window < 0:
+        raise KernelError("a window must not be negative")
     _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
     if step.n_tokens == 0:
         return
     if step.all_single and _prefer_optimized:
         return attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
-    keys, values = cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, sparse=True)
-    places = torch.arange(keys.shape[0], dtype=torch.int32, device=keys.device).view(step.n_seqs, -1)
+    # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
+    keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, True)
     attention(queries, keys, values, out, step, places, n_heads, n_kv_heads, head_dim, scale, window)
 
 
