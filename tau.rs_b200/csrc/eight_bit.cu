@@ -186,22 +186,21 @@ struct StoreSource {
 };
 constexpr int kQueryHeads = 4;      // query heads to a block
 
-// One warp: norm and rotation of one head into `row` (shared memory).
-__device__ __forceinline__ void prepare_row(const bf16* __restrict__ source, const float* __restrict__ weight, float eps, const float* __restrict__ cosines,
-                                            const float* __restrict__ sines, int rotary_dim, int D, bf16* row, int lane) {
-    float inverse = 1.0f;
+// One warp: norm and rotation of one head, in place (shared memory).
+__device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__ weight, float eps, const float* __restrict__ cosines, const float* __restrict__ sines, int rotary_dim, int D,
+                                            int lane) {
     if (weight) {
         float squares = 0.0f;
         // In the order of the 16-bit cache's prepare kernel, so that a key is the same before it is rounded to 8 bits: neighbours to a lane where 32 divides the head, else strides of 32.
         const int per = D % 32 == 0 ? D / 32 : 1, begin = per > 1 ? lane * per : lane, end = per > 1 ? begin + per : D, by = per > 1 ? 1 : 32;
         for (int e = begin; e < end; e += by) {
-            const float value = to_float(source[e]);
+            const float value = to_float(row[e]);
             squares += value * value;
         }
-        inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + eps);
+        const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + eps);
+        for (int e = lane; e < D; e += 32) row[e] = __float2bfloat16_rn(to_float(row[e]) * inverse * weight[e]);
+        __syncwarp();
     }
-    for (int e = lane; e < D; e += 32) row[e] = weight ? __float2bfloat16_rn(to_float(source[e]) * inverse * weight[e]) : source[e];
-    __syncwarp();
     const int half = rotary_dim / 2;
     for (int j = lane; j < half; j += 32) {      // a pair is one lane's
         const float first = to_float(row[j]), second = to_float(row[j + half]), c = cosines[j], s = sines[j];
@@ -211,6 +210,27 @@ __device__ __forceinline__ void prepare_row(const bf16* __restrict__ source, con
     __syncwarp();
 }
 
+// All threads: `count` rows of D elements, `stride` apart, one behind the other in shared memory; 16 bytes at a time and four such loads on their way where the rows allow it.
+__device__ __forceinline__ void stage_rows(const bf16* __restrict__ source, long long stride, int count, int D, bf16* staged) {
+    if (((reinterpret_cast<uintptr_t>(source) | static_cast<uintptr_t>(stride * 2)) & 15) == 0) {
+        const int per_row = D / 8, pieces = count * per_row;
+        for (int base = threadIdx.x; base < pieces; base += 4 * 256) {
+            uint4 raw[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int piece = base + 256 * a, row = piece / per_row;
+                if (piece < pieces) raw[a] = __ldg(reinterpret_cast<const uint4*>(source + row * stride) + (piece - row * per_row));
+            }
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                if (base + 256 * a < pieces) reinterpret_cast<uint4*>(staged)[base + 256 * a] = raw[a];
+        }
+    } else {
+        for (int index = threadIdx.x; index < count * D; index += 256) staged[index] = source[index / D * stride + index % D];
+    }
+    __syncthreads();
+}
+
 // grid (pages touched, key heads + value heads + groups of query heads).  A block serves the new tokens of one sequence in one page: it
 // alone reads and writes that page of that head, so a scale that has to grow and the older codes that are rounded to it need no meeting.
 __global__ void __launch_bounds__(256)
@@ -218,7 +238,7 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
              const int* __restrict__ cu_seqlens, const int* __restrict__ seq_start, const int* __restrict__ page_rows, int page_stride, int n_seqs, int n_kv_heads, int D, int most) {
     grid_dependents_launch();
     grid_dependency_wait();
-    extern __shared__ __align__(16) bf16 staged[];      // [tokens here][D]; queries: [warp][D]
+    extern __shared__ __align__(16) bf16 staged[];      // [tokens here][D]
     __shared__ float greatest_of[8];
     __shared__ int found[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -266,17 +286,20 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
     const int seq = found[0], row0 = found[1], position0 = found[2], count = found[3];
     if (seq < 0) return;      // the host counts pages from above
     const int half = source.rotary_dim / 2;
-    if (static_cast<int>(blockIdx.y) >= 2 * n_kv_heads) {      // queries
+    if (static_cast<int>(blockIdx.y) >= 2 * n_kv_heads) {      // queries: one head after another
         const int head0 = (blockIdx.y - 2 * n_kv_heads) * kQueryHeads, heads = min(kQueryHeads, source.n_heads - head0);
-        bf16* row = staged + warp * D;
-        for (int task = warp; task < count * heads; task += 8) {
-            const int token = task / heads, head = head0 + task % heads;
-            const size_t table = static_cast<size_t>(position0 + token) * half;
-            prepare_row(source.query_rows + static_cast<size_t>(row0 + token) * source.query_stride + static_cast<size_t>(head) * D, source.q_weight, source.eps,
-                        source.cos_table + table, source.sin_table + table, source.rotary_dim, D, row, lane);
-            bf16* target = source.queries + (static_cast<size_t>(row0 + token) * source.n_heads + head) * D;
-            for (int e = lane; e < D; e += 32) target[e] = row[e];
-            __syncwarp();
+        for (int head = head0; head < head0 + heads; ++head) {
+            stage_rows(source.query_rows + static_cast<size_t>(row0) * source.query_stride + static_cast<size_t>(head) * D, source.query_stride, count, D, staged);
+            for (int token = warp; token < count; token += 8) {
+                const size_t table = static_cast<size_t>(position0 + token) * half;
+                prepare_row(staged + token * D, source.q_weight, source.eps, source.cos_table + table, source.sin_table + table, source.rotary_dim, D, lane);
+            }
+            __syncthreads();
+            for (int piece = threadIdx.x; piece < count * D / 8; piece += 256) {
+                const int token = piece / (D / 8), part = piece - token * (D / 8);
+                reinterpret_cast<uint4*>(source.queries + (static_cast<size_t>(row0 + token) * source.n_heads + head) * D)[part] = reinterpret_cast<const uint4*>(staged)[piece];
+            }
+            __syncthreads();
         }
         return;
     }
@@ -286,14 +309,21 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
     uint8_t* page = (is_key ? key_pages : value_pages) + place * kPage * D;
     float* scale_at = (is_key ? key_scales : value_scales) + place;
     const int older = position0 % kPage;
+    const long long stride = is_key ? source.key_stride : source.value_stride;
+    stage_rows((is_key ? source.keys : source.values) + static_cast<long long>(row0) * stride + static_cast<long long>(head) * D, stride, count, D, staged);
+    if (is_key && (source.k_weight != nullptr || half > 0)) {
+        for (int token = warp; token < count; token += 8) {
+            const size_t table = static_cast<size_t>(position0 + token) * half;
+            prepare_row(staged + token * D, source.k_weight, source.eps, source.cos_table + table, source.sin_table + table, source.rotary_dim, D, lane);
+        }
+        __syncthreads();
+    }
     float greatest = 0.0f;
-    for (int token = warp; token < count; token += 8) {
-        bf16* row = staged + token * D;
-        const bf16* from = is_key ? source.keys + static_cast<size_t>(row0 + token) * source.key_stride + static_cast<size_t>(head) * D
-                                  : source.values + static_cast<size_t>(row0 + token) * source.value_stride + static_cast<size_t>(head) * D;
-        const size_t table = static_cast<size_t>(position0 + token) * half;
-        prepare_row(from, is_key ? source.k_weight : nullptr, source.eps, source.cos_table + table, source.sin_table + table, is_key ? source.rotary_dim : 0, D, row, lane);
-        for (int e = lane; e < D; e += 32) greatest = fmaxf(greatest, finite_magnitude(to_float(row[e])));
+    for (int piece = threadIdx.x; piece < count * D / 8; piece += 256) {
+        const uint4 raw = reinterpret_cast<const uint4*>(staged)[piece];
+        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) greatest = fmaxf(greatest, fmaxf(finite_magnitude(__uint_as_float(words[i] << 16)), finite_magnitude(__uint_as_float(words[i] & 0xffff0000u))));
     }
     greatest = warp_max(greatest);
     if (lane == 0) greatest_of[warp] = greatest;
@@ -329,40 +359,56 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
 }
 
 // Pages of the step's sequences as the bfloat16 values that they stand for (exact: 4 significant bits times a power of two).
-// grid (page of a sequence, sequence, 2 n_kv_heads).  Positions that a sequence does not have are zeros; with `sparse` only pages that a query sees
-// are written at all (and `places` gets the numbers that the pages have in the result), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of zero would not hide that.
+// grid (page of a sequence, sequence, keys' and then values' groups of `heads` heads).  Positions that a sequence does not have are zeros; with `sparse` only pages that a query sees
+// are written at all (and `places` gets the numbers that the pages have in the result), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of
+// zero would not hide that.  Bound by memory: a page's heads lie one behind the other, so where there are pages enough a block takes several and pays for its page's number and
+// scale once (64 sequences of up to 200 positions, 8 heads of 128: READ_TIME).
 __global__ void __launch_bounds__(256)
 read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
             bf16* __restrict__ keys, bf16* __restrict__ values, int* __restrict__ places, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
-            int page_stride, int n_kv_heads, int D, int window, int sparse) {
+            int page_stride, int n_kv_heads, int heads, int D, int window, int sparse) {
     grid_dependents_launch();
     grid_dependency_wait();
-    const int page = blockIdx.x, seq = blockIdx.y;
-    const bool is_key = static_cast<int>(blockIdx.z) < n_kv_heads;
-    const int head = is_key ? blockIdx.z : blockIdx.z - n_kv_heads;
+    const int page = blockIdx.x, seq = blockIdx.y, groups = (n_kv_heads + heads - 1) / heads;
+    const bool is_key = static_cast<int>(blockIdx.z) < groups;
+    const int head0 = (is_key ? blockIdx.z : blockIdx.z - groups) * heads, here = min(heads, n_kv_heads - head0);
     if (places != nullptr && blockIdx.z == 0 && threadIdx.x == 0) places[static_cast<size_t>(seq) * page_stride + page] = seq * page_stride + page;
     const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
     const int first = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) - page * kPage : 0;      // the first position of this page that a query sees
     if (sparse && (live <= 0 || first >= kPage)) return;
-    const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * n_kv_heads + head : 0;
-    const uint8_t* codes = (is_key ? key_pages : value_pages) + place * kPage * D;
-    const float scale = live > 0 ? (is_key ? key_scales : value_scales)[place] : 0.0f;
-    bf16* target = (is_key ? keys : values) + ((static_cast<size_t>(seq) * page_stride + page) * n_kv_heads + head) * kPage * D;
-    for (int piece = threadIdx.x; piece < kPage * D / 16; piece += 256) {
-        const bool held = piece * 16 < live * D && piece * 16 >= first * D;
-        const uint4 raw = held ? __ldg(reinterpret_cast<const uint4*>(codes) + piece) : make_uint4(0u, 0u, 0u, 0u);
-        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint4 wide[2];
-        unsigned* out = reinterpret_cast<unsigned*>(wide);
+    const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * n_kv_heads + head0 : 0;
+    const uint4* codes = reinterpret_cast<const uint4*>((is_key ? key_pages : value_pages) + place * kPage * D);
+    const float* scales = (is_key ? key_scales : value_scales) + place;
+    uint4* target = reinterpret_cast<uint4*>((is_key ? keys : values) + ((static_cast<size_t>(seq) * page_stride + page) * n_kv_heads + head0) * kPage * D);
+    const int per_head = kPage * D / 16, begin = first * D / 16, end = live * D / 16;      // pieces of 16 elements
+    constexpr int kAhead = 4;
+    for (int base = threadIdx.x; base < here * per_head; base += 256 * kAhead) {
+        uint4 raw[kAhead];
+        float scale[kAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[4];
-            decode_four(words[i], v);
-            out[2 * i] = pack_bf16_pair(v[0] * scale, v[1] * scale);
-            out[2 * i + 1] = pack_bf16_pair(v[2] * scale, v[3] * scale);
+        for (int a = 0; a < kAhead; ++a) {
+            const int piece = base + 256 * a, head = piece / per_head, place_in = piece - head * per_head;
+            const bool held = head < here && place_in >= begin && place_in < end;
+            raw[a] = held ? __ldg(codes + piece) : make_uint4(0u, 0u, 0u, 0u);
+            scale[a] = held ? __ldg(scales + head) : 0.0f;
         }
-        reinterpret_cast<uint4*>(target)[2 * piece] = wide[0];
-        reinterpret_cast<uint4*>(target)[2 * piece + 1] = wide[1];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int piece = base + 256 * a;
+            if (piece >= here * per_head) break;
+            const unsigned words[4] = {raw[a].x, raw[a].y, raw[a].z, raw[a].w};
+            uint4 wide[2];
+            unsigned* out = reinterpret_cast<unsigned*>(wide);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
+                decode_four(words[i], v);
+                out[2 * i] = pack_bf16_pair(v[0] * scale[a], v[1] * scale[a]);
+                out[2 * i + 1] = pack_bf16_pair(v[2] * scale[a], v[3] * scale[a]);
+            }
+            target[2 * piece] = wide[0];
+            target[2 * piece + 1] = wide[1];
+        }
     }
 }
 
@@ -435,7 +481,7 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
                                 float eps, const float* cos_table, const float* sin_table, int rotary_dim, void* stream) {
     if (tokens <= 0 || n_seqs <= 0) return 0;
     if (!keys || !values || !key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !cu_seqlens || !seq_start || !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 ||
-        D > 256 || (D & 15) || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) || (rotary_dim > 0 && (!cos_table || !sin_table)) || (query_rows && (!queries || n_heads <= 0)))
+        D > 256 || (D & 15) || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) || (rotary_dim > 0 && (!cos_table || !sin_table)) || (query_rows && (!queries || (reinterpret_cast<uintptr_t>(queries) & 15) || n_heads <= 0)))
         return cudaErrorInvalidValue;
     const StoreSource source = {static_cast<const bf16*>(keys), static_cast<const bf16*>(values), key_stride, value_stride, static_cast<const bf16*>(query_rows), query_stride,
                                 static_cast<bf16*>(queries), q_weight, k_weight, eps, cos_table, sin_table, rotary_dim, n_heads};
@@ -444,7 +490,7 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
     const unsigned items = single ? static_cast<unsigned>(n_seqs) : static_cast<unsigned>(bound < tokens ? bound : tokens);
     const unsigned parts = 2u * n_kv_heads + (query_rows ? (n_heads + kQueryHeads - 1) / kQueryHeads : 0);
     if (parts > 65535u) return cudaErrorInvalidValue;
-    const int rows = single ? 8 : kPage;      // staged rows; queries stage one for each of 8 warps
+    const int rows = single ? 1 : kPage;      // staged rows
     tau_launch(store_kernel, dim3(items, parts), dim3(256), static_cast<size_t>(rows) * D * sizeof(bf16), static_cast<cudaStream_t>(stream), source, static_cast<uint8_t*>(key_pages),
                static_cast<uint8_t*>(value_pages), key_scales, value_scales, cu_seqlens, seq_start, page_rows, page_stride, n_seqs, n_kv_heads, D, rows);
     return tau_launch_status();
@@ -457,8 +503,10 @@ TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, c
         !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || 2 * n_kv_heads > 65535)
         return cudaErrorInvalidValue;
-    tau_launch(read_kernel, dim3(page_stride, n_seqs, 2 * n_kv_heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
-               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, n_kv_heads, D,
+    const long long blocks = 2ll * n_kv_heads * n_seqs * page_stride, wanted = 148 * 8;      // one head to a block as long as all fit the machine at once
+    const int heads = blocks <= wanted ? 1 : static_cast<int>(blocks / wanted < n_kv_heads ? blocks / wanted : n_kv_heads);
+    tau_launch(read_kernel, dim3(page_stride, n_seqs, 2 * ((n_kv_heads + heads - 1) / heads)), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
+               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, n_kv_heads, heads, D,
                window, sparse);
     return tau_launch_status();
 }
