@@ -85,12 +85,12 @@ __device__ __forceinline__ int key_element(int step, int t, int i) {
 
 constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a lane holds 16 columns, 8 tiles of 16 rows
 
-template <int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 ? 4 : 2)
+template <int NT, bool Runs>
+__global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 && !Runs ? 4 : 2)
 decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
                const float* __restrict__ key_scales, const float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
-               const int* __restrict__ seq_len, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale, int window, int splits,
-               int clustered) {
+               const int* __restrict__ seq_len, const int* __restrict__ cu_seqlens, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale,
+               int window, int splits, int clustered) {
     grid_dependents_launch();
     constexpr int kHeads = 8 * NT;
     extern __shared__ uint8_t shared_raw[];
@@ -106,8 +106,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     const int split = blockIdx.x, seq = blockIdx.z;
     const int kv_head = blockIdx.y / passes, pass = blockIdx.y % passes;
     const int group = n_heads / n_kv_heads;
-    const int head0 = kv_head * group + pass * kHeads;
-    const int heads_here = min(kHeads, group - pass * kHeads);
     volatile int* abort_flag = &shared->abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -119,8 +117,17 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     }
     __syncthreads();
     grid_dependency_wait();
-    const int length = seq_len[seq];
-    const int first = (window > 0 && length > window) ? length - window : 0;
+    // The block's columns: query heads of the group, or, with `Runs`, pairs of a new token and a head, tokens first.  Column j belongs to row `place(j)` of queries and results.
+    const int row0 = Runs ? cu_seqlens[seq] : seq, news = Runs ? cu_seqlens[seq + 1] - row0 : 1;
+    const int column0 = pass * kHeads, heads_here = min(kHeads, news * group - column0);
+    if (Runs && heads_here <= 0) return;      // the whole cluster: a run shorter than the longest
+    auto place = [&](int j) {
+        const int column = column0 + j, token = Runs ? column / group : 0;
+        return static_cast<size_t>(row0 + token) * n_heads + kv_head * group + (Runs ? column - token * group : column);
+    };
+    const int start = seq_len[seq] - news, token_lo = Runs ? column0 / group : 0, token_hi = Runs ? (column0 + heads_here - 1) / group : 0;
+    // What any of the columns sees.
+    const int length = start + token_hi + 1, first = window > 0 ? max(0, start + token_lo + 1 - window) : 0;
     const int first_page = first / kPage, pages_end = (length + kPage - 1) / kPage;
     const int per_split = (max(0, pages_end - first_page) + splits - 1) / splits;
     const int page_lo = first_page + split * per_split, page_hi = min(pages_end, page_lo + per_split);
@@ -195,7 +202,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         for (int n = 0; n < NT; ++n) {
             const int head = n * 8 + g;
             const bool live = head < heads_here && count > 0;
-            const bf16* row = queries + (static_cast<size_t>(seq) * n_heads + head0 + (live ? head : 0)) * D;
+            const bf16* row = queries + place(live ? head : 0) * D;
             float greatest = 0.0f;
 #pragma unroll
             for (int step = 0; step < kKeySteps; ++step) {
@@ -226,6 +233,15 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
             for (int h = 0; h < 2; ++h) factor[n][h] = __shfl_sync(0xffffffffu, q_power[n], (2 * t + h) * 4) * scale * kLog2e;
 
+        // With `Runs` each column sees up to its token's own position, and from its own window's begin on.
+        int column_end[NT][2], column_first[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                column_end[n][h] = Runs ? start + (column0 + n * 8 + 2 * t + h) / group + 1 : length;
+                column_first[n][h] = Runs && window > 0 ? max(0, column_end[n][h] - window) : first;
+            }
         bool alive = true;
         for (int number = 0; number < count; ++number) {
             const int stage = number % kStages;
@@ -280,7 +296,28 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_f16(step & 1 ? score_odd[n] : score[n], a0, a1, a2, a3, q_frag[n][step][0], q_frag[n][step][1]);
                 }
-                const bool live_lo = base + g >= first && base + g < length, live_hi = base + g + 8 >= first && base + g + 8 < length;
+                // Keys whose values are not finite, where some columns see a key that others do not: they count as zeros below, and as NaN in the scores of the columns that see them.
+                unsigned odd_keys = 0;
+                if constexpr (Runs) {
+                    if (base + 16 > start + token_lo + 1 || (window > 0 && base < length - window)) {
+                        const int slots[4] = {2 * t, 2 * t + 1, 2 * t + 8, 2 * t + 9};
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            unsigned odd = 0;
+#pragma unroll
+                            for (int r = 0; r < kValueRounds; ++r) {
+                                if ((8 * r + g) * 16 >= D) continue;
+                                const uint4 v = page_chunk(value_tile, warp * 16 + slots[s], 8 * r + g);
+                                odd |= __vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu) |
+                                       __vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                            }
+                            const unsigned who = __ballot_sync(0xffffffffu, odd != 0u);
+#pragma unroll
+                            for (int other = 0; other < 4; ++other)
+                                if (who & (0x11111111u << other)) odd_keys |= 1u << (2 * other + (s & 1) + 8 * (s >> 1));
+                        }
+                    }
+                }
                 const bool apart = share < kLeastShare;      // a 16-bit weight would lose bits: the page's sums are taken apart and added in 32 bits
                 const float by_share = apart ? 1.0f : share;
                 bool moved = older != 1.0f;
@@ -292,17 +329,21 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float by = factor[n][h] * k_scale;
-                        const float low = live_lo ? (score[n][h] + score_odd[n][h]) * by : -INFINITY, high = live_hi ? (score[n][2 + h] + score_odd[n][2 + h]) * by : -INFINITY;
+                        const bool live_lo = base + g >= column_first[n][h] && base + g < column_end[n][h], live_hi = base + g + 8 >= column_first[n][h] && base + g + 8 < column_end[n][h];
+                        const float nan = __uint_as_float(0x7fffffffu);
+                        const float low = !live_lo ? -INFINITY : Runs && (odd_keys >> g & 1u) ? nan : (score[n][h] + score_odd[n][h]) * by;
+                        const float high = !live_hi ? -INFINITY : Runs && (odd_keys >> (g + 8) & 1u) ? nan : (score[n][2 + h] + score_odd[n][2 + h]) * by;
                         float most = fmaxf(low, high);
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                        const float new_max = fmaxf(running_max[n][h], most);      // finite: one of the 16 keys is visible
+                        const float new_max = fmaxf(running_max[n][h], most);      // finite where one of the 16 keys is visible: always, but for columns of a run
                         moved |= new_max != running_max[n][h];
-                        correction[n][h] = exp2f(running_max[n][h] - new_max);
+                        const float from = Runs && new_max == -INFINITY ? 0.0f : new_max;
+                        correction[n][h] = exp2f(running_max[n][h] - from);
                         running_max[n][h] = new_max;
-                        p[h] = exp2f(low - new_max + kWeightBits);
-                        p[2 + h] = exp2f(high - new_max + kWeightBits);
+                        p[h] = exp2f(low - from + kWeightBits);
+                        p[2 + h] = exp2f(high - from + kWeightBits);
                         running_sum[n][h] = running_sum[n][h] * correction[n][h] + p[h] + p[2 + h];
                     }
                     pb0[n] = pack_half2(p[0] * by_share, p[1] * by_share);
@@ -330,7 +371,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     for (int s = 0; s < 4; ++s) {
                         v[s] = chunk * 16 < D ? page_chunk(value_tile, warp * 16 + slots[s], chunk) : make_uint4(0u, 0u, 0u, 0u);
                         // What nobody sees may be NaN, and a weight of zero would not hide that.
-                        if (!whole && (base + slots[s] < first || base + slots[s] >= length)) v[s] = make_uint4(0u, 0u, 0u, 0u);
+                        if ((!whole && (base + slots[s] < first || base + slots[s] >= length)) || (Runs && (odd_keys >> slots[s] & 1u))) v[s] = make_uint4(0u, 0u, 0u, 0u);
                     }
                     const unsigned w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
                     const unsigned w8[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, w9[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
@@ -411,7 +452,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     }
     __syncthreads();
     const bool failed = *abort_flag != 0;
-    const size_t record = (static_cast<size_t>(seq) * n_heads + head0) * splits + split;
     for (int index = threadIdx.x; index < heads_here * D; index += kThreads) {
         const int h = index / D, c = index % D;
         float total_max = -INFINITY;
@@ -426,7 +466,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             sum += merge_ml[w][h][1] * by;
         }
         if (splits == 1) {
-            if (!failed) out[(static_cast<size_t>(seq) * n_heads + head0 + h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);      // a sequence without positions: zeros
+            if (!failed) out[place(h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);      // a sequence without positions: zeros
         } else if (clustered) {
             merge_o[0][h][c] = o;      // this thread alone reads and writes (h, c) of the first warp's part
             if (c == 0) {
@@ -434,7 +474,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 block_ml[h][1] = sum;
             }
         } else if (!failed) {
-            const size_t slot = record + static_cast<size_t>(h) * splits;
+            const size_t slot = place(h) * splits + split;
             if (sum != 0.0f) partial_o[slot * D + c] = o;
             if (c == 0) {
                 partial_ml[slot * 2] = total_max;
@@ -473,7 +513,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 o += split_o[s] * by;
                 sum += split_sum[s] * by;
             }
-            out[(static_cast<size_t>(seq) * n_heads + head0 + h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);
+            out[place(h) * D + c] = __float2bfloat16_rn(sum != 0.0f ? o / sum : 0.0f);
         }
     }
     cluster_sync_all();      // nobody leaves while its results are read
@@ -527,39 +567,46 @@ int page_map(CUtensorMap* map, const void* pages, long long boxes) {
 
 constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + kStages * kStageBytes; }
 
-template <int NT>
-int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const bf16* queries, bf16* out, const float* key_scales, const float* value_scales, float* partial_o,
-           float* partial_ml, const int* seq_len, const int* page_rows, int page_stride, int n_seqs, int n_heads, int n_kv_heads, int passes, float scale, int window, int splits,
-           cudaStream_t stream) {
+struct Call {
+    const bf16* queries;
+    bf16* out;
+    const float *key_scales, *value_scales;
+    float *partial_o, *partial_ml;
+    const int *seq_len, *cu_seqlens, *page_rows;
+    int page_stride, n_seqs, n_tokens, n_heads, n_kv_heads, passes;
+    float scale;
+    int window, splits;
+};
+
+template <int NT, bool Runs>
+int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call& c, cudaStream_t stream) {
     static bool ready[64] = {};
     int device = 0;
     cudaError_t status = cudaGetDevice(&device);
     if (status != cudaSuccess) return static_cast<int>(status);
     if (device >= 64 || !ready[device]) {
-        status = cudaFuncSetAttribute(decode8_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes());
+        status = cudaFuncSetAttribute(decode8_kernel<NT, Runs>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes());
         if (status != cudaSuccess) return static_cast<int>(status);
         if (device < 64) ready[device] = true;
     }
-    const dim3 grid(splits, n_kv_heads * passes, n_seqs);
-    const bool clustered = splits > 1 && splits <= kMostClustered;
+    const dim3 grid(c.splits, c.n_kv_heads * c.passes, c.n_seqs);
+    const bool clustered = c.splits > 1 && c.splits <= kMostClustered;
     int code;
     if (clustered)
-        code = tau_launch_clusters_as(false, splits, decode8_kernel<NT>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, queries, out, key_scales, value_scales, partial_o,
-                                      partial_ml, seq_len, page_rows, page_stride, n_heads, n_kv_heads, passes, scale, window, splits, 1);
+        code = tau_launch_clusters_as(false, c.splits, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_scales, c.value_scales,
+                                      c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1);
     else
-        code = tau_launch_as(false, decode8_kernel<NT>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, queries, out, key_scales, value_scales, partial_o, partial_ml, seq_len,
-                             page_rows, page_stride, n_heads, n_kv_heads, passes, scale, window, splits, 0);
+        code = tau_launch_as(false, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_scales, c.value_scales, c.partial_o,
+                             c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0);
+    if (code == 0 && c.splits > kMostClustered)
+        code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? D : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
     return code ? code : tau_launch_status();
 }
 
 }  // namespace
 
-// Query heads to a block: 16 where a group has more than 8 and a head's accumulators leave room for them.
-static int heads_to_a_block(int group) { return group > 8 && D <= 128 ? 16 : 8; }
-
-TAU_EXPORT int tau_decode8_passes(int group) { return (group + heads_to_a_block(group) - 1) / heads_to_a_block(group); }
-
-TAU_EXPORT int tau_decode8_most_clustered() { return kMostClustered; }
+// Columns to a block: 16 where there are more than 8 and a head's accumulators leave room for them.
+static int columns_to_a_block(long long columns) { return columns > 8 && D <= 128 ? 16 : 8; }
 
 TAU_EXPORT int tau_decode8_status() {
     int flag = 0;
@@ -568,36 +615,29 @@ TAU_EXPORT int tau_decode8_status() {
     return flag;
 }
 
-// bfloat16 queries and output [sequences, n_heads D]; pages [boxes / n_kv_heads, n_kv_heads, 64, D] of e4m3 codes with scales [boxes].  More than 8 splits need
-// scratch of n_seqs * n_heads * splits * (D + 2) floats.
+// bfloat16 queries and output [tokens, n_heads D]; pages [boxes / n_kv_heads, n_kv_heads, 64, D] of e4m3 codes with scales [boxes].  `cu_seqlens` == nullptr: one token to
+// a sequence; else the runs' bounds, none longer than `max_new`.  More than 8 splits need scratch of n_tokens * n_heads * splits * (D + 2) floats.
 TAU_EXPORT int tau_decode8(const void* queries, const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* out, const int* seq_len,
-                           const int* page_rows, int page_stride, long long boxes, int n_seqs, int n_heads, int n_kv_heads, float scale, int window, int splits, float* scratch,
-                           long long scratch_floats, void* stream) {
-    if (n_seqs <= 0) return 0;
+                           const int* cu_seqlens, const int* page_rows, int page_stride, long long boxes, int n_seqs, int n_tokens, int max_new, int n_heads, int n_kv_heads, float scale,
+                           int window, int splits, float* scratch, long long scratch_floats, void* stream) {
+    if (n_seqs <= 0 || n_tokens <= 0) return 0;
     if (!queries || !key_pages || !value_pages || !key_scales || !value_scales || !out || !seq_len || !page_rows || page_stride <= 0 || boxes <= 0 || n_heads <= 0 || n_kv_heads <= 0 ||
-        n_heads % n_kv_heads != 0 || window < 0 || splits < 1 || splits > 256 || n_seqs > 65535 || boxes > 0x7fffffffll ||
-        (splits > kMostClustered && (!scratch || scratch_floats < static_cast<long long>(n_seqs) * n_heads * splits * (D + 2))))
+        n_heads % n_kv_heads != 0 || window < 0 || splits < 1 || splits > 256 || n_seqs > 65535 || n_tokens > 65535 || max_new < 1 || (!cu_seqlens && (max_new != 1 || n_tokens != n_seqs)) ||
+        boxes > 0x7fffffffll || (reinterpret_cast<uintptr_t>(queries) & 7) ||
+        (splits > kMostClustered && (!scratch || scratch_floats < static_cast<long long>(n_tokens) * n_heads * splits * (D + 2))))
         return cudaErrorInvalidValue;
+    const long long columns = static_cast<long long>(n_heads / n_kv_heads) * max_new;
+    const int to_a_block = columns_to_a_block(columns);
+    if (n_kv_heads * ((columns + to_a_block - 1) / to_a_block) > 65535) return cudaErrorInvalidValue;
     CUtensorMap key_map, value_map;
     int status = page_map(&key_map, key_pages, boxes);
     if (!status) status = page_map(&value_map, value_pages, boxes);
     if (status) return status;
-    const int group = n_heads / n_kv_heads, passes = tau_decode8_passes(group);
-    if (n_kv_heads * passes > 65535) return cudaErrorInvalidValue;
-    float* partial_ml = scratch ? scratch + static_cast<size_t>(n_seqs) * n_heads * splits * D : nullptr;
+    const Call call = {static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch,
+                       scratch ? scratch + static_cast<size_t>(n_tokens) * n_heads * splits * D : nullptr, seq_len, cu_seqlens, page_rows, page_stride, n_seqs, n_tokens, n_heads, n_kv_heads,
+                       static_cast<int>((columns + to_a_block - 1) / to_a_block), scale, window, splits};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if constexpr (D <= 128) {
-        if (heads_to_a_block(group) == 16) {
-            status = launch<2>(key_map, value_map, static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch, partial_ml, seq_len, page_rows, page_stride,
-                               n_seqs, n_heads, n_kv_heads, passes, scale, window, splits, s);
-            if (status || splits <= kMostClustered) return status;
-            tau_launch(join_kernel, dim3(n_heads, n_seqs), dim3(D < 128 ? D : 128), 0, s, scratch, partial_ml, static_cast<bf16*>(out), n_heads, splits);
-            return tau_launch_status();
-        }
-    }
-    status = launch<1>(key_map, value_map, static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch, partial_ml, seq_len, page_rows, page_stride, n_seqs, n_heads,
-                       n_kv_heads, passes, scale, window, splits, s);
-    if (status || splits <= kMostClustered) return status;
-    tau_launch(join_kernel, dim3(n_heads, n_seqs), dim3(D < 128 ? D : 128), 0, s, scratch, partial_ml, static_cast<bf16*>(out), n_heads, splits);
-    return tau_launch_status();
+    if constexpr (D <= 128)
+        if (to_a_block == 16) return cu_seqlens ? launch<2, true>(key_map, value_map, call, s) : launch<2, false>(key_map, value_map, call, s);
+    return cu_seqlens ? launch<1, true>(key_map, value_map, call, s) : launch<1, false>(key_map, value_map, call, s);
 }

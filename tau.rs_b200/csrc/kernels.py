@@ -1295,20 +1295,35 @@ def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int]
 
 
 def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
-    """One query token per sequence over its `seq_len` cached positions, read as they are held (`attention8` checks its arguments)."""
-    n_seqs = step.n_seqs
-    group = n_heads // n_kv_heads
-    passes = -(-group // (16 if group > 8 and head_dim <= 128 else 8))
-    splits = min(step.decode_splits or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
-    scratch = torch.empty(n_seqs * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
+    """One query token per sequence over its `seq_len` cached positions, or a few, read as they are held (`attention8` checks its arguments)."""
+    n_seqs, n_tokens = step.n_seqs, step.n_tokens
+    single = step.all_single
+    columns = n_heads // n_kv_heads * (1 if single else step.max_new)
+    passes = -(-columns // (16 if columns > 8 and head_dim <= 128 else 8))
+    splits = min((step.decode_splits if single else 0) or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
+    scratch = torch.empty(n_tokens * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
     run = _decode8_functions.get(head_dim)
     if run is None:
-        run = _decode8_functions[head_dim] = _function("attention_decode8.cu", "tau_decode8", "ppppppppiliiifiipl", (f"TAU_HEAD_DIM={head_dim}",))
+        run = _decode8_functions[head_dim] = _function("attention_decode8.cu", "tau_decode8", "pppppppppiliiiiifiipl", (f"TAU_HEAD_DIM={head_dim}",))
     _check(run(queries.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.seq_len.data_ptr(),
-               page_rows.data_ptr(), page_rows.shape[1], key_pages.shape[0] * n_kv_heads, n_seqs, n_heads, n_kv_heads, scale, window, splits, _address(scratch),
-               0 if scratch is None else scratch.numel(), _stream_handle()), "attention_decode8", 1 if scratch is None else 2)
+               None if single else step.cu_seqlens.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], key_pages.shape[0] * n_kv_heads, n_seqs, n_tokens, 1 if single else step.max_new,
+               n_heads, n_kv_heads, scale, window, splits, _address(scratch), 0 if scratch is None else scratch.numel(), _stream_handle()), "attention_decode8", 1 if scratch is None else 2)
 
 
+RUNS8_COLUMNS = 64          # of new tokens times a group's query heads, up to which runs are worked on like single tokens, 16 columns to a reading of the pages (us against pages laid
+                            # out in 16 bits and their kernels: 4 sequences of 2,000 positions, 32 heads of 128 over 8, 8 tokens each 23 and 50, 32 tokens 69 and 50; 8 of 8,000 and
+                            # 16 tokens 184 and 211) ...
+RUNS8_COLUMNS_OTHER = 160   # ... for heads whose 16-bit kernel has no tensor memory (16 tokens of 32 heads of 80 over 8 behind 2,000: 36 and 97) ...
+RUNS8_FEW_PAGES = 2048      # ... and wherever the pages are read no more often than this in all: a launch where the other way takes two (one sequence of 500, 64 tokens: 19 and 17, and
+                            # 18 us less on the host)
+
+
+def runs8_like_single_tokens(n_seqs: int, max_new: int, max_len: int, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    """Whether `attention8` takes a step of runs to the kernel of single tokens, which reads pages as they are held."""
+    columns = max_new * (n_heads // n_kv_heads)
+    if columns <= (RUNS8_COLUMNS if head_dim in (64, 128) else RUNS8_COLUMNS_OTHER):
+        return True
+    return n_seqs * n_kv_heads * -(-max_len // PAGE_TOKENS) * -(-columns // 16) <= RUNS8_FEW_PAGES
 _decode8_functions = {}
 DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 
@@ -1326,7 +1341,7 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
     if step.n_tokens == 0:
         return
-    if step.all_single and _prefer_optimized:
+    if _prefer_optimized and (step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim))):
         return attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
     keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, True)

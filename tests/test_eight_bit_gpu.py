@@ -341,6 +341,37 @@ def test_runs(heads, kv_heads, dim, window):
     check_attention([(0, 70), (100, 1), (60, 9), (0, 1), (130, 66), (64, 64)], heads, kv_heads, dim, window)
 
 
+@pytest.mark.parametrize("directly", [0, 1])
+@pytest.mark.parametrize("heads, kv_heads, dim, window", [(4, 2, 32, 0), (6, 2, 80, 90), (8, 2, 64, 1), (32, 8, 128, 0), (9, 3, 128, 33), (2, 1, 256, 70), (17, 1, 96, 0)])
+def test_runs_by_either_kernel(monkeypatch, directly, heads, kv_heads, dim, window):
+    """Runs worked on like single tokens and runs over pages laid out in 16 bits, whichever the rule would take: runs of one and of many tokens, a token over two blocks, ranges that no
+    column of a block sees."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: bool(directly))
+    check_attention([(0, 7), (100, 1), (60, 9), (130, 66), (500, 3)], heads, kv_heads, dim, window)
+    check_attention([(3000, 5), (0, 2)], heads, kv_heads, dim, window, seed=4)
+
+
+@pytest.mark.parametrize("directly", [0, 1])
+@pytest.mark.parametrize("kv_heads, dim", [(2, 32), (1, 64), (2, 128), (1, 256)])
+def test_what_later_tokens_hold_reaches_no_earlier_one(monkeypatch, directly, kv_heads, dim):
+    """A key and a value of new tokens that are not finite: the tokens before them are as without them, those behind see NaN."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: bool(directly))
+    torch.manual_seed(dim)
+    for at, what in ((40, "key"), (41, "value")):
+        results = []
+        for spoiled in (False, True):
+            cache = Cache(4, kv_heads, dim, [2, 1])
+            keys, values = random_rows(110, kv_heads, dim, 3)
+            if spoiled:
+                (keys if what == "key" else values)[at] = float("nan")
+            cache.store([(0, 100), (0, 10)], keys, values)
+            queries = torch.randn(110, 2 * kv_heads * dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+            out = torch.empty_like(queries)
+            kernels.attention8(queries, *cache.pages, out, make_step([(0, 100), (0, 10)]), cache.rows, 2 * kv_heads, kv_heads, dim, dim ** -0.5, 0)
+            results.append(out.float())
+        assert torch.equal(results[0][:at], results[1][:at]) and torch.equal(results[0][100:], results[1][100:]) and bool(results[1][at:100].isnan().all())
+
+
 def test_many_single_tokens_and_a_long_context():
     check_attention([(index * 7 % 150, 1) for index in range(70)], 8, 4, 64, 0, seed=2)
     check_attention([(9000, 1)], 2, 1, 64, 0, seed=3)

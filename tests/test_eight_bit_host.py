@@ -215,3 +215,10 @@ def test_ranges_of_a_decode_over_8_bit_pages():
         for length in (1, 65, 1000, 33000, 1 << 20):
             found = splits(n_seqs, length, 8, 148)
             assert 1 <= found <= 64 and found <= max(1, (1 << (length - 1).bit_length()) // 64)
+
+
+def test_which_runs_are_worked_on_like_single_tokens():
+    rule = kernels.runs8_like_single_tokens
+    assert rule(4, 16, 4500, 32, 8, 128) and not rule(4, 17, 4500, 32, 8, 128)      # 64 and 68 columns
+    assert rule(4, 40, 4500, 32, 8, 80) and not rule(4, 41, 4500, 32, 8, 80)        # 160 and 164
+    assert rule(1, 64, 500, 32, 8, 128) and not rule(1, 256, 500, 32, 8, 128)       # 8 heads x 8 pages x 16 readings, x 64
