@@ -191,8 +191,10 @@ __device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__
                                             int lane) {
     if (weight) {
         float squares = 0.0f;
-        // In the order of the 16-bit cache's prepare kernel, so that a key is the same before it is rounded to 8 bits: neighbours to a lane where 32 divides the head, else strides of 32.
-        const int per = D % 32 == 0 ? D / 32 : 1, begin = per > 1 ? lane * per : lane, end = per > 1 ? begin + per : D, by = per > 1 ? 1 : 32;
+        // In the order of the 16-bit cache's prepare kernel, so that a key is the same before it is rounded to 8 bits: neighbours to a lane in heads of 64, 128 and 256 that are rotated
+        // whole or not at all, else strides of 32.
+        const bool neighbours = (D == 64 || D == 128 || D == 256) && (rotary_dim == 0 || rotary_dim == D);
+        const int per = neighbours ? D / 32 : 1, begin = per > 1 ? lane * per : lane, end = per > 1 ? begin + per : D, by = per > 1 ? 1 : 32;
         for (int e = begin; e < end; e += by) {
             const float value = to_float(row[e]);
             squares += value * value;

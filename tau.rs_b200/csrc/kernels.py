@@ -88,7 +88,7 @@ _CLASS_OF = {
     "side_gate": "activation", "unit_add_mix": "norm", "norm_rows": "norm", "relu_squared": "activation",
     "short_conv": "recurrence", "delta_prepare": "recurrence", "delta_rule": "recurrence", "selective_scan": "recurrence",
     "masked_prepare": "attention", "masked_attention": "attention", "talking_decode": "attention", "shared_key_decode": "attention", "gated_rows": "attention",
-    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gemm8_skinny": "product", "gemm8_tc": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
+    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gemm8_skinny": "product", "gemm8_stream": "product", "gemm8_tc": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
     "token_shift": "recurrence", "tanh": "activation", "channel_decay": "recurrence", "wkv": "recurrence", "forget_gates": "recurrence", "turn_heads": "recurrence",
 }
 _timing = None     # while timing: [last event, [(class, event after the launch), ...]]
@@ -1123,17 +1123,16 @@ def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
                _stream_handle()), "gemm8_simt")
 
 
-SKINNY8_FUSED_ROWS = 8      # up to here the skinny kernel can quantise the activations itself ...
-SKINNY8_FUSED_WEIGHT = 8 << 20   # ... and does where the weight is small: a launch less (1 x 1,024 x 4,096 2.8 us against 2.1 and 1.3), but each block quantises for itself (8 x
-                            # 4,096 x 6,144 8.6 us against 6.2 and 1.4, 24,576 26.9 against 22.4 and 1.4)
-SKINNY8_MAX_ROWS = 32       # what it accepts quantised
-SKINNY8_SMALL_ROWS = 16     # up to here it beats the tensor-core product where the weight is small (16 x 1,024 x 4,096 2.5 us against 5.2; 16 x 4,096 x 24,576 30 against 27)
+STREAM8_MAX_ROWS = 8        # rows of the streaming product, which quantises them itself ...
+STREAM8_MAX_DEPTH = 12288   # ... and keeps their codes in shared memory
+SKINNY8_MAX_ROWS = 16       # of the other product for few rows, and where it beats the tensor-core product if the weight has at most so many elements (16 x 1,024 x 4,096 2.5 us against
+SKINNY8_SMALL_WEIGHT = 8 << 20   # 5.2; 16 x 4,096 x 24,576 30 against 27)
 
 
-def _skinny8(x: int, x_stride: int, x_scales, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
-    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "iplpppppiiilif")
+def _skinny8(x: int, x_scales: int, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
+    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "ippppppiiilif")
     features, depth = codes.shape
-    _check(run(_DTYPE_CODE[out.dtype], x, x_stride, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, features, depth, out.stride(0),
+    _check(run(_DTYPE_CODE[out.dtype], x, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, features, depth, out.stride(0),
                1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
 
 
@@ -1143,10 +1142,23 @@ def _tc8(x: int, x_scales: int, rows: int, codes, scales, bias, out, gated: bool
                1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
 
 
-def gemm8_skinny(values, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
-    """The product for a few rows, bound by streaming the weight's codes once: bfloat16 rows (`x_scales` None, at most 8) or quantised ones (at most 32)."""
-    _require(values.shape[0] <= (SKINNY8_FUSED_ROWS if x_scales is None else SKINNY8_MAX_ROWS), "too many rows for the skinny kernel")
-    _skinny8(values.data_ptr(), values.stride(0), _address(x_scales), values.shape[0], codes, scales, bias, out, gated, gate_limit)
+def gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
+    """The product of at most 16 quantised rows, bound by streaming the weight's codes once."""
+    _require(x_codes.shape[0] <= SKINNY8_MAX_ROWS, "too many rows for the skinny kernel")
+    _skinny8(x_codes.data_ptr(), x_scales.data_ptr(), x_codes.shape[0], codes, scales, bias, out, gated, gate_limit)
+
+
+def _stream8(values, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
+    run = _function("gemm8_skinny.cu", "tau_gemm8_stream", "iplppppiiilif")
+    _check(run(_DTYPE_CODE[out.dtype], values.data_ptr(), values.stride(0), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), values.shape[0], codes.shape[0],
+               codes.shape[1], out.stride(0), 1 if gated else 0, gate_limit, _stream_handle()), "gemm8_stream")
+
+
+def gemm8_stream(values, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
+    """The product of at most 8 bfloat16 rows: a block to an SM, which quantises the rows once and streams its share of the weight's codes."""
+    _require(values.dtype == torch.bfloat16 and values.shape[0] <= STREAM8_MAX_ROWS and codes.shape[1] <= STREAM8_MAX_DEPTH,
+             f"the streaming product takes at most {STREAM8_MAX_ROWS} bfloat16 rows of at most {STREAM8_MAX_DEPTH} columns")
+    _stream8(values, codes, scales, bias, out, gated, gate_limit)
 
 
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
@@ -1172,17 +1184,16 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
         gemm8_simt(*quantize_rows(values), codes, scales, None, stacked)
         run = _function("eight_bit.cu", "tau_gate_groups", "pplilf")
         return _check(run(stacked.data_ptr(), out.data_ptr(), rows, features // 2, out.stride(0), limit, _stream_handle()), "gate_groups")
-    small = features * depth <= SKINNY8_FUSED_WEIGHT
-    if small and rows <= SKINNY8_FUSED_ROWS and values.dtype is torch.bfloat16:
-        return _skinny8(values.data_ptr(), values.stride(0), None, rows, codes, scales, bias, out, gated, limit)
+    if rows <= STREAM8_MAX_ROWS and depth <= STREAM8_MAX_DEPTH and values.dtype is torch.bfloat16:
+        return _stream8(values, codes, scales, bias, out, gated, limit)
     # The activations' codes and, behind them, their scales, in one piece of memory.
     held = torch.empty(rows * (depth + 4 * -(-depth // SCALE_BLOCK)), dtype=torch.uint8, device=values.device)
     x = held.data_ptr()
     x_scales = x + rows * depth
     run = _function("eight_bit.cu", "tau_quantize_rows", "iplppii")
     _check(run(_DTYPE_CODE[values.dtype], values.data_ptr(), values.stride(0), x, x_scales, rows, depth, _stream_handle()), "quantize_rows")
-    if rows <= SKINNY8_FUSED_ROWS or (small and rows <= SKINNY8_SMALL_ROWS):
-        return _skinny8(x, depth, x_scales, rows, codes, scales, bias, out, gated, limit)
+    if rows <= STREAM8_MAX_ROWS or (rows <= SKINNY8_MAX_ROWS and features * depth <= SKINNY8_SMALL_WEIGHT):
+        return _skinny8(x, x_scales, rows, codes, scales, bias, out, gated, limit)
     _tc8(x, x_scales, rows, codes, scales, bias, out, gated, limit, 0, 0)
 
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import plain_eight_bit as plain
-from tau_rs_b200.csrc import kernels
+from tau_rs_b200.csrc import build, kernels
 from tau_rs_b200.engine.batch import StepContext
 
 pytestmark = pytest.mark.gpu
@@ -47,7 +47,7 @@ def product_bound(x, w, exact, out_dtype):
 
 
 SIZES = [(1, 16, 16), (1, 1024, 4096), (3, 144, 130), (7, 2000, 257), (8, 4096, 528), (9, 272, 1000), (16, 1104, 384), (17, 128, 2048), (33, 1040, 300), (64, 2048, 512),
-         (100, 416, 1500), (128, 256, 256), (129, 640, 272), (200, 4112, 640), (257, 1024, 1040), (600, 528, 2064)]
+         (100, 416, 1500), (128, 256, 256), (129, 640, 272), (200, 4112, 640), (257, 1024, 1040), (600, 528, 2064), (4, 12416, 144), (14, 12416, 130)]
 
 
 @pytest.mark.parametrize("rows, depth, features", SIZES)
@@ -115,6 +115,32 @@ def test_every_tile_of_the_tensor_core_product(rows, depth, features, tile, rang
         assert bool(((out[:, : features // 2].double() - wanted).abs() <= bound).all()), float(((out[:, : features // 2].double() - wanted).abs() / bound).max())
         assert bool((out[:, features // 2 :] == 7.0).all())
     assert kernels.gemm8_tc_status() == 0
+
+
+@pytest.mark.parametrize("rows, depth, features", [(1, 16, 16), (8, 4096, 530), (3, 400, 4112), (7, 12288, 272), (5, 2064, 5000), (2, 12176, 40)])
+def test_the_streaming_product(rows, depth, features):
+    """One group of features and many to a block, fewer chunks of K than warps, a last chunk that is cut, the deepest K; against the statement, and gated against itself."""
+    x, w = spread_values(rows, depth, seed=depth, outliers=False).to(torch.bfloat16), (spread_values(features, depth, seed=features, outliers=False) * depth ** -0.5).to(torch.bfloat16)
+    offset = spread_values(features, seed=3, outliers=False).cuda()
+    codes, scales = kernels.quantize_blocks(w.cuda())
+    held_x, held_w = plain.held_rows(x)[0].cuda(), plain.held_blocks(w)[0].cuda()
+    exact = held_x @ held_w.T + offset.double()
+    wide = torch.zeros(rows, depth + 16, dtype=torch.bfloat16, device="cuda")
+    wide[:, :depth] = x.cuda()
+    assert build.load_library("gemm8_skinny.cu").tau_gemm8_stream_most_depth() >= kernels.STREAM8_MAX_DEPTH
+    for out_dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((rows, features + 3), 7.0, device="cuda", dtype=out_dtype)
+        kernels.gemm8_stream(wide[:, :depth], codes, scales, offset, out[:, :features])
+        bound = product_bound(held_x, held_w, exact, out_dtype) + 2.0 ** -24 * exact.abs().max()
+        assert bool(((out[:, :features].double() - exact).abs() <= bound).all()) and bool((out[:, features:] == 7.0).all())
+    if features % 16 == 0:
+        stacked, out = torch.empty(rows, features, device="cuda", dtype=torch.bfloat16), torch.empty(rows, features // 2, device="cuda", dtype=torch.bfloat16)
+        kernels.gemm8_stream(wide[:, :depth], codes, scales, None, stacked)
+        kernels.gemm8_stream(wide[:, :depth], codes, scales, None, out, gated=True)
+        gate, up = (stacked.double().view(rows, -1, 2, 8)[:, :, i].reshape(rows, -1) for i in (0, 1))
+        wanted = torch.nn.functional.silu(gate) * up
+        bound = (2.0 ** -8 + 2.0 ** -23 * (6.0 + 1.173 * gate.abs())) * wanted.abs() + 2.0 ** -126 * (gate * up).abs() + 1e-37      # as above
+        assert bool(((out.double() - wanted).abs() <= bound).all())
 
 
 def test_a_row_that_is_not_finite_stays_alone():
