@@ -47,7 +47,23 @@ struct Shared {
     uint64_t empty[kStages];
     float key_scale[kStages], share[kStages], older[kStages];
     float unit;
+    uint64_t stored;                              // the newest position is in its page
+    float new_key_scale, new_value_scale;         // that page's scales
     int abort_flag;
+};
+
+// What the kernel needs to prepare single tokens itself: queries, and where `store` is set keys and values, come as a stacked projection left them, [sequences,
+// (n_heads + 2 n_kv_heads) D]; they are normalised per head, rotated, and the newest key and value enter their pages.  `projected` == nullptr: queries are ready, the cache complete.
+struct Prepare {
+    const bf16* projected;
+    long long stride;
+    const float* q_weight;
+    const float* k_weight;
+    float eps;
+    const float* cos_table;
+    const float* sin_table;
+    int rotary_dim;
+    int store;
 };
 
 __device__ __forceinline__ void tma_load_3d(void* destination, const CUtensorMap* map, int x, int y, int z, uint64_t* barrier) {
@@ -88,10 +104,9 @@ constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a l
 template <int NT, bool Runs>
 __global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 && !Runs ? 4 : 2)
 decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
-               const float* __restrict__ key_scales, const float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
+               uint8_t* __restrict__ key_pages, uint8_t* __restrict__ value_pages, float* __restrict__ key_scales, float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                const int* __restrict__ seq_len, const int* __restrict__ cu_seqlens, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale,
-               int window, int splits, int clustered) {
-    grid_dependents_launch();
+               int window, int splits, int clustered, Prepare prepare) {
     constexpr int kHeads = 8 * NT;
     extern __shared__ uint8_t shared_raw[];
     Shared* shared = reinterpret_cast<Shared*>(shared_raw);
@@ -101,6 +116,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     static_assert(kWarps * kHeads * D * 4 <= kStages * kStageBytes, "the join must fit the stages");
     __shared__ float merge_ml[kWarps][kHeads][2];
     __shared__ float block_ml[kHeads][2];
+    __shared__ __align__(16) bf16 own[Runs ? 1 : kHeads + 2][D];      // prepared here: queries, then the newest key and value
+    __shared__ float greatest_of[2 * kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x, seq = blockIdx.z;
@@ -112,6 +129,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             barrier_init(&shared->full[s], 2);      // the copies', and the scales'
             barrier_init(&shared->empty[s], kWarps);
         }
+        barrier_init(&shared->stored, kWarps);
         shared->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -132,6 +150,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     const int per_split = (max(0, pages_end - first_page) + splits - 1) / splits;
     const int page_lo = first_page + split * per_split, page_hi = min(pages_end, page_lo + per_split);
     const int count = max(0, page_hi - page_lo);
+    // The range with the newest position: nobody else reads that page of that head.
+    const bool stores = !Runs && prepare.projected != nullptr && prepare.store && count > 0 && page_hi == pages_end;
     float running_max[NT][2], running_sum[NT][2];      // log2 units; the sums and accumulators belong to weights exp2(score - max + 14)
     float unit = 0.0f;      // producer: what one in the accumulators stands for, the greatest value scale of the pages so far
     float acc[NT][kValueRounds][8][4];
@@ -165,6 +185,10 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     alive = false;
                     break;
                 }
+                if (stores && number == count - 1 && !__all_sync(0xffffffffu, barrier_wait(&shared->stored, 0, abort_flag))) {
+                    alive = false;
+                    break;
+                }
                 if (lane == 0) {
                     barrier_expect_bytes(&shared->full[stage], kStageBytes);
                     uint8_t* tile = stages + stage * kStageBytes;
@@ -177,7 +201,11 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 // The scales of the stages that were free from the start follow once all their copies are on their way.
                 if (number < kStages - 1 && number + 1 < count) continue;
                 for (int n = number < kStages ? 0 : number; n <= number; ++n) {
-                    const float k_of = __shfl_sync(0xffffffffu, k_scale, n - base), v_of = __shfl_sync(0xffffffffu, v_scale, n - base);
+                    float k_of = __shfl_sync(0xffffffffu, k_scale, n - base), v_of = __shfl_sync(0xffffffffu, v_scale, n - base);
+                    if (stores && n == count - 1) {
+                        k_of = shared->new_key_scale;
+                        v_of = shared->new_value_scale;
+                    }
                     // A page's value scale joins the weights as its share of the accumulators' unit (powers of two: exact), so a unit that grows rescales them.
                     const float grown = fmaxf(unit, v_of);
                     if (lane == 0) {
@@ -195,6 +223,35 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         if (!alive && lane == 0)      // giving up: the copies in flight own their stages until they have landed
             for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
     } else {
+        if (!Runs && prepare.projected != nullptr && count > 0) {
+            // ---- the token's own rows, one to a warp at a time
+            const int position = length - 1;
+            const bf16* from = prepare.projected + static_cast<size_t>(seq) * prepare.stride;
+            const float* cosines = prepare.cos_table + static_cast<size_t>(position) * (prepare.rotary_dim / 2);
+            const float* sines = prepare.sin_table + static_cast<size_t>(position) * (prepare.rotary_dim / 2);
+            for (int task = warp; task < heads_here + (stores ? 2 : 0); task += kWarps) {
+                const bool is_key = task == heads_here, is_value = task == heads_here + 1;
+                const int head = is_key ? n_heads + kv_head : is_value ? n_heads + n_kv_heads + kv_head : kv_head * group + task;
+                bf16* row = own[is_key ? kHeads : is_value ? kHeads + 1 : task];
+                for (int e = lane; e < D; e += 32) row[e] = from[static_cast<size_t>(head) * D + e];
+                __syncwarp();
+                prepare_row(row, is_value ? nullptr : is_key ? prepare.k_weight : prepare.q_weight, prepare.eps, cosines, sines, is_value ? 0 : prepare.rotary_dim, D, lane);
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");      // every consumer warp comes here before any of its waits
+            if (stores) {
+                const size_t place_of = static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + position / kPage]) * n_kv_heads + kv_head;
+                const int older = position % kPage;
+                const float k_of = store_in_page<false>(own[Runs ? 0 : kHeads], 1, D, older, key_pages + place_of * kPage * D, key_scales + place_of, greatest_of, kWarps * 32);
+                const float v_of = store_in_page<false>(own[Runs ? 0 : kHeads + 1], 1, D, older, value_pages + place_of * kPage * D, value_scales + place_of, greatest_of + kWarps, kWarps * 32);
+                if (threadIdx.x == 0) {
+                    key_scales[place_of] = shared->new_key_scale = k_of;
+                    value_scales[place_of] = shared->new_value_scale = v_of;
+                }
+                asm volatile("fence.proxy.async;" ::: "memory");      // the page is read back by a copy
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&shared->stored);
+            }
+        }
         // ---- queries: this lane's elements of heads g (and g + 8), brought to [1, 2) per head
         unsigned q_frag[NT][kKeySteps][2];
         float q_power[NT];
@@ -202,7 +259,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         for (int n = 0; n < NT; ++n) {
             const int head = n * 8 + g;
             const bool live = head < heads_here && count > 0;
-            const bf16* row = queries + place(live ? head : 0) * D;
+            const bf16* row = !Runs && prepare.projected != nullptr ? own[live ? head : 0] : queries + place(live ? head : 0) * D;
             float greatest = 0.0f;
 #pragma unroll
             for (int step = 0; step < kKeySteps; ++step) {
@@ -430,6 +487,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             }
     }
     __syncthreads();      // the stages are done with
+    grid_dependents_launch();      // only now: what starts beside this kernel takes room that its own later blocks, or clusters, wait for
     if (warp < kWarps) {
         const float one = shared->unit;
 #pragma unroll
@@ -519,7 +577,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     cluster_sync_all();      // nobody leaves while its results are read
 }
 
-// Joins the records of a sequence's ranges in their order: a block to a head, a thread to a column.
+// Joins the records of a sequence's ranges in their order: a block (of whole warps) to a head, a thread to a column.
 __global__ void join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out, int n_heads, int splits) {
     grid_dependents_launch();
     grid_dependency_wait();
@@ -570,12 +628,13 @@ constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + 
 struct Call {
     const bf16* queries;
     bf16* out;
-    const float *key_scales, *value_scales;
-    float *partial_o, *partial_ml;
+    uint8_t *key_pages, *value_pages;
+    float *key_scales, *value_scales, *partial_o, *partial_ml;
     const int *seq_len, *cu_seqlens, *page_rows;
     int page_stride, n_seqs, n_tokens, n_heads, n_kv_heads, passes;
     float scale;
     int window, splits;
+    Prepare prepare;
 };
 
 template <int NT, bool Runs>
@@ -591,15 +650,17 @@ int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call&
     }
     const dim3 grid(c.splits, c.n_kv_heads * c.passes, c.n_seqs);
     const bool clustered = c.splits > 1 && c.splits <= kMostClustered;
+    // Beside the kernel before it only where all blocks find room at once (8 sequences of 2,048 positions 14.4 -> 13.9 us; 640 blocks of 40 sequences 73 -> 78).
+    const bool early = static_cast<long long>(grid.x) * grid.y * grid.z <= 148ll * (NT == 1 && kHalves == 1 && !Runs ? 4 : 2);
     int code;
     if (clustered)
-        code = tau_launch_clusters_as(false, c.splits, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_scales, c.value_scales,
-                                      c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1);
+        code = tau_launch_clusters_as(early, c.splits, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales,
+                                      c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1, c.prepare);
     else
-        code = tau_launch_as(false, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_scales, c.value_scales, c.partial_o,
-                             c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0);
+        code = tau_launch_as(early, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales, c.partial_o,
+                             c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0, c.prepare);
     if (code == 0 && c.splits > kMostClustered)
-        code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? D : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
+        code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? (D + 31) / 32 * 32 : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
     return code ? code : tau_launch_status();
 }
 
@@ -616,26 +677,30 @@ TAU_EXPORT int tau_decode8_status() {
 }
 
 // bfloat16 queries and output [tokens, n_heads D]; pages [boxes / n_kv_heads, n_kv_heads, 64, D] of e4m3 codes with scales [boxes].  `cu_seqlens` == nullptr: one token to
-// a sequence; else the runs' bounds, none longer than `max_new`.  More than 8 splits need scratch of n_tokens * n_heads * splits * (D + 2) floats.
-TAU_EXPORT int tau_decode8(const void* queries, const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* out, const int* seq_len,
+// a sequence; else the runs' bounds, none longer than `max_new`.  `projected` != nullptr (single tokens, a group of query heads that one block serves):
+// `queries` is not read, see `Prepare`.  More than 8 splits need scratch of n_tokens * n_heads * splits * (D + 2) floats.
+TAU_EXPORT int tau_decode8(const void* queries, void* key_pages, void* value_pages, float* key_scales, float* value_scales, void* out, const int* seq_len,
                            const int* cu_seqlens, const int* page_rows, int page_stride, long long boxes, int n_seqs, int n_tokens, int max_new, int n_heads, int n_kv_heads, float scale,
-                           int window, int splits, float* scratch, long long scratch_floats, void* stream) {
+                           int window, int splits, float* scratch, long long scratch_floats, const void* projected, long long projected_stride, const float* q_weight, const float* k_weight,
+                           float eps, const float* cos_table, const float* sin_table, int rotary_dim, int store, void* stream) {
     if (n_seqs <= 0 || n_tokens <= 0) return 0;
-    if (!queries || !key_pages || !value_pages || !key_scales || !value_scales || !out || !seq_len || !page_rows || page_stride <= 0 || boxes <= 0 || n_heads <= 0 || n_kv_heads <= 0 ||
+    if ((!queries && !projected) || !key_pages || !value_pages || !key_scales || !value_scales || !out || !seq_len || !page_rows || page_stride <= 0 || boxes <= 0 || n_heads <= 0 || n_kv_heads <= 0 ||
         n_heads % n_kv_heads != 0 || window < 0 || splits < 1 || splits > 256 || n_seqs > 65535 || n_tokens > 65535 || max_new < 1 || (!cu_seqlens && (max_new != 1 || n_tokens != n_seqs)) ||
         boxes > 0x7fffffffll || (reinterpret_cast<uintptr_t>(queries) & 7) ||
+        (projected && (cu_seqlens || rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) || (rotary_dim > 0 && (!cos_table || !sin_table)))) ||
         (splits > kMostClustered && (!scratch || scratch_floats < static_cast<long long>(n_tokens) * n_heads * splits * (D + 2))))
         return cudaErrorInvalidValue;
     const long long columns = static_cast<long long>(n_heads / n_kv_heads) * max_new;
     const int to_a_block = columns_to_a_block(columns);
-    if (n_kv_heads * ((columns + to_a_block - 1) / to_a_block) > 65535) return cudaErrorInvalidValue;
+    if (n_kv_heads * ((columns + to_a_block - 1) / to_a_block) > 65535 || (projected && columns > to_a_block)) return cudaErrorInvalidValue;      // a page is stored by one block alone
     CUtensorMap key_map, value_map;
     int status = page_map(&key_map, key_pages, boxes);
     if (!status) status = page_map(&value_map, value_pages, boxes);
     if (status) return status;
-    const Call call = {static_cast<const bf16*>(queries), static_cast<bf16*>(out), key_scales, value_scales, scratch,
+    const Call call = {static_cast<const bf16*>(queries), static_cast<bf16*>(out), static_cast<uint8_t*>(key_pages), static_cast<uint8_t*>(value_pages), key_scales, value_scales, scratch,
                        scratch ? scratch + static_cast<size_t>(n_tokens) * n_heads * splits * D : nullptr, seq_len, cu_seqlens, page_rows, page_stride, n_seqs, n_tokens, n_heads, n_kv_heads,
-                       static_cast<int>((columns + to_a_block - 1) / to_a_block), scale, window, splits};
+                       static_cast<int>((columns + to_a_block - 1) / to_a_block), scale, window, splits,
+                       {static_cast<const bf16*>(projected), projected_stride, q_weight, k_weight, eps, cos_table, sin_table, rotary_dim, store}};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if constexpr (D <= 128)
         if (to_a_block == 16) return cu_seqlens ? launch<2, true>(key_map, value_map, call, s) : launch<2, false>(key_map, value_map, call, s);

@@ -186,32 +186,6 @@ struct StoreSource {
 };
 constexpr int kQueryHeads = 4;      // query heads to a block
 
-// One warp: norm and rotation of one head, in place (shared memory).
-__device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__ weight, float eps, const float* __restrict__ cosines, const float* __restrict__ sines, int rotary_dim, int D,
-                                            int lane) {
-    if (weight) {
-        float squares = 0.0f;
-        // In the order of the 16-bit cache's prepare kernel, so that a key is the same before it is rounded to 8 bits: neighbours to a lane in heads of 64, 128 and 256 that are rotated
-        // whole or not at all, else strides of 32.
-        const bool neighbours = (D == 64 || D == 128 || D == 256) && (rotary_dim == 0 || rotary_dim == D);
-        const int per = neighbours ? D / 32 : 1, begin = per > 1 ? lane * per : lane, end = per > 1 ? begin + per : D, by = per > 1 ? 1 : 32;
-        for (int e = begin; e < end; e += by) {
-            const float value = to_float(row[e]);
-            squares += value * value;
-        }
-        const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + eps);
-        for (int e = lane; e < D; e += 32) row[e] = __float2bfloat16_rn(to_float(row[e]) * inverse * weight[e]);
-        __syncwarp();
-    }
-    const int half = rotary_dim / 2;
-    for (int j = lane; j < half; j += 32) {      // a pair is one lane's
-        const float first = to_float(row[j]), second = to_float(row[j + half]), c = cosines[j], s = sines[j];
-        row[j] = __float2bfloat16_rn(first * c - second * s);
-        row[j + half] = __float2bfloat16_rn(second * c + first * s);
-    }
-    __syncwarp();
-}
-
 // All threads: `count` rows of D elements, `stride` apart, one behind the other in shared memory; 16 bytes at a time and four such loads on their way where the rows allow it.
 __device__ __forceinline__ void stage_rows(const bf16* __restrict__ source, long long stride, int count, int D, bf16* staged) {
     if (((reinterpret_cast<uintptr_t>(source) | static_cast<uintptr_t>(stride * 2)) & 15) == 0) {
@@ -327,43 +301,7 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
         }
         __syncthreads();
     }
-    float greatest = 0.0f;
-    for (int piece = threadIdx.x; piece < count * D / 8; piece += 256) {
-        const uint4 raw = reinterpret_cast<const uint4*>(staged)[piece];
-        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) greatest = fmaxf(greatest, fmaxf(finite_magnitude(__uint_as_float(words[i] << 16)), finite_magnitude(__uint_as_float(words[i] & 0xffff0000u))));
-    }
-    greatest = warp_max(greatest);
-    if (lane == 0) greatest_of[warp] = greatest;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) greatest = fmaxf(greatest, greatest_of[w]);
-    float scale = power_of_two(scale_exponent(greatest));
-    if (older > 0) {      // the page holds positions of this sequence: its scale counts, and grows where the new ones need it
-        const float kept = fmaxf(*scale_at, kLeastScale);
-        if (kept >= scale) {
-            scale = kept;
-        } else {
-            const float ratio = kept / scale;      // powers of two
-            for (int piece = threadIdx.x; piece < older * D / 4; piece += 256) {
-                unsigned* word = reinterpret_cast<unsigned*>(page) + piece;
-                float v[4];
-                decode_four(*word, v);
-                *word = encode_four(v[0], v[1], v[2], v[3], ratio);
-            }
-        }
-    }
-    const float inverse = 1.0f / scale;
-    for (int piece = threadIdx.x; piece < count * D / 8; piece += 256) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(staged + piece * 8);
-        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint2 codes;
-        codes.x = encode_four(__uint_as_float(words[0] << 16), __uint_as_float(words[0] & 0xffff0000u), __uint_as_float(words[1] << 16), __uint_as_float(words[1] & 0xffff0000u), inverse);
-        codes.y = encode_four(__uint_as_float(words[2] << 16), __uint_as_float(words[2] & 0xffff0000u), __uint_as_float(words[3] << 16), __uint_as_float(words[3] & 0xffff0000u), inverse);
-        *reinterpret_cast<uint2*>(page + static_cast<size_t>(older) * D + piece * 8) = codes;
-    }
-    __syncthreads();      // every thread has read the old scale
+    const float scale = store_in_page(staged, count, D, older, page, scale_at, greatest_of, 256);
     if (threadIdx.x == 0) *scale_at = scale;
 }
 

@@ -65,4 +65,75 @@ __device__ __forceinline__ unsigned pack_bf16_pair(float low, float high) {
     return *reinterpret_cast<const unsigned*>(&pair);
 }
 
+// One warp: norm and rotation of one head, in place (shared memory).
+__device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__ weight, float eps, const float* __restrict__ cosines, const float* __restrict__ sines, int rotary_dim, int D,
+                                            int lane) {
+    if (weight) {
+        float squares = 0.0f;
+        // In the order of the 16-bit cache's prepare kernel, so that a key is the same before it is rounded to 8 bits: neighbours to a lane in heads of 64, 128 and 256 that are rotated
+        // whole or not at all, else strides of 32.
+        const bool neighbours = (D == 64 || D == 128 || D == 256) && (rotary_dim == 0 || rotary_dim == D);
+        const int per = neighbours ? D / 32 : 1, begin = per > 1 ? lane * per : lane, end = per > 1 ? begin + per : D, by = per > 1 ? 1 : 32;
+        for (int e = begin; e < end; e += by) {
+            const float value = to_float(row[e]);
+            squares += value * value;
+        }
+        const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + eps);
+        for (int e = lane; e < D; e += 32) row[e] = __float2bfloat16_rn(to_float(row[e]) * inverse * weight[e]);
+        __syncwarp();
+    }
+    const int half = rotary_dim / 2;
+    for (int j = lane; j < half; j += 32) {      // a pair is one lane's
+        const float first = to_float(row[j]), second = to_float(row[j + half]), c = cosines[j], s = sines[j];
+        row[j] = __float2bfloat16_rn(first * c - second * s);
+        row[j + half] = __float2bfloat16_rn(second * c + first * s);
+    }
+    __syncwarp();
+}
+
+// `threads` threads of a block (numbers 0 .. threads - 1, all of its threads if `whole_block`, else its first four warps) bring `count` rows of D elements in shared memory into a page of one head, behind the `older`
+// positions that it holds: the scale is the page's own (none for a page that starts here) or what the new rows need, whichever is greater, and codes that are there are rounded to
+// one that grew.  Returns the page's scale, which one thread then writes to `scale_at`; every thread has read the old one by then.  `greatest_of`: a float for each warp.
+template <bool WholeBlock = true>
+__device__ __forceinline__ float store_in_page(const bf16* rows, int count, int D, int older, uint8_t* page, const float* scale_at, float* greatest_of, int threads) {
+    auto meet = [&]() {
+        if constexpr (WholeBlock) __syncthreads();
+        else asm volatile("bar.sync 1, 128;" ::: "memory");
+    };
+    float greatest = 0.0f;
+    for (int piece = threadIdx.x; piece < count * D / 8; piece += threads) {
+        const uint4 raw = reinterpret_cast<const uint4*>(rows)[piece];
+        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) greatest = fmaxf(greatest, fmaxf(finite_magnitude(__uint_as_float(words[i] << 16)), finite_magnitude(__uint_as_float(words[i] & 0xffff0000u))));
+    }
+    const float kept = older > 0 ? fmaxf(*scale_at, kLeastScale) : 0.0f;
+    greatest = warp_max(greatest);
+    if ((threadIdx.x & 31) == 0) greatest_of[threadIdx.x >> 5] = greatest;
+    meet();
+    for (int w = 0; w < threads / 32; ++w) greatest = fmaxf(greatest, greatest_of[w]);
+    float scale = power_of_two(scale_exponent(greatest));
+    if (kept >= scale) {
+        scale = kept;
+    } else if (older > 0) {
+        const float ratio = kept / scale;      // powers of two
+        for (int piece = threadIdx.x; piece < older * D / 4; piece += threads) {
+            unsigned* word = reinterpret_cast<unsigned*>(page) + piece;
+            float v[4];
+            decode_four(*word, v);
+            *word = encode_four(v[0], v[1], v[2], v[3], ratio);
+        }
+    }
+    const float inverse = 1.0f / scale;
+    for (int piece = threadIdx.x; piece < count * D / 8; piece += threads) {
+        const uint4 raw = reinterpret_cast<const uint4*>(rows)[piece];
+        const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint2 codes;
+        codes.x = encode_four(__uint_as_float(words[0] << 16), __uint_as_float(words[0] & 0xffff0000u), __uint_as_float(words[1] << 16), __uint_as_float(words[1] & 0xffff0000u), inverse);
+        codes.y = encode_four(__uint_as_float(words[2] << 16), __uint_as_float(words[2] & 0xffff0000u), __uint_as_float(words[3] << 16), __uint_as_float(words[3] & 0xffff0000u), inverse);
+        *reinterpret_cast<uint2*>(page + static_cast<size_t>(older) * D + piece * 8) = codes;
+    }
+    return scale;
+}
+
 }  // namespace

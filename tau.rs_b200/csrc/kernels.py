@@ -1244,14 +1244,10 @@ def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales,
     eps, rotary_dim, n_heads = 0.0, 0, 0
     if prepare is not None:
         projected, queries, q_weight, k_weight, eps, cos, sin, rotary_dim, n_heads = prepare
-        _f32_vector(q_weight, head_dim, "the q norm weight")
-        _f32_vector(k_weight, head_dim, "the k norm weight")
+        _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim)
         _require(projected.dtype == torch.bfloat16 and projected.dim() == 2 and projected.shape[0] == step.n_tokens and projected.shape[1] >= n_heads * head_dim and projected.stride(1) == 1,
                  "projected rows must hold every query head in bfloat16")
         _require(queries.dtype == torch.bfloat16 and queries.shape == (step.n_tokens, n_heads * head_dim) and queries.is_contiguous(), "queries must be [tokens, n_heads * head_dim]")
-        if rotary_dim:
-            _require(rotary_dim % 2 == 0 and 0 < rotary_dim <= head_dim and cos is not None and sin is not None and cos.dtype == torch.float32 == sin.dtype and cos.shape == sin.shape
-                     and cos.shape[1] == rotary_dim // 2 and cos.is_contiguous() and sin.is_contiguous(), "rotation tables must be float32 [positions, rotary_dim / 2]")
     _here(keys, values, key_pages, value_pages, key_scales, value_scales, step.cu_seqlens, step.seq_start, page_rows, projected, queries, q_weight, k_weight, cos, sin)
     if step.n_tokens == 0:
         return
@@ -1305,20 +1301,63 @@ def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int]
     return DECODE8_CLUSTERED if DECODE8_CLUSTERED < splits < 12 else splits
 
 
-def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
-    """One query token per sequence over its `seq_len` cached positions, or a few, read as they are held (`attention8` checks its arguments)."""
+def _passes8(columns: int, head_dim: int) -> int:
+    """Times that `attention_decode8` reads the pages for so many columns (query heads of a group times new tokens)."""
+    return -(-columns // (16 if columns > 8 and head_dim <= 128 else 8))
+
+
+def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int,
+                      prepare=None) -> None:
+    """One query token per sequence over its `seq_len` cached positions, or a few, read as they are held (`attention8` and `attention8_decode_fused` check their arguments).
+    `prepare`: see there; `queries` is then None."""
     n_seqs, n_tokens = step.n_seqs, step.n_tokens
     single = step.all_single
-    columns = n_heads // n_kv_heads * (1 if single else step.max_new)
-    passes = -(-columns // (16 if columns > 8 and head_dim <= 128 else 8))
+    passes = _passes8(n_heads // n_kv_heads * (1 if single else step.max_new), head_dim)
     splits = min((step.decode_splits if single else 0) or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
     scratch = torch.empty(n_tokens * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
     run = _decode8_functions.get(head_dim)
     if run is None:
-        run = _decode8_functions[head_dim] = _function("attention_decode8.cu", "tau_decode8", "pppppppppiliiiiifiipl", (f"TAU_HEAD_DIM={head_dim}",))
-    _check(run(queries.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.seq_len.data_ptr(),
+        run = _decode8_functions[head_dim] = _function("attention_decode8.cu", "tau_decode8", "pppppppppiliiiiifiiplplppfppii", (f"TAU_HEAD_DIM={head_dim}",))
+    if prepare is None:
+        more = (None, 0, None, None, 0.0, None, None, 0, 0)
+    else:
+        projected, q_weight, k_weight, eps, cos, sin, rotary_dim, store = prepare
+        more = (projected.data_ptr(), projected.stride(0), _address(q_weight), _address(k_weight), eps, _address(cos), _address(sin), rotary_dim, 1 if store else 0)
+    _check(run(_address(queries), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.seq_len.data_ptr(),
                None if single else step.cu_seqlens.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], key_pages.shape[0] * n_kv_heads, n_seqs, n_tokens, 1 if single else step.max_new,
-               n_heads, n_kv_heads, scale, window, splits, _address(scratch), 0 if scratch is None else scratch.numel(), _stream_handle()), "attention_decode8", 1 if scratch is None else 2)
+               n_heads, n_kv_heads, scale, window, splits, _address(scratch), 0 if scratch is None else scratch.numel(), *more, _stream_handle()), "attention_decode8",
+           1 if scratch is None else 2)
+
+
+def attention8_decode_fused(projected, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, write_cache: bool, q_weight, k_weight, eps: float, cos, sin, rotary_dim: int,
+                            n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> bool:
+    """Norm, rotation, the store (`cache8_store`, unless another run stored this step's keys and values) and attention in one kernel, where that exists: one token to a sequence and a group
+    of query heads that one block serves.  Returns False (and does nothing) otherwise."""
+    group = n_heads // n_kv_heads if n_kv_heads > 0 else 0
+    if not (step.all_single and _prefer_optimized and group > 0 and _passes8(group, head_dim) == 1):
+        return False
+    _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
+    if key_pages.shape[1] != n_kv_heads or key_pages.shape[3] != head_dim or n_heads % n_kv_heads:
+        raise KernelError("the pages must be [pages, n_kv_heads, 64, head_dim] and n_heads a multiple of n_kv_heads")
+    needed = (n_heads + (2 * n_kv_heads if write_cache else 0)) * head_dim
+    if projected.dtype is not torch.bfloat16 or projected.dim() != 2 or projected.shape[0] != step.n_tokens or projected.shape[1] < needed or projected.stride(1) != 1:
+        raise KernelError(f"projected rows must hold {needed} bfloat16 elements")
+    if out.dtype is not torch.bfloat16 or out.shape != (step.n_tokens, n_heads * head_dim) or not out.is_contiguous() or window < 0:
+        raise KernelError("the output must be bfloat16 [tokens, n_heads * head_dim], and a window not negative")
+    _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim)
+    _here(projected, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_len, q_weight, k_weight, cos, sin)
+    if step.n_tokens:
+        attention_decode8(None, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window,
+                          prepare=(projected, q_weight, k_weight, eps, cos, sin, rotary_dim, write_cache))
+    return True
+
+
+def _check_rotation(q_weight, k_weight, cos, sin, rotary_dim: int, head_dim: int) -> None:
+    _f32_vector(q_weight, head_dim, "the q norm weight")
+    _f32_vector(k_weight, head_dim, "the k norm weight")
+    if rotary_dim and (rotary_dim % 2 or not 0 < rotary_dim <= head_dim or cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+                       or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise KernelError("rotation tables must be float32 [positions, rotary_dim / 2]")
 
 
 RUNS8_COLUMNS = 64          # of new tokens times a group's query heads, up to which runs are worked on like single tokens, 16 columns to a reading of the pages (us against pages laid

@@ -112,8 +112,11 @@ class Attention(Mixer):
         """The same over pages held in 8 bits: norm, rotation and the store, or the queries alone where another run stored keys and values, then attention."""
         spec = self.spec
         q_weight, k_weight, eps, cos, sin, rotary_dim = prepare
-        queries = torch.empty_like(context)
         held = (cache.keys, cache.values, cache.key_scales, cache.value_scales)
+        if kernels.attention8_decode_fused(projected, *held, context, step, pages, writes_cache, *prepare, spec.n_heads, spec.n_kv_heads, spec.head_dim, spec.softmax_scale,
+                                           spec.window or 0):
+            return context
+        queries = torch.empty_like(context)
         if writes_cache:
             keys = projected[:, self.q_width : self.q_width + self.kv_width].unflatten(1, (spec.n_kv_heads, spec.head_dim))
             values = projected[:, self.q_width + self.kv_width :].unflatten(1, (spec.n_kv_heads, spec.head_dim))

@@ -358,6 +358,7 @@ def test_single_tokens_with_a_given_number_of_splits(splits):
     """More splits than pages, ranges without a position, one sequence far longer than the others."""
     check_attention([(1500, 1), (0, 1), (64, 1), (700, 1)], 8, 2, 64, 0, seed=splits, splits=splits)
     check_attention([(1500, 1), (3, 1)], 4, 1, 128, 333, seed=splits, splits=splits)
+    check_attention([(600, 1), (3, 1)], 3, 3, 16, 0, seed=splits, splits=splits)
 
 
 @pytest.mark.parametrize("heads, kv_heads, dim", [(4, 2, 32), (6, 2, 80), (8, 2, 64), (32, 8, 128), (12, 1, 128), (2, 1, 256)])
@@ -401,6 +402,38 @@ def test_what_later_tokens_hold_reaches_no_earlier_one(monkeypatch, directly, kv
 def test_many_single_tokens_and_a_long_context():
     check_attention([(index * 7 % 150, 1) for index in range(70)], 8, 4, 64, 0, seed=2)
     check_attention([(9000, 1)], 2, 1, 64, 0, seed=3)
+
+
+@pytest.mark.parametrize("n_heads, n_kv_heads, dim, rotary, normed, window", [(4, 2, 32, 32, True, 0), (8, 8, 128, 128, True, 70), (32, 4, 64, 64, True, 0), (6, 2, 80, 40, True, 1), (16, 1, 128, 0, False, 0),
+                                                                               (8, 1, 256, 256, True, 100), (3, 3, 16, 8, False, 0)])
+@pytest.mark.parametrize("splits", [0, 1, 3, 8, 20])
+def test_single_tokens_stored_and_attended_in_one_kernel(n_heads, n_kv_heads, dim, rotary, normed, window, splits):
+    """Against the store and the attention one after the other, bit for bit: pages that start, end and are in the middle, scales that grow, several steps behind each other, and a run that
+    only reads what another stored."""
+    lengths = [0, 1, 62, 63, 64, 130, 300]
+    cache, straight = (Cache(7 * 5, n_kv_heads, dim, [5] * 7) for _ in range(2))
+    keys, values = random_rows(sum(lengths), n_kv_heads, dim, 2)
+    for each in (cache, straight):
+        if sum(lengths):
+            kernels.cache8_store(keys.cuda(), values.cuda(), *each.pages, make_step([(0, length) for length in lengths]), each.rows)
+    weights = [torch.rand(dim, device="cuda") + 0.5 if normed else None for _ in range(2)]
+    angles = torch.rand(512, rotary // 2, device="cuda") * 6 if rotary else None
+    cos, sin = (angles.cos(), angles.sin()) if rotary else (None, None)
+    for turn in range(3):
+        step = make_step([(length + turn, 1) for length in lengths])
+        step.decode_splits = splits
+        projected = torch.randn(7, (n_heads + 2 * n_kv_heads) * dim + 8, device="cuda").to(torch.bfloat16)[:, : (n_heads + 2 * n_kv_heads) * dim] * (4.0 ** turn)
+        queries, wanted, found = (torch.empty(7, n_heads * dim, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+        split = [projected[:, (n_heads + i * n_kv_heads) * dim : (n_heads + (i + 1) * n_kv_heads) * dim].unflatten(1, (n_kv_heads, dim)) for i in (0, 1)]
+        kernels.cache8_store(*split, *straight.pages, step, straight.rows, prepare=(projected, queries, *weights, 1e-6, cos, sin, rotary, n_heads))
+        kernels.attention8(queries, *straight.pages, wanted, step, straight.rows, n_heads, n_kv_heads, dim, dim ** -0.5, window)
+        numbers = (*weights, 1e-6, cos, sin, rotary, n_heads, n_kv_heads, dim, dim ** -0.5, window)
+        assert kernels.attention8_decode_fused(projected, *cache.pages, found, step, cache.rows, True, *numbers)
+        assert torch.equal(found, wanted)
+        for mine, theirs in zip(cache.pages, straight.pages):
+            assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8))
+        assert kernels.attention8_decode_fused(projected[:, : n_heads * dim], *cache.pages, found.zero_(), step, cache.rows, False, *numbers) and torch.equal(found, wanted)
+    assert not kernels.attention8_decode_fused(projected, *cache.pages, found, make_step([(0, 2)] * 7), cache.rows, True, *numbers)
 
 
 def test_attention_of_a_captured_step():
