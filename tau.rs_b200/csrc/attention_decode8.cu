@@ -64,6 +64,7 @@ struct Prepare {
     const float* sin_table;
     int rotary_dim;
     int store;
+    int vectors;      // heads of 64, 128 or 256 that are rotated whole or not at all, in rows on 16-byte borders
 };
 
 __device__ __forceinline__ void tma_load_3d(void* destination, const CUtensorMap* map, int x, int y, int z, uint64_t* barrier) {
@@ -134,6 +135,28 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    // Heads that are rotated whole (or not at all): a lane holds kNear neighbours of a row, and what it multiplies them with is here before the rows are.  (A step's lengths and the tables are
+    // there before its first kernel begins.)
+    constexpr bool kVectors = !Runs && (D == 64 || D == 128 || D == 256);
+    constexpr int kNear = kVectors ? D / 32 : 1;
+    __shared__ float rotation[2][kVectors ? D / 2 : 1];
+    const bool near = kVectors && prepare.vectors != 0;
+    float q_weights[kNear], k_weights[kNear];
+    if constexpr (kVectors) {
+        if (near) {
+            const size_t row = static_cast<size_t>(max(0, seq_len[seq] - 1)) * (D / 2);
+            for (int j = threadIdx.x; j < D / 2; j += kThreads) {
+                rotation[0][j] = prepare.rotary_dim ? prepare.cos_table[row + j] : 1.0f;
+                rotation[1][j] = prepare.rotary_dim ? prepare.sin_table[row + j] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kNear; ++i) {
+                q_weights[i] = prepare.q_weight ? prepare.q_weight[kNear * lane + i] : 1.0f;
+                k_weights[i] = prepare.k_weight ? prepare.k_weight[kNear * lane + i] : 1.0f;
+            }
+            __syncthreads();
+        }
+    }
     grid_dependency_wait();
     // The block's columns: query heads of the group, or, with `Runs`, pairs of a new token and a head, tokens first.  Column j belongs to row `place(j)` of queries and results.
     const int row0 = Runs ? cu_seqlens[seq] : seq, news = Runs ? cu_seqlens[seq + 1] - row0 : 1;
@@ -229,7 +252,52 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             const bf16* from = prepare.projected + static_cast<size_t>(seq) * prepare.stride;
             const float* cosines = prepare.cos_table + static_cast<size_t>(position) * (prepare.rotary_dim / 2);
             const float* sines = prepare.sin_table + static_cast<size_t>(position) * (prepare.rotary_dim / 2);
-            for (int task = warp; task < heads_here + (stores ? 2 : 0); task += kWarps) {
+            const int tasks = heads_here + (stores ? 2 : 0);
+            if constexpr (kVectors) {
+                if (near) {
+                    // All of the warp's rows are on their way together; the arithmetic is that of the 16-bit cache's prepare kernel for such heads.
+                    struct alignas(2 * kNear) Near { bf16 v[kNear]; };
+                    constexpr int kMost = (kHeads + 2 + kWarps - 1) / kWarps;
+                    Near raw[kMost];
+#pragma unroll
+                    for (int a = 0; a < kMost; ++a) {
+                        const int task = warp + kWarps * a;
+                        const int head = task == heads_here ? n_heads + kv_head : task == heads_here + 1 ? n_heads + n_kv_heads + kv_head : kv_head * group + task;
+                        if (task < tasks) raw[a] = *reinterpret_cast<const Near*>(from + static_cast<size_t>(head) * D + kNear * lane);
+                    }
+#pragma unroll
+                    for (int a = 0; a < kMost; ++a) {
+                        const int task = warp + kWarps * a;
+                        if (task >= tasks) break;
+                        const bool is_key = task == heads_here, is_value = task == heads_here + 1;
+                        Near* row = reinterpret_cast<Near*>(own[is_key ? kHeads : is_value ? kHeads + 1 : task]) + lane;
+                        if (is_value) {
+                            *row = raw[a];
+                            continue;
+                        }
+                        float value[kNear], squares = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < kNear; ++i) {
+                            value[i] = to_float(raw[a].v[i]);
+                            squares += value[i] * value[i];
+                        }
+                        if (is_key ? prepare.k_weight != nullptr : prepare.q_weight != nullptr) {
+                            const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + prepare.eps);
+#pragma unroll
+                            for (int i = 0; i < kNear; ++i) value[i] = round_through<bf16>(value[i] * inverse * (is_key ? k_weights[i] : q_weights[i]));
+                        }
+                        Near result;
+#pragma unroll
+                        for (int i = 0; i < kNear; ++i) {
+                            // First half of the head: x cos - partner sin; second half: x cos + partner sin.
+                            const float partner = __shfl_xor_sync(0xffffffffu, value[i], 16), turned = __fmul_rn(partner, rotation[1][kNear * (lane & 15) + i]);
+                            result.v[i] = from_float<bf16>(prepare.rotary_dim ? __fmaf_rn(value[i], rotation[0][kNear * (lane & 15) + i], lane < 16 ? -turned : turned) : value[i]);
+                        }
+                        *row = result;
+                    }
+                }
+            }
+            for (int task = near ? tasks : warp; task < tasks; task += kWarps) {
                 const bool is_key = task == heads_here, is_value = task == heads_here + 1;
                 const int head = is_key ? n_heads + kv_head : is_value ? n_heads + n_kv_heads + kv_head : kv_head * group + task;
                 bf16* row = own[is_key ? kHeads : is_value ? kHeads + 1 : task];
@@ -700,7 +768,8 @@ TAU_EXPORT int tau_decode8(const void* queries, void* key_pages, void* value_pag
     const Call call = {static_cast<const bf16*>(queries), static_cast<bf16*>(out), static_cast<uint8_t*>(key_pages), static_cast<uint8_t*>(value_pages), key_scales, value_scales, scratch,
                        scratch ? scratch + static_cast<size_t>(n_tokens) * n_heads * splits * D : nullptr, seq_len, cu_seqlens, page_rows, page_stride, n_seqs, n_tokens, n_heads, n_kv_heads,
                        static_cast<int>((columns + to_a_block - 1) / to_a_block), scale, window, splits,
-                       {static_cast<const bf16*>(projected), projected_stride, q_weight, k_weight, eps, cos_table, sin_table, rotary_dim, store}};
+                       {static_cast<const bf16*>(projected), projected_stride, q_weight, k_weight, eps, cos_table, sin_table, rotary_dim, store,
+                        projected && (D == 64 || D == 128 || D == 256) && (rotary_dim == 0 || rotary_dim == D) && (projected_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(projected) & 15) == 0}};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if constexpr (D <= 128)
         if (to_a_block == 16) return cu_seqlens ? launch<2, true>(key_map, value_map, call, s) : launch<2, false>(key_map, value_map, call, s);

@@ -85,8 +85,9 @@ __device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__
     const int half = rotary_dim / 2;
     for (int j = lane; j < half; j += 32) {      // a pair is one lane's
         const float first = to_float(row[j]), second = to_float(row[j + half]), c = cosines[j], s = sines[j];
-        row[j] = __float2bfloat16_rn(first * c - second * s);
-        row[j + half] = __float2bfloat16_rn(second * c + first * s);
+        // Which product is rounded before the sum is fixed, so that every kernel that prepares a row leaves the same bits.
+        row[j] = __float2bfloat16_rn(__fmaf_rn(first, c, -__fmul_rn(second, s)));
+        row[j + half] = __float2bfloat16_rn(__fmaf_rn(second, c, __fmul_rn(first, s)));
     }
     __syncwarp();
 }
