@@ -7,7 +7,7 @@
 // cp.async in whole lines.  Two forms: up to 8 bfloat16 rows, quantised here, a block to an SM; and up to 16 quantised rows, a block to 16 features.
 //
 // Needs K % 16 == 0 and contiguous codes on a 16-byte border.
-#include "eight_bit.cuh"
+#include "quantize_rows.cuh"
 
 namespace {
 
@@ -395,4 +395,14 @@ TAU_EXPORT int tau_gemm8_skinny(int out_dtype, const void* x, const float* x_sca
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (M <= 8) return launch_typed<1>(out_dtype, gated, x, x_scales, w, w_scales, bias, out, M, N, K, out_stride, gate_limit, s);
     return launch_typed<2>(out_dtype, gated, x, x_scales, w, w_scales, bias, out, M, N, K, out_stride, gate_limit, s);
+}
+
+// The same of bfloat16 or float32 rows `x_stride` elements apart on 16-byte borders, which are quantised into `held` first: M * K codes, then M floats for each 128 columns.
+TAU_EXPORT int tau_linear8_skinny(int x_dtype, const void* x, long long x_stride, void* held, int out_dtype, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K,
+                                  long long out_stride, int gated, float gate_limit, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!held || K <= 0 || M > 16) return cudaErrorInvalidValue;
+    float* scales = scales_behind(held, M, K);
+    const int code = launch_quantize_rows(x_dtype, x, x_stride, held, scales, M, K, static_cast<cudaStream_t>(stream));
+    return code ? code : tau_gemm8_skinny(out_dtype, held, scales, w, w_scales, bias, out, M, N, K, out_stride, gated, gate_limit, stream);
 }

@@ -14,7 +14,7 @@
 //
 // Needs K % 16 == 0, contiguous codes on 16-byte borders.
 #include "tcgen05.cuh"
-#include "eight_bit.cuh"
+#include "quantize_rows.cuh"
 
 namespace {
 
@@ -421,4 +421,14 @@ TAU_EXPORT int tau_gemm8_tc(int out_dtype, const void* x, const float* x_scales,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (features == 256) return launch_typed<256>(out_dtype, gated, call, s);
     return launch_typed<128>(out_dtype, gated, call, s);
+}
+
+// The same of bfloat16 or float32 rows `x_stride` elements apart on 16-byte borders, which are quantised into `held` first: M * K codes, then M floats for each 128 columns.
+TAU_EXPORT int tau_linear8_tc(int x_dtype, const void* x, long long x_stride, void* held, int out_dtype, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K,
+                              long long out_stride, int gated, float gate_limit, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (!held || K <= 0) return cudaErrorInvalidValue;
+    float* scales = scales_behind(held, M, K);
+    const int code = launch_quantize_rows(x_dtype, x, x_stride, held, scales, M, K, static_cast<cudaStream_t>(stream));
+    return code ? code : tau_gemm8_tc(out_dtype, held, scales, w, w_scales, bias, out, M, N, K, out_stride, gated, gate_limit, 0, 0, stream);
 }

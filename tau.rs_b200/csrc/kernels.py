@@ -1129,23 +1129,13 @@ SKINNY8_MAX_ROWS = 16       # of the other product for few rows, and where it be
 SKINNY8_SMALL_WEIGHT = 8 << 20   # 5.2; 16 x 4,096 x 24,576 30 against 27)
 
 
-def _skinny8(x: int, x_scales: int, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
-    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "ippppppiiilif")
-    features, depth = codes.shape
-    _check(run(_DTYPE_CODE[out.dtype], x, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, features, depth, out.stride(0),
-               1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
-
-
-def _tc8(x: int, x_scales: int, rows: int, codes, scales, bias, out, gated: bool, gate_limit: float, features: int, ranges: int) -> None:
-    run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
-    _check(run(_DTYPE_CODE[out.dtype], x, x_scales, codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], codes.shape[1], out.stride(0),
-               1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
-
-
 def gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
     """The product of at most 16 quantised rows, bound by streaming the weight's codes once."""
     _require(x_codes.shape[0] <= SKINNY8_MAX_ROWS, "too many rows for the skinny kernel")
-    _skinny8(x_codes.data_ptr(), x_scales.data_ptr(), x_codes.shape[0], codes, scales, bias, out, gated, gate_limit)
+    rows, depth = x_codes.shape
+    run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "ippppppiiilif")
+    _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
+               1 if gated else 0, gate_limit, _stream_handle()), "gemm8_skinny")
 
 
 def _stream8(values, codes, scales, bias, out, gated: bool, gate_limit: float) -> None:
@@ -1164,7 +1154,10 @@ def gemm8_stream(values, codes, scales, bias, out, gated: bool = False, gate_lim
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
     """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 256; 0: by the number of tiles) with K cut into `ranges`
     (1 to 8; 0: as many as leave no SM without work)."""
-    _tc8(x_codes.data_ptr(), x_scales.data_ptr(), x_codes.shape[0], codes, scales, bias, out, gated, gate_limit, features, ranges)
+    rows, depth = x_codes.shape
+    run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
+    _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
+               1 if gated else 0, gate_limit, features, ranges, _stream_handle()), "gemm8_tc")
 
 
 def gemm8_tc_status() -> int:
@@ -1188,13 +1181,10 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
         return _stream8(values, codes, scales, bias, out, gated, limit)
     # The activations' codes and, behind them, their scales, in one piece of memory.
     held = torch.empty(rows * (depth + 4 * -(-depth // SCALE_BLOCK)), dtype=torch.uint8, device=values.device)
-    x = held.data_ptr()
-    x_scales = x + rows * depth
-    run = _function("eight_bit.cu", "tau_quantize_rows", "iplppii")
-    _check(run(_DTYPE_CODE[values.dtype], values.data_ptr(), values.stride(0), x, x_scales, rows, depth, _stream_handle()), "quantize_rows")
-    if rows <= STREAM8_MAX_ROWS or (rows <= SKINNY8_MAX_ROWS and features * depth <= SKINNY8_SMALL_WEIGHT):
-        return _skinny8(x, x_scales, rows, codes, scales, bias, out, gated, limit)
-    _tc8(x, x_scales, rows, codes, scales, bias, out, gated, limit, 0, 0)
+    few = rows <= STREAM8_MAX_ROWS or (rows <= SKINNY8_MAX_ROWS and features * depth <= SKINNY8_SMALL_WEIGHT)
+    run = _function("gemm8_skinny.cu", "tau_linear8_skinny", "iplpippppiiilif") if few else _function("gemm8_tc.cu", "tau_linear8_tc", "iplpippppiiilif")
+    _check(run(_DTYPE_CODE[values.dtype], values.data_ptr(), values.stride(0), held.data_ptr(), _DTYPE_CODE[out.dtype], codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(),
+               rows, features, depth, out.stride(0), 1 if gated else 0, limit, _stream_handle()), "linear8", 2)
 
 
 def linear8(values, codes, scales, bias, out) -> None:
