@@ -37,6 +37,7 @@ constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kStages = kHalves == 1 ? 2 : 3;
 constexpr int kKeySteps = D / 16;                 // products of 16 head elements
 constexpr int kMostClustered = 8;
+constexpr int kMostOrdered = 1024;                // sequences that a block puts in order
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are kept times 2^14: what f16 holds with all its bits then reaches down to 2^-28 of the greatest, and a long tail of small weights keeps its sum.
 constexpr float kWeightBits = 14.0f;
@@ -100,6 +101,47 @@ __device__ __forceinline__ int key_element(int step, int t, int i) {
     return group < D / 64 ? group * 64 + t * 16 + (step & 3) * 4 + i : step * 16 + t * 4 + i;
 }
 
+// Sequence number `place` of `n` when longer ones come first: lengths are told apart by quarters of a power of two (of pages), within such a class the order is that of the
+// sequences.  Every thread of the block calls it.
+__device__ __forceinline__ int by_length(const int* __restrict__ seq_len, int n, int place) {
+    constexpr int kClasses = 64;
+    __shared__ unsigned char class_of[kMostOrdered];
+    __shared__ int members[kClasses];
+    __shared__ int chosen;
+    for (int i = threadIdx.x; i < kClasses; i += kThreads) members[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int pages = max(1, (seq_len[i] + kPage - 1) / kPage);
+        const int of = kClasses - 1 - min(kClasses - 1, (__float_as_int(static_cast<float>(pages)) >> 21) - (127 << 2));      // the two leading bits behind the first
+        class_of[i] = static_cast<unsigned char>(of);
+        atomicAdd(&members[of], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, mine = members[2 * lane] + members[2 * lane + 1];
+        int up_to = mine;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, up_to, offset);
+            if (lane >= offset) up_to += other;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, up_to > place)) - 1;      // place < n: some lane's
+        int left = place - __shfl_sync(0xffffffffu, up_to - mine, owner), of = 2 * owner;
+        if (left >= members[of]) left -= members[of++];
+        for (int first = 0; first < n; first += 32) {
+            const unsigned here = __ballot_sync(0xffffffffu, first + lane < n && class_of[min(first + lane, n - 1)] == of);
+            const int count = __popc(here);
+            if (left < count) {
+                if ((here >> lane & 1u) && __popc(here & ((1u << lane) - 1u)) == left) chosen = first + lane;
+                break;
+            }
+            left -= count;
+        }
+    }
+    __syncthreads();
+    return chosen;
+}
+
 constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a lane holds 16 columns, 8 tiles of 16 rows
 
 template <int NT, bool Runs>
@@ -107,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 && !Runs ? 4
 decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
                uint8_t* __restrict__ key_pages, uint8_t* __restrict__ value_pages, float* __restrict__ key_scales, float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                const int* __restrict__ seq_len, const int* __restrict__ cu_seqlens, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale,
-               int window, int splits, int clustered, Prepare prepare) {
+               int window, int splits, int clustered, int longest_first, Prepare prepare) {
     constexpr int kHeads = 8 * NT;
     extern __shared__ uint8_t shared_raw[];
     Shared* shared = reinterpret_cast<Shared*>(shared_raw);
@@ -121,10 +163,14 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     __shared__ float greatest_of[2 * kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, seq = blockIdx.z;
+    const int split = blockIdx.x;
     const int kv_head = blockIdx.y / passes, pass = blockIdx.y % passes;
     const int group = n_heads / n_kv_heads;
     volatile int* abort_flag = &shared->abort_flag;
+    int seq = blockIdx.z;
+    if constexpr (!Runs) {
+        if (longest_first) seq = by_length(seq_len, gridDim.z, seq);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             barrier_init(&shared->full[s], 2);      // the copies', and the scales'
@@ -718,15 +764,20 @@ int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call&
     }
     const dim3 grid(c.splits, c.n_kv_heads * c.passes, c.n_seqs);
     const bool clustered = c.splits > 1 && c.splits <= kMostClustered;
+    // Long sequences start first, so that the SMs share them out and short ones fill what is left at the end, up to three times as many blocks as there are places: 40 of 64 to 6,000
+    // positions 74 -> 59 us, 64 of up to 2,048 46 -> 36, 200 of up to 1,000 58 -> 52, 8 of 2,048 no slower; beyond that putting them in order costs a block more than it gives
+    // (256 of up to 300: 36 -> 38).
+    const long long places = 148ll * (NT == 1 && kHalves == 1 && !Runs ? 4 : 2), blocks = static_cast<long long>(grid.x) * grid.y * grid.z;
+    const int longest_first = !Runs && c.n_seqs > 1 && c.n_seqs <= kMostOrdered && blocks <= 3 * places;
     // Beside the kernel before it only where all blocks find room at once (8 sequences of 2,048 positions 14.4 -> 13.9 us; 640 blocks of 40 sequences 73 -> 78).
-    const bool early = static_cast<long long>(grid.x) * grid.y * grid.z <= 148ll * (NT == 1 && kHalves == 1 && !Runs ? 4 : 2);
+    const bool early = blocks <= places;
     int code;
     if (clustered)
         code = tau_launch_clusters_as(early, c.splits, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales,
-                                      c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1, c.prepare);
+                                      c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1, longest_first, c.prepare);
     else
         code = tau_launch_as(early, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales, c.partial_o,
-                             c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0, c.prepare);
+                             c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0, longest_first, c.prepare);
     if (code == 0 && c.splits > kMostClustered)
         code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? (D + 31) / 32 * 32 : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
     return code ? code : tau_launch_status();

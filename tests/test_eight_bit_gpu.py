@@ -404,6 +404,12 @@ def test_many_single_tokens_and_a_long_context():
     check_attention([(9000, 1)], 2, 1, 64, 0, seed=3)
 
 
+@pytest.mark.parametrize("sequences", [2, 31, 33, 100, 257, 1000, 1024, 1025])
+def test_sequences_of_unequal_lengths(sequences):
+    """The longest may start first: every sequence is still worked on once, whatever their lengths, in every class of lengths."""
+    check_attention([((37 * index * index + 64 * index) % (700 if sequences > 100 else 3000), 1) for index in range(sequences)], 2, 1, 32, 0)
+
+
 @pytest.mark.parametrize("n_heads, n_kv_heads, dim, rotary, normed, window", [(4, 2, 32, 32, True, 0), (8, 8, 128, 128, True, 70), (32, 4, 64, 64, True, 0), (6, 2, 80, 40, True, 1), (16, 1, 128, 0, False, 0),
                                                                                (8, 1, 256, 256, True, 100), (3, 3, 16, 8, False, 0)])
 @pytest.mark.parametrize("splits", [0, 1, 3, 8, 20])
