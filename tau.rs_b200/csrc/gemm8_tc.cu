@@ -4,7 +4,7 @@
 //
 // The scales change every 128 columns of K, so the accumulator in tensor memory holds one such block at a time (four tcgen05.mma of kind f8f6f4, 32 columns each)
 // and the sums over blocks are kept in registers: four warps for each 64 features read a block's sums with tcgen05.ld and add them times both scales, while
-// the next blocks' products fill the other accumulators (two of 256 features, four of 128).  Rows (tokens) are the lanes of tensor memory and features its columns, so a thread's factor
+// the next blocks' products fill the other accumulators (two of 256 or 192 features, four of 128).  Rows (tokens) are the lanes of tensor memory and features its columns, so a thread's factor
 // is one number for each 128 features: 64 multiply-adds a thread and block, 256 on each quarter of an SM, against the 512 clocks that the products of a 128 x 256 block take.
 //
 // Operands come by TMA (128-byte swizzle, no multicast): a stage is 128 bytes of K of 128 rows of x and BN of w.  One warp asks for tiles, one issues products,
@@ -48,7 +48,7 @@ __device__ __forceinline__ void mma_issue_e4m3(uint32_t sums, uint64_t a, uint64
 }
 
 constexpr int stage_bytes(int bn) { return (BM + bn) * BK; }
-constexpr int stages_of(int bn) { return bn == 256 ? 4 : 6; }
+constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 192 ? 5 : 6; }
 constexpr int shared_bytes(int bn) { return static_cast<int>(sizeof(Shared)) + 1024 + stages_of(bn) * stage_bytes(bn); }
 
 // Adds a block's sums of this warp's 32 tokens and 64 features, times the token's factor; `Step` columns of tensor memory at a time: 32, or 16 where 18 warps leave a thread 100
@@ -266,7 +266,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
                 auto release = [&]() {
                     if (lane == 0) barrier_arrive(&shared->sums_empty[slot]);
                 };
-                if (token - lane < M) add_block<(BN > 128 ? 16 : 32)>(address, factor, sums, release);      // some of these 32 tokens are there
+                if (token - lane < M) add_block<(BN > 192 ? 16 : 32)>(address, factor, sums, release);      // some of these 32 tokens are there
                 else release();
             }
             if (!alive) break;
@@ -395,31 +395,44 @@ TAU_EXPORT int tau_gemm8_tc_status() {
     return flag;
 }
 
-// x codes [M, K] with scales [blocks][M]; w codes [N, K] with scales [blocks of N][blocks].  `features`: 128 or 256 to a tile of 128 tokens; `ranges`: 1 to 8 ranges of K to a
+// x codes [M, K] with scales [blocks][M]; w codes [N, K] with scales [blocks of N][blocks].  `features`: 128, 192 or 256 to a tile of 128 tokens; `ranges`: 1 to 8 ranges of K to a
 // tile.  0: chosen.
 TAU_EXPORT int tau_gemm8_tc(int out_dtype, const void* x, const float* x_scales, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K, long long out_stride,
                             int gated, float gate_limit, int features, int ranges, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (!x || !x_scales || !w || !w_scales || !out || K <= 0 || (K & 15) || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
-        (out_dtype != TAU_BF16 && out_dtype != TAU_F32) || (gated && ((N & 15) || out_dtype != TAU_BF16)) || (features != 0 && features != 128 && features != 256) ||
+        (out_dtype != TAU_BF16 && out_dtype != TAU_F32) || (gated && ((N & 15) || out_dtype != TAU_BF16)) || (features != 0 && features != 128 && features != 192 && features != 256) ||
         ranges < 0 || ranges > kMostRanges)
         return cudaErrorInvalidValue;
     int device = 0, sms = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return cudaErrorInvalidValue;
     const int k_blocks = (K + BK - 1) / BK, token_tiles = (M + BM - 1) / BM;
-    auto tiles = [&](int bn) { return static_cast<long long>((N + bn - 1) / bn) * token_tiles; };
-    // Wide tiles where they give three of five SMs work (64 x 4,096 x 24,576: 96 wide tiles 23 us, 192 narrow ones 29) or where narrow ones would take a second round (512 x 4,096 x
-    // 6,144: 22 and 30).  Else narrow ones, K cut into ranges of four blocks and more as long as their clusters fit the machine at once, whose groups of SMs hold about 72 clusters of two,
-    // 32 of four and 12 of eight (64 x 12,288 x 4,096: 32 tiles in four ranges 16 us, in two 23, in one 38; 333 x 2,000 x 1,500: 36 tiles in two ranges 10 us, in four 16).
-    if (features == 0) features = tiles(256) * 5 >= sms * 3 || tiles(128) > sms ? 256 : 128;
-    if (ranges == 0) {
-        const long long n = tiles(features);
-        ranges = n <= 12 && k_blocks >= 32 ? 8 : n <= 32 && k_blocks >= 16 ? 4 : n <= 72 && k_blocks >= 8 ? 2 : 1;
+    // What is not given is chosen by what a round of tiles costs: a block of K takes a tile about as long as 192 features and its own (some 1.1 ns a feature; 4,096 columns: 15 us at
+    // 128 features, 18 at 192, 21 at 256), and the join of two, four or eight ranges as long as 1,500, 3,500 and 6,000 such steps of a feature.  Clusters have to fit the machine at
+    // once, whose groups of SMs hold about 72 of two, 32 of four and 12 of eight.  (us at 128, 192 and 256 features: 16 x 4,096 x 24,576 31, 23 and 28; 512 x 4,096 x 6,144
+    // 30, 19 and 22; 2,048 x 4,096 x 6,144 85, 68 and 61; 64 x 12,288 x 4,096 in one, two and four ranges 38, 23 and 16; 64 x 1,024 x 6,144 in one and two 5.7 and 7.0.)
+    long long least = 0;
+    int best_features = 0, best_ranges = 0;
+    for (int bn = 256; bn >= 128; bn -= 64) {
+        if (features != 0 && features != bn) continue;
+        const long long n = static_cast<long long>((N + bn - 1) / bn) * token_tiles;
+        for (int r = 1; r <= kMostRanges; r *= 2) {
+            if (ranges != 0 ? r > 1 : r > 1 && (n > (r == 2 ? 72 : r == 4 ? 32 : 12) || k_blocks < 4 * r)) break;
+            const long long cost = (n + sms - 1) / sms * ((k_blocks + r - 1) / r) * (bn + 192) + (r == 1 ? 0 : r == 2 ? 1500 : r == 4 ? 3500 : 6000);
+            if (best_features == 0 || cost < least) {
+                least = cost;
+                best_features = bn;
+                best_ranges = r;
+            }
+        }
     }
+    features = best_features;
+    if (ranges == 0) ranges = best_ranges;
     if (ranges > k_blocks) ranges = k_blocks;
     const Call call = {x, x_scales, w, w_scales, bias, out, M, N, K, out_stride, ranges, sms, gate_limit};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (features == 256) return launch_typed<256>(out_dtype, gated, call, s);
+    if (features == 192) return launch_typed<192>(out_dtype, gated, call, s);
     return launch_typed<128>(out_dtype, gated, call, s);
 }
 

@@ -1125,8 +1125,9 @@ def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
 
 STREAM8_MAX_ROWS = 8        # rows of the streaming product, which quantises them itself ...
 STREAM8_MAX_DEPTH = 12288   # ... and keeps their codes in shared memory
-SKINNY8_MAX_ROWS = 16       # of the other product for few rows, and where it beats the tensor-core product if the weight has at most so many elements (16 x 1,024 x 4,096 2.5 us against
-SKINNY8_SMALL_WEIGHT = 8 << 20   # 5.2; 16 x 4,096 x 24,576 30 against 27)
+SKINNY8_MAX_ROWS = 16       # of the other product for few rows, and the weights with which it beats the tensor-core product: its blocks of 16 features fit the machine about
+SKINNY8_MOST_FEATURES = 8192     # once, and K is not so deep that several blocks should share it (16 rows, K x features, us against the tensor-core product's: 1,024 x 4,096 2.7 and
+SKINNY8_MOST_DEPTH = 6144        # 5.5; 6,144 x 4,096 8.4 and 11.6; 2,048 x 8,192 7.4 and 9.4; 1,024 x 16,384 8.9 and 7.6; 12,288 x 2,048 13.7 and 10.5)
 
 
 def gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
@@ -1152,8 +1153,8 @@ def gemm8_stream(values, codes, scales, bias, out, gated: bool = False, gate_lim
 
 
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
-    """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 256; 0: by the number of tiles) with K cut into `ranges`
-    (1 to 8; 0: as many as leave no SM without work)."""
+    """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 192, 256) with K cut into `ranges` (1 to 8);
+    0: by what the tiles' rounds cost."""
     rows, depth = x_codes.shape
     run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
     _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
@@ -1181,7 +1182,7 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
         return _stream8(values, codes, scales, bias, out, gated, limit)
     # The activations' codes and, behind them, their scales, in one piece of memory.
     held = torch.empty(rows * (depth + 4 * -(-depth // SCALE_BLOCK)), dtype=torch.uint8, device=values.device)
-    few = rows <= STREAM8_MAX_ROWS or (rows <= SKINNY8_MAX_ROWS and features * depth <= SKINNY8_SMALL_WEIGHT)
+    few = rows <= STREAM8_MAX_ROWS or (rows <= SKINNY8_MAX_ROWS and features <= SKINNY8_MOST_FEATURES and depth <= SKINNY8_MOST_DEPTH)
     run = _function("gemm8_skinny.cu", "tau_linear8_skinny", "iplpippppiiilif") if few else _function("gemm8_tc.cu", "tau_linear8_tc", "iplpippppiiilif")
     _check(run(_DTYPE_CODE[values.dtype], values.data_ptr(), values.stride(0), held.data_ptr(), _DTYPE_CODE[out.dtype], codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(),
                rows, features, depth, out.stride(0), 1 if gated else 0, limit, _stream_handle()), "linear8", 2)

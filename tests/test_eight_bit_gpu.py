@@ -90,7 +90,7 @@ def test_gated_products(rows, depth, inner, limit):
 
 
 @pytest.mark.parametrize("rows, depth, features", [(1, 16, 16), (100, 1040, 530), (300, 400, 272), (513, 1296, 800)])
-@pytest.mark.parametrize("tile, ranges", [(128, 1), (128, 2), (128, 3), (128, 7), (128, 8), (256, 1), (256, 2), (256, 5)])
+@pytest.mark.parametrize("tile, ranges", [(128, 1), (128, 2), (128, 3), (128, 7), (128, 8), (192, 1), (192, 3), (192, 8), (256, 1), (256, 2), (256, 5)])
 def test_every_tile_of_the_tensor_core_product(rows, depth, features, tile, ranges):
     """Each width of tile, ranges of K (more than there are blocks of K too), ungated in both types and gated, into rows of a wider tensor."""
     x, w = spread_values(rows, depth, seed=depth, outliers=False).to(torch.bfloat16), (spread_values(features, depth, seed=features, outliers=False) * depth ** -0.5).to(torch.bfloat16)

@@ -17,7 +17,7 @@ def lost_rank(monkeypatch):
     monkeypatch.setattr(kernels, "_decode8_functions", {})
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, 192, 256])
 def test_products_whose_ranges_meet_in_a_cluster(lost_rank, tile):
     """Four ranges of K, one of which gives up: no block of the cluster stores a sum that lacks it."""
     codes, w_codes = torch.zeros(64, 2048, device="cuda").to(eight.CODES), torch.zeros(256, 2048, device="cuda").to(eight.CODES)
