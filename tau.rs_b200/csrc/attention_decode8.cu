@@ -302,7 +302,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
             if constexpr (kVectors) {
                 if (near) {
                     // All of the warp's rows are on their way together; the arithmetic is that of the 16-bit cache's prepare kernel for such heads.
-                    struct alignas(2 * kNear) Near { bf16 v[kNear]; };
+                    typedef Neighbours<kNear> Near;
                     constexpr int kMost = (kHeads + 2 + kWarps - 1) / kWarps;
                     Near raw[kMost];
 #pragma unroll
@@ -321,25 +321,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                             *row = raw[a];
                             continue;
                         }
-                        float value[kNear], squares = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < kNear; ++i) {
-                            value[i] = to_float(raw[a].v[i]);
-                            squares += value[i] * value[i];
-                        }
-                        if (is_key ? prepare.k_weight != nullptr : prepare.q_weight != nullptr) {
-                            const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(D) + prepare.eps);
-#pragma unroll
-                            for (int i = 0; i < kNear; ++i) value[i] = round_through<bf16>(value[i] * inverse * (is_key ? k_weights[i] : q_weights[i]));
-                        }
-                        Near result;
-#pragma unroll
-                        for (int i = 0; i < kNear; ++i) {
-                            // First half of the head: x cos - partner sin; second half: x cos + partner sin.
-                            const float partner = __shfl_xor_sync(0xffffffffu, value[i], 16), turned = __fmul_rn(partner, rotation[1][kNear * (lane & 15) + i]);
-                            result.v[i] = from_float<bf16>(prepare.rotary_dim ? __fmaf_rn(value[i], rotation[0][kNear * (lane & 15) + i], lane < 16 ? -turned : turned) : value[i]);
-                        }
-                        *row = result;
+                        *row = prepare_neighbours<kNear>(raw[a], is_key ? prepare.k_weight != nullptr : prepare.q_weight != nullptr, is_key ? k_weights : q_weights, prepare.eps,
+                                                         prepare.rotary_dim != 0, &rotation[0][kNear * (lane & 15)], &rotation[1][kNear * (lane & 15)], lane);
                     }
                 }
             }

@@ -92,6 +92,36 @@ __device__ __forceinline__ void prepare_row(bf16* row, const float* __restrict__
     __syncwarp();
 }
 
+// The same of a head of 32 PER elements that is rotated whole (`rotated`) or not at all, in registers: a lane holds PER neighbours, `weight` theirs, `cosines` and `sines` those of
+// elements PER (lane % 16) + i of the half-wide tables.
+template <int PER>
+struct alignas(2 * PER) Neighbours {
+    bf16 v[PER];
+};
+template <int PER>
+__device__ __forceinline__ Neighbours<PER> prepare_neighbours(const Neighbours<PER>& raw, bool normed, const float* weight, float eps, bool rotated, const float* cosines, const float* sines,
+                                                              int lane) {
+    float value[PER], squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        value[i] = to_float(raw.v[i]);
+        squares += value[i] * value[i];
+    }
+    if (normed) {
+        const float inverse = rsqrtf(warp_sum(squares) / static_cast<float>(32 * PER) + eps);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) value[i] = round_through<bf16>(value[i] * inverse * weight[i]);
+    }
+    Neighbours<PER> result;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        // First half of the head: x cos - partner sin; second half: x cos + partner sin.
+        const float partner = __shfl_xor_sync(0xffffffffu, value[i], 16), turned = __fmul_rn(partner, sines[i]);
+        result.v[i] = from_float<bf16>(rotated ? __fmaf_rn(value[i], cosines[i], lane < 16 ? -turned : turned) : value[i]);
+    }
+    return result;
+}
+
 // `threads` threads of a block (numbers 0 .. threads - 1, all of its threads if `whole_block`, else its first four warps) bring `count` rows of D elements in shared memory into a page of one head, behind the `older`
 // positions that it holds: the scale is the page's own (none for a page that starts here) or what the new rows need, whichever is greater, and codes that are there are rounded to
 // one that grew.  Returns the page's scale, which one thread then writes to `scale_at`; every thread has read the old one by then.  `greatest_of`: a float for each warp.
