@@ -8,6 +8,7 @@ cover instead of computing something else.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import replace
 from typing import Optional
 
 import torch
@@ -1215,6 +1216,8 @@ def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_r
     sequences = step.n_seqs
     if page_rows.dtype is not torch.int32 or page_rows.dim() != 2 or page_rows.shape[0] != sequences or not page_rows.is_contiguous():
         raise KernelError("page rows must be int32 [sequences, stride]")
+    if step.max_len > page_rows.shape[1] * PAGE_TOKENS:
+        raise KernelError("page rows must hold the pages of the step's longest sequence")
     for tensor, count in ((step.cu_seqlens, sequences + 1), (step.seq_start, sequences), (step.seq_len, sequences)):
         if tensor.dtype is not torch.int32 or tensor.numel() != count or tensor.stride(0) != 1:
             raise KernelError("a step's cu_seqlens, seq_start and seq_len must be int32, one (and one more bound) to a sequence")
@@ -1235,7 +1238,7 @@ def cache8_store(keys, values, key_pages, value_pages, key_scales, value_scales,
     eps, rotary_dim, n_heads = 0.0, 0, 0
     if prepare is not None:
         projected, queries, q_weight, k_weight, eps, cos, sin, rotary_dim, n_heads = prepare
-        _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim)
+        _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim, step.max_len)
         _require(projected.dtype == torch.bfloat16 and projected.dim() == 2 and projected.shape[0] == step.n_tokens and projected.shape[1] >= n_heads * head_dim and projected.stride(1) == 1,
                  "projected rows must hold every query head in bfloat16")
         _require(queries.dtype == torch.bfloat16 and queries.shape == (step.n_tokens, n_heads * head_dim) and queries.is_contiguous(), "queries must be [tokens, n_heads * head_dim]")
@@ -1336,7 +1339,7 @@ def attention8_decode_fused(projected, key_pages, value_pages, key_scales, value
         raise KernelError(f"projected rows must hold {needed} bfloat16 elements")
     if out.dtype is not torch.bfloat16 or out.shape != (step.n_tokens, n_heads * head_dim) or not out.is_contiguous() or window < 0:
         raise KernelError("the output must be bfloat16 [tokens, n_heads * head_dim], and a window not negative")
-    _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim)
+    _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim, step.max_len)
     _here(projected, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_len, q_weight, k_weight, cos, sin)
     if step.n_tokens:
         attention_decode8(None, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window,
@@ -1344,12 +1347,12 @@ def attention8_decode_fused(projected, key_pages, value_pages, key_scales, value
     return True
 
 
-def _check_rotation(q_weight, k_weight, cos, sin, rotary_dim: int, head_dim: int) -> None:
+def _check_rotation(q_weight, k_weight, cos, sin, rotary_dim: int, head_dim: int, positions: int) -> None:
     _f32_vector(q_weight, head_dim, "the q norm weight")
     _f32_vector(k_weight, head_dim, "the k norm weight")
     if rotary_dim and (rotary_dim % 2 or not 0 < rotary_dim <= head_dim or cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
-                       or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise KernelError("rotation tables must be float32 [positions, rotary_dim / 2]")
+                       or cos.shape != sin.shape or cos.shape[0] < positions or cos.shape[1] != rotary_dim // 2 or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise KernelError("rotation tables must be float32 [positions, rotary_dim / 2], as many positions as the longest sequence has")
 
 
 RUNS8_COLUMNS = 64          # of new tokens times a group's query heads, up to which runs are worked on like single tokens, 16 columns to a reading of the pages (us against pages laid
@@ -1370,6 +1373,9 @@ _decode8_functions = {}
 DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 
 
+READ8_BYTES = 1 << 30      # of pages read back at once
+
+
 def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
     """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
     _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
@@ -1386,8 +1392,14 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     if _prefer_optimized and (step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim))):
         return attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
-    keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, window, True)
-    attention(queries, keys, values, out, step, places, n_heads, n_kv_heads, head_dim, scale, window)
+    # Every sequence has room for the longest, so they are taken a few at a time where that would be much (the plain kernel goes by the step's own numbers and takes all at once).
+    sequences, stride = page_rows.shape
+    at_once = sequences if not _prefer_optimized else max(1, READ8_BYTES // (4 * stride * PAGE_TOKENS * n_kv_heads * head_dim))
+    for first in range(0, sequences, at_once):
+        last = min(first + at_once, sequences)
+        part = step if at_once >= sequences else replace(step, n_seqs=last - first, cu_seqlens=step.cu_seqlens[first : last + 1], seq_start=step.seq_start[first:last], seq_len=step.seq_len[first:last])
+        keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, part, page_rows[first:last], window, True)
+        attention(queries, keys, values, out, part, places, n_heads, n_kv_heads, head_dim, scale, window)
 
 
 # ---------------------------------------------------------------------------- latent attention

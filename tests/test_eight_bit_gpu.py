@@ -378,6 +378,15 @@ def test_runs_by_either_kernel(monkeypatch, directly, heads, kv_heads, dim, wind
     check_attention([(3000, 5), (0, 2)], heads, kv_heads, dim, window, seed=4)
 
 
+@pytest.mark.parametrize("heads, kv_heads, dim, window", [(4, 2, 48, 0), (8, 2, 64, 90), (4, 1, 128, 0)])
+def test_runs_whose_pages_are_read_back_a_few_sequences_at_a_time(monkeypatch, heads, kv_heads, dim, window):
+    """Room for two sequences at a time, then for less than one: the result of each is that of all at once."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: False)
+    for room in (2, 0):
+        monkeypatch.setattr(kernels, "READ8_BYTES", room * 4 * 4 * 64 * kv_heads * dim)      # the longest has four pages
+        check_attention([(0, 70), (100, 1), (60, 9), (0, 1), (130, 66)], heads, kv_heads, dim, window)
+
+
 @pytest.mark.parametrize("directly", [0, 1])
 @pytest.mark.parametrize("kv_heads, dim", [(2, 32), (1, 64), (2, 128), (1, 256)])
 def test_what_later_tokens_hold_reaches_no_earlier_one(monkeypatch, directly, kv_heads, dim):

@@ -104,6 +104,19 @@ def test_attention_refuses(change):
                            operands["page_rows"], operands["heads"], operands["kv_heads"], operands["head_dim"], 1.0, operands["window"])
 
 
+def test_page_rows_hold_the_longest_sequence():
+    operands = cache_operands()
+    operands["step"].max_len = 129      # two pages are listed
+    with pytest.raises(kernels.KernelError, match="longest sequence"):
+        kernels.cache8_store(**operands)
+
+
+def test_rotation_tables_hold_the_longest_sequence():
+    operands, tables = cache_operands(), [torch.zeros(5, 16) for _ in range(2)]      # six positions are there
+    with pytest.raises(kernels.KernelError, match="rotation tables"):
+        kernels.cache8_store(**operands, prepare=(torch.zeros(5, 128, dtype=torch.bfloat16), torch.zeros(5, 128, dtype=torch.bfloat16), None, None, 1e-6, *tables, 32, 4))
+
+
 # ---- configuration, cache and budget: host logic ---------------------------------------------------------------------------------
 def tiny_spec(which="B"):
     import tiny_configs
