@@ -26,15 +26,16 @@ namespace {
 constexpr int D = TAU_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head_dim must be a multiple of 16 between 16 and 256");
 constexpr int kPage = 64;
-constexpr int kWarps = 4;                         // consumers; one more asks for pages
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kGroupWarps = 4;                    // consumers of a page; one more warp asks for pages
 constexpr int kHalves = (D + 127) / 128;          // boxes of 128 bytes to a row
 constexpr int kBoxBytes = kPage * 128;
 constexpr int kTileBytes = kHalves * kBoxBytes;   // a page of a head's keys, or of its values
 constexpr int kStageBytes = 2 * kTileBytes;
 // Two pages ahead and four blocks to an SM where a page is 16 KB; three of 32 KB and two blocks for wider heads (64 sequences of 2,048 positions, 32 heads of 128 over 8: 54 us so,
 // 60 with four pages and three blocks, 61 with six and two).
-constexpr int kStages = kHalves == 1 ? 2 : 3;
+template <int Groups>
+constexpr int kStagesOf = kHalves == 1 ? 2 * Groups : 3;
+constexpr int kMostStages = kHalves == 1 ? 4 : 3;
 constexpr int kKeySteps = D / 16;                 // products of 16 head elements
 constexpr int kMostClustered = 8;
 constexpr int kMostOrdered = 1024;                // sequences that a block puts in order
@@ -44,10 +45,10 @@ constexpr float kWeightBits = 14.0f;
 constexpr float kLeastShare = 0.00390625f;      // 2^-8: a page whose value scale is smaller than this share of the accumulators' is added in 32 bits
 
 struct Shared {
-    uint64_t full[kStages];
-    uint64_t empty[kStages];
-    float key_scale[kStages], share[kStages], older[kStages];
-    float unit;
+    uint64_t full[kMostStages];
+    uint64_t empty[kMostStages];
+    float key_scale[kMostStages], share[kMostStages], older[kMostStages];
+    float unit[2];
     uint64_t stored;                              // the newest position is in its page
     float new_key_scale, new_value_scale;         // that page's scales
     int abort_flag;
@@ -104,13 +105,14 @@ __device__ __forceinline__ int key_element(int step, int t, int i) {
 // Sequence number `place` of `n` when longer ones come first: lengths are told apart by quarters of a power of two (of pages), within such a class the order is that of the
 // sequences.  Every thread of the block calls it.
 __device__ __forceinline__ int by_length(const int* __restrict__ seq_len, int n, int place) {
+    const int threads = blockDim.x;
     constexpr int kClasses = 64;
     __shared__ unsigned char class_of[kMostOrdered];
     __shared__ int members[kClasses];
     __shared__ int chosen;
-    for (int i = threadIdx.x; i < kClasses; i += kThreads) members[i] = 0;
+    for (int i = threadIdx.x; i < kClasses; i += threads) members[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += threads) {
         const int pages = max(1, (seq_len[i] + kPage - 1) / kPage);
         const int of = kClasses - 1 - min(kClasses - 1, (__float_as_int(static_cast<float>(pages)) >> 21) - (127 << 2));      // the two leading bits behind the first
         class_of[i] = static_cast<unsigned char>(of);
@@ -144,13 +146,15 @@ __device__ __forceinline__ int by_length(const int* __restrict__ seq_len, int n,
 
 constexpr int kValueRounds = (D + 127) / 128;      // rounds of 128 columns: a lane holds 16 columns, 8 tiles of 16 rows
 
-template <int NT, bool Runs>
-__global__ void __launch_bounds__(kThreads, NT == 1 && kHalves == 1 && !Runs ? 4 : 2)
+// Groups of four warps share the pages of a block's range out, every other page to each of two, and a block's warps are joined in shared memory; accumulators stand in a unit of their own.
+template <int NT, bool Runs, int Groups>
+__global__ void __launch_bounds__((4 * Groups + 1) * 32, NT == 1 && kHalves == 1 && !Runs && Groups == 1 ? 4 : 2)
 decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const bf16* __restrict__ queries, bf16* __restrict__ out,
                uint8_t* __restrict__ key_pages, uint8_t* __restrict__ value_pages, float* __restrict__ key_scales, float* __restrict__ value_scales, float* __restrict__ partial_o, float* __restrict__ partial_ml,
                const int* __restrict__ seq_len, const int* __restrict__ cu_seqlens, const int* __restrict__ page_rows, int page_stride, int n_heads, int n_kv_heads, int passes, float scale,
                int window, int splits, int clustered, int longest_first, Prepare prepare) {
-    constexpr int kHeads = 8 * NT;
+    constexpr int kHeads = 8 * NT, kWarps = kGroupWarps * Groups, kThreads = (kWarps + 1) * 32, kStages = kStagesOf<Groups>;
+    static_assert(Groups == 1 || kHalves == 1, "a group has two stages of its own");
     extern __shared__ uint8_t shared_raw[];
     Shared* shared = reinterpret_cast<Shared*>(shared_raw);
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared_raw) + sizeof(Shared) + 1023) & ~uintptr_t(1023));
@@ -174,7 +178,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             barrier_init(&shared->full[s], 2);      // the copies', and the scales'
-            barrier_init(&shared->empty[s], kWarps);
+            barrier_init(&shared->empty[s], kGroupWarps);
         }
         barrier_init(&shared->stored, kWarps);
         shared->abort_flag = 0;
@@ -222,7 +226,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     // The range with the newest position: nobody else reads that page of that head.
     const bool stores = !Runs && prepare.projected != nullptr && prepare.store && count > 0 && page_hi == pages_end;
     float running_max[NT][2], running_sum[NT][2];      // log2 units; the sums and accumulators belong to weights exp2(score - max + 14)
-    float unit = 0.0f;      // producer: what one in the accumulators stands for, the greatest value scale of the pages so far
+    float unit[2] = {0.0f, 0.0f};      // producer: what one in a group's accumulators stands for, the greatest value scale of its pages so far
     float acc[NT][kValueRounds][8][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -276,19 +280,24 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                         v_of = shared->new_value_scale;
                     }
                     // A page's value scale joins the weights as its share of the accumulators' unit (powers of two: exact), so a unit that grows rescales them.
-                    const float grown = fmaxf(unit, v_of);
+                    const bool other = Groups == 2 && (n & 1);
+                    const float before = other ? unit[1] : unit[0], grown = fmaxf(before, v_of);
                     if (lane == 0) {
                         shared->key_scale[n % kStages] = k_of;
                         shared->share[n % kStages] = v_of / grown;
-                        shared->older[n % kStages] = unit / grown;
+                        shared->older[n % kStages] = before / grown;
                         barrier_arrive(&shared->full[n % kStages]);
                     }
-                    unit = grown;
+                    if (other) unit[1] = grown;
+                    else unit[0] = grown;
                 }
                 __syncwarp();
             }
         }
-        if (lane == 0) shared->unit = unit;
+        if (lane == 0) {
+            shared->unit[0] = unit[0];
+            shared->unit[1] = unit[1];
+        }
         if (!alive && lane == 0)      // giving up: the copies in flight own their stages until they have landed
             for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
     } else {
@@ -334,12 +343,12 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 __syncwarp();
                 prepare_row(row, is_value ? nullptr : is_key ? prepare.k_weight : prepare.q_weight, prepare.eps, cosines, sines, is_value ? 0 : prepare.rotary_dim, D, lane);
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");      // every consumer warp comes here before any of its waits
+            asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");      // every consumer warp comes here before any of its waits
             if (stores) {
                 const size_t place_of = static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + position / kPage]) * n_kv_heads + kv_head;
                 const int older = position % kPage;
-                const float k_of = store_in_page<false>(own[Runs ? 0 : kHeads], 1, D, older, key_pages + place_of * kPage * D, key_scales + place_of, greatest_of, kWarps * 32);
-                const float v_of = store_in_page<false>(own[Runs ? 0 : kHeads + 1], 1, D, older, value_pages + place_of * kPage * D, value_scales + place_of, greatest_of + kWarps, kWarps * 32);
+                const float k_of = store_in_page<kWarps * 32>(own[Runs ? 0 : kHeads], 1, D, older, key_pages + place_of * kPage * D, key_scales + place_of, greatest_of);
+                const float v_of = store_in_page<kWarps * 32>(own[Runs ? 0 : kHeads + 1], 1, D, older, value_pages + place_of * kPage * D, value_scales + place_of, greatest_of + kWarps);
                 if (threadIdx.x == 0) {
                     key_scales[place_of] = shared->new_key_scale = k_of;
                     value_scales[place_of] = shared->new_value_scale = v_of;
@@ -396,12 +405,13 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 column_end[n][h] = Runs ? start + (column0 + n * 8 + 2 * t + h) / group + 1 : length;
                 column_first[n][h] = Runs && window > 0 ? max(0, column_end[n][h] - window) : first;
             }
+        const int page_part = (warp & (kGroupWarps - 1)) * 16;      // this warp's positions of a page
         bool alive = true;
-        for (int number = 0; number < count; ++number) {
+        for (int number = Groups == 1 ? 0 : warp / kGroupWarps; number < count; number += Groups) {
             const int stage = number % kStages;
             alive = __all_sync(0xffffffffu, barrier_wait(&shared->full[stage], (number / kStages) & 1, abort_flag));
             if (!alive) break;
-            const int base = (page_lo + number) * kPage + warp * 16;      // position of this warp's first key
+            const int base = (page_lo + number) * kPage + page_part;      // position of this warp's first key
             if (base < length && base + 16 > first) {
                 const uint8_t* key_tile = stages + stage * kStageBytes;
                 const uint8_t* value_tile = key_tile + kTileBytes;
@@ -413,7 +423,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) score[n][j] = score_odd[n][j] = 0.0f;
-                const int row_lo = warp * 16 + g, row_hi = row_lo + 8;
+                const int row_lo = page_part + g, row_hi = row_lo + 8;
                 constexpr int kGroups = D / 64;
 #pragma unroll
                 for (int c = 0; c < kGroups; ++c) {
@@ -461,7 +471,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
 #pragma unroll
                             for (int r = 0; r < kValueRounds; ++r) {
                                 if ((8 * r + g) * 16 >= D) continue;
-                                const uint4 v = page_chunk(value_tile, warp * 16 + slots[s], 8 * r + g);
+                                const uint4 v = page_chunk(value_tile, page_part + slots[s], 8 * r + g);
                                 odd |= __vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu) | __vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu) |
                                        __vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
                             }
@@ -523,7 +533,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                     const int slots[4] = {2 * t, 2 * t + 1, 2 * t + 8, 2 * t + 9};
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        v[s] = chunk * 16 < D ? page_chunk(value_tile, warp * 16 + slots[s], chunk) : make_uint4(0u, 0u, 0u, 0u);
+                        v[s] = chunk * 16 < D ? page_chunk(value_tile, page_part + slots[s], chunk) : make_uint4(0u, 0u, 0u, 0u);
                         // What nobody sees may be NaN, and a weight of zero would not hide that.
                         if ((!whole && (base + slots[s] < first || base + slots[s] >= length)) || (Runs && (odd_keys >> slots[s] & 1u))) v[s] = make_uint4(0u, 0u, 0u, 0u);
                     }
@@ -586,7 +596,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     __syncthreads();      // the stages are done with
     grid_dependents_launch();      // only now: what starts beside this kernel takes room that its own later blocks, or clusters, wait for
     if (warp < kWarps) {
-        const float one = shared->unit;
+        const float one = shared->unit[Groups == 1 ? 0 : warp / kGroupWarps];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -720,7 +730,8 @@ int page_map(CUtensorMap* map, const void* pages, long long boxes) {
     return result == CUDA_SUCCESS ? 0 : cudaErrorInvalidValue;
 }
 
-constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + kStages * kStageBytes; }
+template <int Groups>
+constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + kStagesOf<Groups> * kStageBytes; }
 
 struct Call {
     const bf16* queries;
@@ -734,14 +745,14 @@ struct Call {
     Prepare prepare;
 };
 
-template <int NT, bool Runs>
-int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call& c, cudaStream_t stream) {
+template <int NT, bool Runs, int Groups>
+int launch_groups(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call& c, cudaStream_t stream) {
     static bool ready[64] = {};
     int device = 0;
     cudaError_t status = cudaGetDevice(&device);
     if (status != cudaSuccess) return static_cast<int>(status);
     if (device >= 64 || !ready[device]) {
-        status = cudaFuncSetAttribute(decode8_kernel<NT, Runs>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes());
+        status = cudaFuncSetAttribute(decode8_kernel<NT, Runs, Groups>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes<Groups>());
         if (status != cudaSuccess) return static_cast<int>(status);
         if (device < 64) ready[device] = true;
     }
@@ -750,20 +761,32 @@ int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call&
     // Long sequences start first, so that the SMs share them out and short ones fill what is left at the end, up to three times as many blocks as there are places: 40 of 64 to 6,000
     // positions 74 -> 59 us, 64 of up to 2,048 46 -> 36, 200 of up to 1,000 58 -> 52, 8 of 2,048 no slower; beyond that putting them in order costs a block more than it gives
     // (256 of up to 300: 36 -> 38).
-    const long long places = 148ll * (NT == 1 && kHalves == 1 && !Runs ? 4 : 2), blocks = static_cast<long long>(grid.x) * grid.y * grid.z;
+    const long long places = 148ll * (NT == 1 && kHalves == 1 && !Runs && Groups == 1 ? 4 : 2), blocks = static_cast<long long>(grid.x) * grid.y * grid.z;
     const int longest_first = !Runs && c.n_seqs > 1 && c.n_seqs <= kMostOrdered && blocks <= 3 * places;
     // Beside the kernel before it only where all blocks find room at once (8 sequences of 2,048 positions 14.4 -> 13.9 us; 640 blocks of 40 sequences 73 -> 78).
     const bool early = blocks <= places;
     int code;
     if (clustered)
-        code = tau_launch_clusters_as(early, c.splits, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales,
+        code = tau_launch_clusters_as(early, c.splits, decode8_kernel<NT, Runs, Groups>, grid, dim3((kGroupWarps * Groups + 1) * 32), shared_bytes<Groups>(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales,
                                       c.partial_o, c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 1, longest_first, c.prepare);
     else
-        code = tau_launch_as(early, decode8_kernel<NT, Runs>, grid, dim3(kThreads), shared_bytes(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales, c.partial_o,
+        code = tau_launch_as(early, decode8_kernel<NT, Runs, Groups>, grid, dim3((kGroupWarps * Groups + 1) * 32), shared_bytes<Groups>(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales, c.partial_o,
                              c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0, longest_first, c.prepare);
     if (code == 0 && c.splits > kMostClustered)
         code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? (D + 31) / 32 * 32 : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
     return code ? code : tau_launch_status();
+}
+
+template <int NT, bool Runs>
+int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call& c, cudaStream_t stream) {
+    // Two groups of warps where all their blocks, two to an SM, fit at once, one to an SM in clusters of more than four, which find room less easily (a decode step of 8 layers, ms in one
+    // group and two: one sequence of 300 positions 0.556 and 0.541, of 16,000 0.72 and 0.68; 8 of 2,000 in two ranges 0.683 and 0.641; 4 of 1,000 in four ranges 0.630 and 0.601, in
+    // eight 0.608 and 0.646).
+    if constexpr (NT == 1 && kHalves == 1 && !Runs) {
+        const bool crowded = c.splits > 4 && c.splits <= kMostClustered;
+        if (static_cast<long long>(c.splits) * c.n_kv_heads * c.passes * c.n_seqs <= (crowded ? 148 : 2 * 148)) return launch_groups<NT, Runs, 2>(key_map, value_map, c, stream);
+    }
+    return launch_groups<NT, Runs, 1>(key_map, value_map, c, stream);
 }
 
 }  // namespace

@@ -315,7 +315,7 @@ store_kernel(StoreSource source, uint8_t* __restrict__ key_pages, uint8_t* __res
         }
         __syncthreads();
     }
-    const float scale = store_in_page(staged, count, D, older, page, scale_at, greatest_of, 256);
+    const float scale = store_in_page(staged, count, D, older, page, scale_at, greatest_of);
     if (threadIdx.x == 0) *scale_at = scale;
 }
 

@@ -122,14 +122,15 @@ __device__ __forceinline__ Neighbours<PER> prepare_neighbours(const Neighbours<P
     return result;
 }
 
-// `threads` threads of a block (numbers 0 .. threads - 1, all of its threads if `whole_block`, else its first four warps) bring `count` rows of D elements in shared memory into a page of one head, behind the `older`
+// `Threads` threads of a block (its first ones, or, with 0, all of it) bring `count` rows of D elements in shared memory into a page of one head, behind the `older`
 // positions that it holds: the scale is the page's own (none for a page that starts here) or what the new rows need, whichever is greater, and codes that are there are rounded to
 // one that grew.  Returns the page's scale, which one thread then writes to `scale_at`; every thread has read the old one by then.  `greatest_of`: a float for each warp.
-template <bool WholeBlock = true>
-__device__ __forceinline__ float store_in_page(const bf16* rows, int count, int D, int older, uint8_t* page, const float* scale_at, float* greatest_of, int threads) {
+template <int Threads = 0>
+__device__ __forceinline__ float store_in_page(const bf16* rows, int count, int D, int older, uint8_t* page, const float* scale_at, float* greatest_of) {
+    const int threads = Threads == 0 ? static_cast<int>(blockDim.x) : Threads;
     auto meet = [&]() {
-        if constexpr (WholeBlock) __syncthreads();
-        else asm volatile("bar.sync 1, 128;" ::: "memory");
+        if constexpr (Threads == 0) __syncthreads();
+        else asm volatile("bar.sync 1, %0;" ::"n"(Threads) : "memory");
     };
     float greatest = 0.0f;
     for (int piece = threadIdx.x; piece < count * D / 8; piece += threads) {

@@ -1283,16 +1283,18 @@ def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_row
 def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int] = None) -> int:
     """Ranges that the pages of a sequence are cut into for `attention_decode8`, whose blocks (`kv_blocks` to a sequence and range) fit an SM four at a time.
 
-    Two blocks to an SM are wanted however few pages each then has (one sequence of 300 positions over 8 heads: 5.2 us in five ranges, 6.6 in one; 8 of 2,048: 14.0 us in
-    four ranges, 18.3 in two, 15.2 in eight); the other two places only with 8 pages or more to a block (2 of 120,000: 88 us in 37 ranges, 110 in 16); and where sequences alone
-    nearly fill the places long ones are halved, since they may differ (40 of 64 to 6,000 positions: 59 us in two ranges, 84 in one; but 100 of up to 3,000, more than there
-    are places: 75 in two, 63 in one).  Four rather than three (20 of up to 12,000: 59 and 68; 24 of 6,000: 68 and 77; of up to 6,000: 45 and 43).  Up to 8 ranges
-    meet in a cluster, more through memory and a second launch, so numbers just above 8 become 8.  The length is rounded up to a power of two first, so that a
+    One block to an SM is wanted however few pages each then has, though no more than 8 ranges, which meet in a cluster (a decode step of 8 layers, ms: one sequence of 300 positions
+    over 8 heads 0.547 in eight ranges, 0.583 in one; 4 of 1,000 0.601 in four, 0.65 in eight); two blocks to an SM with 8 pages or more to a block (4 of 4,000: 0.66 in eight, 0.71 in
+    four); and all places with 16 or more (us alone: 2 of 120,000 88 in 37 ranges, 98 in 16; 8 of 16,000 44 in eight, 49 in four).  Where sequences alone nearly fill the places long
+    ones are halved, since they may differ (40 of 64 to 6,000 positions: 59 us in two ranges, 84 in one; but 100 of up to 3,000, more than there
+    are places: 75 in two, 63 in one).  Four rather than three (20 of up to 12,000: 59 and 68; 24 of 6,000: 68 and 77; of up to 6,000: 45 and 43).  More than 8 ranges
+    meet through memory and a second launch, so numbers just above 8 become 8.  The length is rounded up to a power of two first, so that a
     captured graph serves a range of lengths."""
     sms = sms or sm_count()
     pages = max(1, (1 << max(0, (max_len - 1).bit_length())) // PAGE_TOKENS)
     blocks = max(1, n_seqs * kv_blocks)
-    splits = max(1, min(pages, 64, max(2 * sms // blocks, min(4 * sms // blocks, pages // 8), min(2, pages // 32) if blocks <= 4 * sms else 1)))
+    splits = max(1, min(pages, 64, max(min(sms // blocks, DECODE8_CLUSTERED), min(2 * sms // blocks, pages // 8), min(4 * sms // blocks, pages // 16),
+                                       min(2, pages // 32) if blocks <= 4 * sms else 1)))
     return 4 if splits == 3 else DECODE8_CLUSTERED if DECODE8_CLUSTERED < splits < 12 else splits
 
 

@@ -223,7 +223,7 @@ def test_ranges_of_a_decode_over_8_bit_pages():
     """The rule's corners: never more ranges than pages, one where sequences fill the machine, numbers just above a cluster's eight become eight."""
     splits = kernels.decode8_splits
     assert splits(1, 1, 8, 148) == 1 and splits(1, 64, 8, 148) == 1 and splits(1, 300, 8, 148) == 8 and splits(8, 2048, 8, 148) == 4
-    assert splits(64, 2048, 8, 148) == 1 and splits(40, 6000, 8, 148) == 2 and splits(2, 120000, 8, 148) == 37 and splits(4, 1000, 8, 148) == 8
+    assert splits(64, 2048, 8, 148) == 1 and splits(40, 6000, 8, 148) == 2 and splits(2, 120000, 8, 148) == 37 and splits(4, 1000, 8, 148) == 4
     for n_seqs in (1, 3, 17, 64, 500):
         for length in (1, 65, 1000, 33000, 1 << 20):
             found = splits(n_seqs, length, 8, 148)
