@@ -12,8 +12,7 @@ namespace {
 template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_blocks_kernel(const T* __restrict__ values, long long stride, uint8_t* __restrict__ codes, float* __restrict__ scales, int rows, int columns) {
-    grid_dependents_launch();
-    grid_dependency_wait();
+    grid_dependency_wait();      // and nothing starts beside this kernel: products ask for their weight before what is in front of them has ended
     __shared__ float greatest_of[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row0 = blockIdx.y * kScaleBlock, column = blockIdx.x * kScaleBlock + lane * 4;

@@ -143,6 +143,27 @@ def test_the_streaming_product(rows, depth, features):
         assert bool(((out.double() - wanted).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("rows", [1, 12, 40, 300])
+def test_a_product_directly_behind_its_weights_quantising(rows):
+    """Codes land where the weight before had its own: a product that asked for them too early would multiply with those."""
+    x = torch.randn(rows, 4096, device="cuda").to(torch.bfloat16)
+    weights = [(torch.randn(6144, 4096, device="cuda") * 4.0 ** turn).to(torch.bfloat16) for turn in range(4)]
+    wanted = []
+    for weight in weights:
+        held = kernels.quantize_blocks(weight)
+        torch.cuda.synchronize()
+        out = torch.empty(rows, 6144, device="cuda")
+        kernels.linear8(x, *held, None, out)
+        wanted.append(out)
+        del held
+    for weight, result in zip(weights, wanted):
+        out = torch.empty(rows, 6144, device="cuda")
+        held = kernels.quantize_blocks(weight)
+        kernels.linear8(x, *held, None, out)
+        del held
+        assert torch.equal(out, result)
+
+
 def test_a_row_that_is_not_finite_stays_alone():
     """An infinity and a NaN in two rows make those rows' results NaN and leave the others as they are; so does a NaN in a weight's row for its feature."""
     for rows in (4, 40, 300):
