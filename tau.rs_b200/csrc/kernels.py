@@ -1096,10 +1096,11 @@ def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
         raise KernelError("the depth must be a multiple of 16")
     if scales.dtype is not torch.float32 or scales.shape != (-(-features // SCALE_BLOCK), -(-depth // SCALE_BLOCK)) or not scales.is_contiguous():
         raise KernelError("the weight's scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)]")
-    if values.dtype not in _DTYPE_CODE or values.stride(1) != 1 or values.stride(0) % 8 or values.data_ptr() % 16:
+    apart, unit = values.stride()
+    if values.dtype not in _DTYPE_CODE or unit != 1 or apart % 8 or values.data_ptr() % 16:
         raise KernelError("activations must be bfloat16 or float32 with rows on 16-byte borders")
     columns = features // 2 if gated else features
-    if out.shape != (rows, columns) or (columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns):
+    if out.shape != (rows, columns) or not out.is_contiguous() and ((columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns)):
         raise KernelError("the output must be [M, N], or [M, N / 2] of a gated product")
     if out.dtype is not torch.bfloat16 and (gated or out.dtype is not torch.float32):
         raise KernelError("the output must be bfloat16 (or float32 where nothing is gated)")
@@ -1210,8 +1211,9 @@ def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_r
         raise KernelError("cache pages must be float8_e4m3fn [pages, n_kv_heads, 64, head_dim]")
     if shape[3] % 16 or not 16 <= shape[3] <= 256:
         raise KernelError("head_dim must be a multiple of 16 between 16 and 256")
+    page_heads = shape[:2]
     for scales in (key_scales, value_scales):
-        if scales.dtype is not torch.float32 or scales.shape != shape[:2] or not scales.is_contiguous():
+        if scales.dtype is not torch.float32 or scales.shape != page_heads or not scales.is_contiguous():
             raise KernelError("the pages' scales must be float32 [pages, n_kv_heads]")
     sequences = step.n_seqs
     if page_rows.dtype is not torch.int32 or page_rows.dim() != 2 or page_rows.shape[0] != sequences or not page_rows.is_contiguous():
@@ -1219,7 +1221,7 @@ def _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_r
     if step.max_len > page_rows.shape[1] * PAGE_TOKENS:
         raise KernelError("page rows must hold the pages of the step's longest sequence")
     for tensor, count in ((step.cu_seqlens, sequences + 1), (step.seq_start, sequences), (step.seq_len, sequences)):
-        if tensor.dtype is not torch.int32 or tensor.numel() != count or tensor.stride(0) != 1:
+        if tensor.dtype is not torch.int32 or tensor.numel() != count or not tensor.is_contiguous():
             raise KernelError("a step's cu_seqlens, seq_start and seq_len must be int32, one (and one more bound) to a sequence")
 
 
