@@ -1361,18 +1361,23 @@ def _check_rotation(q_weight, k_weight, cos, sin, rotary_dim: int, head_dim: int
 
 RUNS8_COLUMNS = 64          # of new tokens times a group's query heads, up to which runs are worked on like single tokens, 16 columns to a reading of the pages (us against pages laid
                             # out in 16 bits and their kernels: 4 sequences of 2,000 positions, 32 heads of 128 over 8, 8 tokens each 23 and 50, 32 tokens 69 and 50; 8 of 8,000 and
-                            # 16 tokens 184 and 211) ...
-RUNS8_COLUMNS_OTHER = 160   # ... for heads whose 16-bit kernel has no tensor memory (16 tokens of 32 heads of 80 over 8 behind 2,000: 36 and 97) ...
+                            # 16 tokens 184 and 211); heads of more than 128, 8 columns to a reading, half as many
 RUNS8_FEW_PAGES = 2048      # ... and wherever the pages are read no more often than this in all: a launch where the other way takes two (one sequence of 500, 64 tokens: 19 and 17, and
-                            # 18 us less on the host)
+                            # 18 us less on the host) ...
+RUNS8_READINGS = 700        # ... and, for heads whose 16-bit kernel has no tensor memory and takes some 3 us to a page one after another, than so often for each page of the longest but 8
+RUNS8_READINGS_WIDE = 400   # (32 heads over 8, of 80: one sequence of 3,000, 100 tokens 71 and 158; 4 of 2,000, 64 tokens 86 and 115, 128 tokens 160 and 115; 16 of 2,000, 32 tokens
+                            # 160 and 135; of 256: one of 3,000, 100 tokens 147 and 202; 4 of 2,000, 64 tokens 206 and 154)
 
 
 def runs8_like_single_tokens(n_seqs: int, max_new: int, max_len: int, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
     """Whether `attention8` takes a step of runs to the kernel of single tokens, which reads pages as they are held."""
-    columns = max_new * (n_heads // n_kv_heads)
-    if columns <= (RUNS8_COLUMNS if head_dim in (64, 128) else RUNS8_COLUMNS_OTHER):
+    columns, pages = max_new * (n_heads // n_kv_heads), -(-max_len // PAGE_TOKENS)
+    readings = n_seqs * n_kv_heads * pages * -(-columns // 16)
+    if columns <= (RUNS8_COLUMNS if head_dim <= 128 else RUNS8_COLUMNS // 2) or readings <= RUNS8_FEW_PAGES:
         return True
-    return n_seqs * n_kv_heads * -(-max_len // PAGE_TOKENS) * -(-columns // 16) <= RUNS8_FEW_PAGES
+    return head_dim not in (64, 128) and readings <= (RUNS8_READINGS if head_dim <= 128 else RUNS8_READINGS_WIDE) * (pages - 8)
+
+
 _decode8_functions = {}
 DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 

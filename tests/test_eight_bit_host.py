@@ -233,5 +233,6 @@ def test_ranges_of_a_decode_over_8_bit_pages():
 def test_which_runs_are_worked_on_like_single_tokens():
     rule = kernels.runs8_like_single_tokens
     assert rule(4, 16, 4500, 32, 8, 128) and not rule(4, 17, 4500, 32, 8, 128)      # 64 and 68 columns
-    assert rule(4, 40, 4500, 32, 8, 80) and not rule(4, 41, 4500, 32, 8, 80)        # 160 and 164
+    assert rule(4, 76, 4500, 32, 8, 80) and not rule(4, 77, 4500, 32, 8, 80)        # 19 and 20 readings of 4 x 8 x 71 pages, for 700 x 63
+    assert rule(64, 8, 2000, 32, 8, 256) and not rule(64, 9, 2000, 32, 8, 256)      # 32 and 36 columns
     assert rule(1, 64, 500, 32, 8, 128) and not rule(1, 256, 500, 32, 8, 128)       # 8 heads x 8 pages x 16 readings, x 64
