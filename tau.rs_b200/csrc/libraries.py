@@ -33,7 +33,7 @@ def all_libraries() -> List[Tuple[str, Sequence[str]]]:
         # Specialised libraries: the head sizes of the benchmark shape and of the tests' tiny models.
         *[("attention_decode.cu", (f"TAU_HEAD_DIM={head_dim}", f"TAU_DTYPE={dtype}"))
           for head_dim in (128, 64, 16, 32, 48, 80) for dtype in (0, 1)],
-        *[("attention_decode8.cu", (f"TAU_HEAD_DIM={head_dim}",)) for head_dim in (128, 64, 16, 32, 48, 80)],
+        *[("attention_decode8.cu", (f"TAU_HEAD_DIM={head_dim}",)) for head_dim in (128, 64, 16, 32, 48, 80, 96, 256)],
         *[("attention_prefill.cu", (f"TAU_HEAD_DIM={head_dim}",)) for head_dim in (128, 16, 32, 48, 80, 192)],
         *[("attention_prefill_tc.cu", (f"TAU_HEAD_DIM={head_dim}",)) for head_dim in (128, 64)],
         ("attention_prefill_tc.cu", ("TAU_HEAD_DIM=192", "TAU_VALUE_DIM=128")),
