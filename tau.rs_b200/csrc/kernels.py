@@ -1312,7 +1312,8 @@ def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales,
     n_seqs, n_tokens = step.n_seqs, step.n_tokens
     single = step.all_single
     passes = _passes8(n_heads // n_kv_heads * (1 if single else step.max_new), head_dim)
-    splits = min((step.decode_splits if single else 0) or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes), 256)
+    splits = (step.decode_splits if single else 0) or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes)
+    splits = min(splits, window // PAGE_TOKENS + 2 if window and single else 256, 256)      # a window lies in so many pages
     scratch = torch.empty(n_tokens * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
     run = _decode8_functions.get(head_dim)
     if run is None:
