@@ -38,6 +38,7 @@ constexpr int kStagesOf = kHalves == 1 ? 2 * Groups : 3;
 constexpr int kMostStages = kHalves == 1 ? 4 : 3;
 constexpr int kKeySteps = D / 16;                 // products of 16 head elements
 constexpr int kMostClustered = 8;
+constexpr float kFailed = -1.0f;                  // in the place of a range's sum of weights (never negative): a wait ran out there
 constexpr int kMostOrdered = 1024;                // sequences that a block puts in order
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are kept times 2^14: what f16 holds with all its bits then reaches down to 2^-28 of the greatest, and a long tail of small weights keeps its sum.
@@ -71,6 +72,9 @@ struct Prepare {
 
 __device__ __forceinline__ void tma_load_3d(void* destination, const CUtensorMap* map, int x, int y, int z, uint64_t* barrier) {
     if (operands_lost()) return;
+#ifdef TAU_LOST_RANGE      // the test of a wait that runs out where ranges meet through memory
+    if (blockIdx.x == TAU_LOST_RANGE) return;
+#endif
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_address(destination)),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_address(barrier))
                  : "memory");
@@ -638,12 +642,12 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 block_ml[h][0] = total_max;
                 block_ml[h][1] = sum;
             }
-        } else if (!failed) {
+        } else {
             const size_t slot = place(h) * splits + split;
-            if (sum != 0.0f) partial_o[slot * D + c] = o;
+            if (sum != 0.0f && !failed) partial_o[slot * D + c] = o;
             if (c == 0) {
                 partial_ml[slot * 2] = total_max;
-                partial_ml[slot * 2 + 1] = sum;
+                partial_ml[slot * 2 + 1] = failed ? kFailed : sum;
             }
         }
     }
@@ -684,28 +688,38 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     cluster_sync_all();      // nobody leaves while its results are read
 }
 
-// Joins the records of a sequence's ranges in their order: a block (of whole warps) to a head, a thread to a column.
+// Joins the records of a sequence's ranges in their order: a block (of whole warps) to a head, a thread to a column.  A head of which a range failed is left as it was.
 __global__ void join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out, int n_heads, int splits) {
     grid_dependents_launch();
     grid_dependency_wait();
     __shared__ float factor[256];
     __shared__ float inverse;
+    __shared__ bool failed;
     const int head = blockIdx.x, seq = blockIdx.y;
     const size_t base = (static_cast<size_t>(seq) * n_heads + head) * splits;
     if (threadIdx.x < 32) {
         float total_max = -INFINITY, sum = 0.0f;
-        for (int s = threadIdx.x; s < splits; s += 32)
-            if (partial_ml[(base + s) * 2 + 1] != 0.0f) total_max = fmaxf(total_max, partial_ml[(base + s) * 2]);
+        bool lost = false;
+        for (int s = threadIdx.x; s < splits; s += 32) {
+            const float own = partial_ml[(base + s) * 2 + 1];
+            if (own != 0.0f) total_max = fmaxf(total_max, partial_ml[(base + s) * 2]);
+            lost |= own == kFailed;
+        }
         total_max = warp_max(total_max);
+        lost = __any_sync(0xffffffffu, lost);
         for (int s = threadIdx.x; s < splits; s += 32) {
             const float own = partial_ml[(base + s) * 2 + 1];
             factor[s] = own != 0.0f ? exp2f(partial_ml[(base + s) * 2] - total_max) : 0.0f;
             sum += own != 0.0f ? own * factor[s] : 0.0f;
         }
         sum = warp_sum(sum);
-        if (threadIdx.x == 0) inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (threadIdx.x == 0) {
+            inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+            failed = lost;
+        }
     }
     __syncthreads();
+    if (failed) return;
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
         float o = 0.0f;
 #pragma unroll 8

@@ -37,3 +37,27 @@ def test_attention_whose_ranges_meet_in_a_cluster(lost_rank, heads, dim):
         step.decode_splits = 4
         kernels.attention_decode8(queries, *pages, out, step, table, heads, 2, dim, dim ** -0.5, 0)
         assert build.load_library("attention_decode8.cu", (f"TAU_HEAD_DIM={dim}",)).tau_decode8_status() == 1 and bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("heads, dim", [(8, 64), (32, 128)])
+def test_attention_whose_ranges_meet_through_memory(monkeypatch, heads, dim):
+    """Sixteen ranges leave records for a second kernel, and one of them gives up: what it is missing from stays as it was, a sequence that has no page there is complete."""
+    lost = ("TAU_LOST_COPIES", "TAU_WAIT_LIMIT_NS=1000000ull", "TAU_LOST_RANGE=1")
+    torch.manual_seed(0)
+    pages = [torch.randn(33, 2, 64, dim, device="cuda").to(eight.CODES) for _ in range(2)] + [torch.ones(33, 2, device="cuda") for _ in range(2)]
+    table = torch.zeros(3, 16, dtype=torch.int32, device="cuda")
+    table[0], table[1, 0], table[2] = torch.arange(16), 16, torch.arange(17, 33)
+    runs = [(1000, 1), (40, 1), (1023, 1)]
+    queries = torch.randn(3, heads * dim, device="cuda").to(torch.bfloat16)
+    out, wanted = (torch.full_like(queries, 7.0) for _ in range(2))
+    step = eight.make_step(runs)
+    step.decode_splits = 16
+    kernels.attention_decode8(queries, *pages, wanted, step, table, heads, 2, dim, dim ** -0.5, 0)
+    torch.cuda.synchronize()
+    assert not bool((wanted == 7.0).all(1).any())
+    monkeypatch.setattr(build, "load_library", lambda source, defines=(), load=build.load_library: load(source, (*defines, *lost)))
+    monkeypatch.setattr(kernels, "_functions", {})
+    monkeypatch.setattr(kernels, "_decode8_functions", {})
+    kernels.attention_decode8(queries, *pages, out, step, table, heads, 2, dim, dim ** -0.5, 0)
+    assert build.load_library("attention_decode8.cu", (f"TAU_HEAD_DIM={dim}",)).tau_decode8_status() == 1
+    assert bool((out[0] == 7.0).all()) and bool((out[2] == 7.0).all()) and torch.equal(out[1], wanted[1])
