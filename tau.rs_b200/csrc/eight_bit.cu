@@ -419,11 +419,13 @@ TAU_EXPORT int tau_quantize_rows(int dtype, const void* values, long long stride
     return launch_quantize_rows(dtype, values, stride, codes, scales, rows, columns, static_cast<cudaStream_t>(stream));
 }
 
-// x codes [M, K] with scales [blocks, M]; w codes [N, K] with scales [blocks of N, blocks]; both contiguous, K a multiple of 16.
+// x codes [M, K] with scales [blocks, M]; w codes [N, K] with scales [blocks of N, blocks]; both contiguous on 16-byte borders, K a multiple of 16.
 TAU_EXPORT int tau_gemm8_simt(int out_dtype, const void* x, const float* x_scales, const void* w, const float* w_scales, const float* bias, void* out, int M, int N, int K,
                               long long out_stride, void* stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (!x || !x_scales || !w || !w_scales || !out || K <= 0 || (K & 15) || (out_dtype != TAU_BF16 && out_dtype != TAU_F32)) return cudaErrorInvalidValue;
+    if (!x || !x_scales || !w || !w_scales || !out || K <= 0 || (K & 15) || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
+        (out_dtype != TAU_BF16 && out_dtype != TAU_F32))
+        return cudaErrorInvalidValue;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (M > 65535 * 32) return cudaErrorInvalidValue;
     const dim3 grid((N + 31) / 32, (M + 31) / 32);

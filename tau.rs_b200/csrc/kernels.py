@@ -1092,6 +1092,8 @@ def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
         raise KernelError("shapes must be [M,K] x [N,K] -> [M,N]")
     if codes.dtype is not CODE_DTYPE or not codes.is_contiguous():
         raise KernelError("the weight must be contiguous float8_e4m3fn codes")
+    if codes.data_ptr() % 16:
+        raise KernelError("the weight's codes must begin on a 16-byte border")
     if depth % 16 or not depth:
         raise KernelError("the depth must be a multiple of 16")
     if scales.dtype is not torch.float32 or scales.shape != (-(-features // SCALE_BLOCK), -(-depth // SCALE_BLOCK)) or not scales.is_contiguous():

@@ -236,3 +236,19 @@ def test_which_runs_are_worked_on_like_single_tokens():
     assert rule(4, 76, 4500, 32, 8, 80) and not rule(4, 77, 4500, 32, 8, 80)        # 19 and 20 readings of 4 x 8 x 71 pages, for 700 x 63
     assert rule(64, 8, 2000, 32, 8, 256) and not rule(64, 9, 2000, 32, 8, 256)      # 32 and 36 columns
     assert rule(1, 64, 500, 32, 8, 128) and not rule(1, 256, 500, 32, 8, 128)       # 8 heads x 8 pages x 16 readings, x 64
+
+
+@pytest.mark.parametrize("optimized", [True, False])
+def test_products_refuse_codes_that_begin_between_borders(optimized):
+    """Codes are read four and sixteen at a time, by the plain kernel too."""
+    operands = product_operands()
+    operands["codes"] = torch.zeros(16 * 32 + 1, dtype=torch.uint8)[1:].view(16, 32).view(CODES)
+    assert operands["codes"].is_contiguous()
+    kernels.prefer_optimized(optimized)
+    try:
+        with pytest.raises(kernels.KernelError, match="16-byte border"):
+            kernels.linear8(operands["values"], operands["codes"], operands["scales"], None, operands["out"])
+        with pytest.raises(kernels.KernelError, match="16-byte border"):
+            kernels.linear8_gated(operands["values"], operands["codes"], operands["scales"], torch.zeros(3, 8, dtype=torch.bfloat16))
+    finally:
+        kernels.prefer_optimized(True)
