@@ -1087,6 +1087,25 @@ def quantize_rows(values):
 
 
 def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
+    _two(values, codes)
+    apart, unit = values.stride()
+    if values.dtype not in _DTYPE_CODE or unit != 1 or apart % 8 or values.data_ptr() % 16:
+        raise KernelError("activations must be bfloat16 or float32 with rows on 16-byte borders")
+    _check_weight8(values, codes, scales, bias, out, gated)
+
+
+def _check_codes8(x_codes, x_scales, codes, scales, bias, out, gated: bool) -> None:
+    """For the products whose activations are quantised already (`quantize_rows`)."""
+    if x_codes.dtype is not CODE_DTYPE or not x_codes.is_contiguous() or x_codes.data_ptr() % 16:
+        raise KernelError("the activations must be contiguous float8_e4m3fn codes on a 16-byte border")
+    (rows, depth), _ = _two(x_codes, codes)
+    if x_scales.dtype is not torch.float32 or x_scales.shape != (-(-depth // SCALE_BLOCK), rows) or not x_scales.is_contiguous():
+        raise KernelError("the activations' scales must be contiguous float32 [ceil(K / 128), M]")
+    _check_weight8(x_codes, codes, scales, bias, out, gated)
+    _here(x_scales)
+
+
+def _check_weight8(values, codes, scales, bias, out, gated: bool) -> None:
     (rows, depth), (features, weight_depth) = _two(values, codes)
     if depth != weight_depth:
         raise KernelError("shapes must be [M,K] x [N,K] -> [M,N]")
@@ -1098,9 +1117,6 @@ def _check_linear8(values, codes, scales, bias, out, gated: bool) -> None:
         raise KernelError("the depth must be a multiple of 16")
     if scales.dtype is not torch.float32 or scales.shape != (-(-features // SCALE_BLOCK), -(-depth // SCALE_BLOCK)) or not scales.is_contiguous():
         raise KernelError("the weight's scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)]")
-    apart, unit = values.stride()
-    if values.dtype not in _DTYPE_CODE or unit != 1 or apart % 8 or values.data_ptr() % 16:
-        raise KernelError("activations must be bfloat16 or float32 with rows on 16-byte borders")
     columns = features // 2 if gated else features
     if out.shape != (rows, columns) or not out.is_contiguous() and ((columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns)):
         raise KernelError("the output must be [M, N], or [M, N / 2] of a gated product")
@@ -1121,6 +1137,7 @@ def _two(values, codes):
 
 def gemm8_simt(x_codes, x_scales, codes, scales, bias, out) -> None:
     """The plain product of operands in 8 bits (`quantize_rows`, `quantize_blocks`), on the 32-bit pipes: every size, the kernel that the others are checked against."""
+    _check_codes8(x_codes, x_scales, codes, scales, bias, out, False)
     rows, depth = x_codes.shape
     run = _function("eight_bit.cu", "tau_gemm8_simt", "ippppppiiil")
     _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
@@ -1136,6 +1153,7 @@ SKINNY8_MOST_DEPTH = 6144        # 5.5; 6,144 x 4,096 8.4 and 11.6; 2,048 x 8,19
 
 def gemm8_skinny(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
     """The product of at most 16 quantised rows, bound by streaming the weight's codes once."""
+    _check_codes8(x_codes, x_scales, codes, scales, bias, out, gated)
     _require(x_codes.shape[0] <= SKINNY8_MAX_ROWS, "too many rows for the skinny kernel")
     rows, depth = x_codes.shape
     run = _function("gemm8_skinny.cu", "tau_gemm8_skinny", "ippppppiiilif")
@@ -1153,12 +1171,15 @@ def gemm8_stream(values, codes, scales, bias, out, gated: bool = False, gate_lim
     """The product of at most 8 bfloat16 rows: a block to an SM, which quantises the rows once and streams its share of the weight's codes."""
     _require(values.dtype == torch.bfloat16 and values.shape[0] <= STREAM8_MAX_ROWS and codes.shape[1] <= STREAM8_MAX_DEPTH,
              f"the streaming product takes at most {STREAM8_MAX_ROWS} bfloat16 rows of at most {STREAM8_MAX_DEPTH} columns")
+    _check_linear8(values, codes, scales, bias, out, gated)
     _stream8(values, codes, scales, bias, out, gated, gate_limit)
 
 
 def gemm8_tc(x_codes, x_scales, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0, features: int = 0, ranges: int = 0) -> None:
     """The product on the tcgen05 tensor cores, any number of rows, in tiles of 128 rows and `features` (128, 192, 256) with K cut into `ranges` (1 to 8);
     0: by what the tiles' rounds cost."""
+    _check_codes8(x_codes, x_scales, codes, scales, bias, out, gated)
+    _require(features in (0, 128, 192, 256) and 0 <= ranges <= 8, "tiles have 128, 192 or 256 features, and K is cut into 1 to 8 ranges")
     rows, depth = x_codes.shape
     run = _function("gemm8_tc.cu", "tau_gemm8_tc", "ippppppiiilifii")
     _check(run(_code(out), x_codes.data_ptr(), x_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), _address(bias), out.data_ptr(), rows, codes.shape[0], depth, out.stride(0),
@@ -1307,10 +1328,15 @@ def _passes8(columns: int, head_dim: int) -> int:
     return -(-columns // (16 if columns > 8 and head_dim <= 128 else 8))
 
 
-def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int,
-                      prepare=None) -> None:
-    """One query token per sequence over its `seq_len` cached positions, or a few, read as they are held (`attention8` and `attention8_decode_fused` check their arguments).
-    `prepare`: see there; `queries` is then None."""
+def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
+    """`attention8` by the kernel that reads pages as they are held, whatever the step: one query token per sequence over its `seq_len` cached positions, or a few."""
+    _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, window)
+    if step.n_tokens:
+        _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
+
+
+def _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int, prepare=None) -> None:
+    """The launch; its arguments are checked.  `prepare`: see `attention8_decode_fused`; `queries` is then None."""
     n_seqs, n_tokens = step.n_seqs, step.n_tokens
     single = step.all_single
     passes = _passes8(n_heads // n_kv_heads * (1 if single else step.max_new), head_dim)
@@ -1349,8 +1375,8 @@ def attention8_decode_fused(projected, key_pages, value_pages, key_scales, value
     _check_rotation(q_weight, k_weight, cos, sin, rotary_dim, head_dim, step.max_len)
     _here(projected, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_len, q_weight, k_weight, cos, sin)
     if step.n_tokens:
-        attention_decode8(None, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window,
-                          prepare=(projected, q_weight, k_weight, eps, cos, sin, rotary_dim, write_cache))
+        _decode8(None, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window,
+                 prepare=(projected, q_weight, k_weight, eps, cos, sin, rotary_dim, write_cache))
     return True
 
 
@@ -1388,8 +1414,7 @@ DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluste
 READ8_BYTES = 1 << 30      # of pages read back at once
 
 
-def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
-    """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
+def _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, window: int) -> None:
     _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
     if key_pages.shape[1] != n_kv_heads or key_pages.shape[3] != head_dim or n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads <= 0:
         raise KernelError("the pages must be [pages, n_kv_heads, 64, head_dim] and n_heads a multiple of n_kv_heads")
@@ -1399,10 +1424,15 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     if window < 0:
         raise KernelError("a window must not be negative")
     _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
+
+
+def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
+    """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
+    _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, window)
     if step.n_tokens == 0:
         return
     if _prefer_optimized and (step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim))):
-        return attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
+        return _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
     # Every sequence has room for the longest, so they are taken a few at a time where that would be much (the plain kernel goes by the step's own numbers and takes all at once).
     sequences, stride = page_rows.shape

@@ -252,3 +252,57 @@ def test_products_refuse_codes_that_begin_between_borders(optimized):
             kernels.linear8_gated(operands["values"], operands["codes"], operands["scales"], torch.zeros(3, 8, dtype=torch.bfloat16))
     finally:
         kernels.prefer_optimized(True)
+
+
+def quantised_operands(rows=3, depth=272, features=16):
+    return dict(x_codes=torch.zeros(rows, depth, dtype=torch.uint8).view(CODES), x_scales=torch.ones(-(-depth // 128), rows), codes=torch.zeros(features, depth, dtype=torch.uint8).view(CODES),
+                scales=torch.ones(-(-features // 128), -(-depth // 128)), bias=None, out=torch.zeros(rows, features, dtype=torch.bfloat16))
+
+
+BETWEEN_BORDERS = torch.zeros(3 * 272 + 1, dtype=torch.uint8)[1:].view(3, 272).view(CODES)
+
+
+@pytest.mark.parametrize("product", [kernels.gemm8_simt, kernels.gemm8_skinny, kernels.gemm8_tc])
+@pytest.mark.parametrize("change, message", [
+    (dict(x_scales=torch.ones(2, 3)), "activations' scales"),
+    (dict(x_scales=torch.ones(3, 2)), "activations' scales"),
+    (dict(x_scales=torch.ones(3, 3, dtype=torch.float64)), "activations' scales"),
+    (dict(x_scales=torch.ones(3, 6)[:, ::2]), "activations' scales"),
+    (dict(x_codes=torch.zeros(3, 272, dtype=torch.bfloat16)), "activations"),
+    (dict(x_codes=torch.zeros(3, 256, dtype=torch.uint8).view(CODES), x_scales=torch.ones(2, 3)), "shapes"),
+    (dict(x_codes=torch.zeros(3, 288, dtype=torch.uint8).view(CODES)[:, :272]), "activations"),
+    (dict(x_codes=BETWEEN_BORDERS), "16-byte border"),
+    (dict(scales=torch.ones(1, 2)), "weight's scales"),
+    (dict(scales=torch.ones(2, 3)), "weight's scales"),
+    (dict(codes=torch.zeros(16, 272, dtype=torch.uint8)), "float8_e4m3fn"),
+    (dict(codes=BETWEEN_BORDERS, out=torch.zeros(3, 3)), "16-byte border"),
+    (dict(bias=torch.ones(15)), "bias"),
+    (dict(out=torch.zeros(2, 16)), "output"),
+    (dict(out=torch.zeros(3, 8)), "output"),
+    (dict(out=torch.zeros(3, 16, dtype=torch.float16)), "output"),
+    (dict(out=torch.zeros(16, 3).T), "output"),
+    (dict(), "CUDA"),
+])
+def test_products_of_quantised_operands_refuse(product, change, message):
+    with pytest.raises(kernels.KernelError, match=message):
+        product(**{**quantised_operands(), **change})
+
+
+def test_the_streaming_and_the_tiled_product_refuse():
+    operands = product_operands()
+    arguments = (operands["values"], operands["codes"], torch.ones(1, 2), None, operands["out"])
+    with pytest.raises(kernels.KernelError, match="scales"):
+        kernels.gemm8_stream(*arguments)
+    with pytest.raises(kernels.KernelError, match="output"):
+        kernels.gemm8_stream(operands["values"], operands["codes"], operands["scales"], None, operands["out"], gated=True)
+    for wrong in (dict(features=64), dict(ranges=9), dict(ranges=-1)):
+        with pytest.raises(kernels.KernelError, match="CUDA|tiles"):
+            kernels.gemm8_tc(**quantised_operands(), **wrong)
+
+
+@pytest.mark.parametrize("change", BAD_PAGES + [dict(queries=torch.zeros(5, 127, dtype=torch.bfloat16)), dict(out=torch.zeros(5, 64, dtype=torch.bfloat16)), dict(heads=3), dict(window=-1), dict()])
+def test_attention_over_pages_as_they_are_held_refuses(change):
+    operands = {**cache_operands(), "queries": torch.zeros(5, 128, dtype=torch.bfloat16), "out": torch.zeros(5, 128, dtype=torch.bfloat16), "heads": 4, "window": 0, **change}
+    with pytest.raises(kernels.KernelError):
+        kernels.attention_decode8(operands["queries"], operands["key_pages"], operands["value_pages"], operands["key_scales"], operands["value_scales"], operands["out"], operands["step"],
+                                  operands["page_rows"], operands["heads"], 2, 32, 1.0, operands["window"])
