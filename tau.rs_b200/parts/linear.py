@@ -28,7 +28,8 @@ class StackedLinear(Part):
         """`biased` (with `bias`): only the pieces whose prefixes it lists have a bias tensor; the others' part of the stacked bias is zero.
         The tensors are named `<prefix><weight_suffix>` and `<prefix><bias_suffix>`.  `interleave` > 0 (two pieces of equal size, no bias): rows are stored in groups of `interleave` rows of the
         first piece followed by the matching rows of the second, which is what a gated product reads.
-        `weight_format` "fp8": the stacked weight is brought to e4m3 codes with a scale for each 128 x 128 when it is complete, and `weight` is None from then on."""
+        `weight_format` "fp8": the stacked weight is brought to e4m3 codes with a scale for each 128 x 128 as soon as its last piece is assigned, so that a model that is being
+        loaded holds one stack at a time in the run's dtype; `weight` stays None."""
         if weight_format not in ("", "fp8"):
             raise ValueError(f"unknown weight format {weight_format!r}")
         width = sum(width for _, width in pieces)
@@ -61,24 +62,26 @@ class StackedLinear(Part):
         if name not in self.tensor_specs():
             raise KeyError(name)
         self._parts[name] = tensor
+        if self.weight_format and all(f"{prefix}{self.weight_suffix}" in self._parts for prefix, _ in self.pieces):
+            self.codes, self.scales = kernels.quantize_blocks(self._stacked())
 
-    def finalize_weights(self):
+    def _stacked(self):
+        """The pieces' weights as one; the pieces are given up."""
         weights = [self._parts.pop(f"{prefix}{self.weight_suffix}") for prefix, _ in self.pieces]
         if self.interleave:
             first, second = weights
             group, width = self.interleave, first.shape[1]
-            self.weight = torch.stack([first.view(-1, group, width), second.view(-1, group, width)], dim=1).reshape(-1, width).contiguous()
-        else:
-            self.weight = weights[0] if len(weights) == 1 else torch.cat(weights, dim=0).contiguous()
-        del weights
+            return torch.stack([first.view(-1, group, width), second.view(-1, group, width)], dim=1).reshape(-1, width).contiguous()
+        return weights[0] if len(weights) == 1 else torch.cat(weights, dim=0).contiguous()
+
+    def finalize_weights(self):
+        if self.codes is None:
+            self.weight = self._stacked()
         if self.has_bias:
             like = next(tensor for name, tensor in self._parts.items() if name.endswith(self.bias_suffix))
             biases = [self._parts.pop(f"{prefix}{self.bias_suffix}") if self.biased is None or prefix in self.biased else torch.zeros(width, dtype=like.dtype, device=like.device)
                       for prefix, width in self.pieces]
             self.bias = biases[0] if len(biases) == 1 else torch.cat(biases, dim=0).contiguous()
-        if self.weight_format:
-            self.codes, self.scales = kernels.quantize_blocks(self.weight)
-            self.weight = None
 
     def bytes_saved_per_step(self) -> int:
         """How many bytes fewer a step reads of this weight than its tensors have in the run's dtype."""

@@ -202,3 +202,23 @@ def test_the_command_line_with_both_formats(folders):
     assert len(json.loads(result.stdout.splitlines()[0])["tokens"]) == 5
     refused = subprocess.run(command[:4] + ["--dtype", "f32"] + command[6:], capture_output=True, text=True, timeout=600)
     assert refused.returncode != 0 and "bfloat16" in refused.stderr
+
+
+def test_loading_weights_in_8_bits_never_holds_the_model_in_16(tmp_path):
+    """From a folder and drawn on the device: the greatest memory in between is the codes' (half the products' bytes), embedding and head, and a stack or two; allowed three quarters of the products."""
+    config = dict(tiny_configs.TINY_B, hidden_size=512, intermediate_size=1536, num_hidden_layers=10, num_attention_heads=8, num_key_value_heads=4, head_dim=64)
+    from tau_rs_b200.api import random_model
+    from tau_rs_b200.weights import write_random_model
+
+    folder = str(tmp_path / "model")
+    write_random_model(folder, config, seed=1, storage="bfloat16")
+    for load in (lambda: load_model(folder, "bfloat16", weights="fp8"), lambda: random_model(config, weights="fp8")):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        model = load()
+        peak = torch.cuda.max_memory_allocated() - before
+        wide = {name: 2 * spec.shape[0] * spec.shape[1] for name, spec in model.tensor_specs().items() if spec.role == "matrix"}
+        products = sum(size for name, size in wide.items() if "proj" in name)
+        assert products > 60e6 and peak < 0.75 * products + sum(wide.values()) - products, (peak, products)
+        del model

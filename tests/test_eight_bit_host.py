@@ -306,3 +306,32 @@ def test_attention_over_pages_as_they_are_held_refuses(change):
     with pytest.raises(kernels.KernelError):
         kernels.attention_decode8(operands["queries"], operands["key_pages"], operands["value_pages"], operands["key_scales"], operands["value_scales"], operands["out"], operands["step"],
                                   operands["page_rows"], operands["heads"], 2, 32, 1.0, operands["window"])
+
+
+def test_weights_are_brought_to_8_bits_as_the_tensors_arrive(monkeypatch):
+    """Tensor by tensor as a loader hands them over: a stack's pieces are gone with its last one, whatever the order inside it, biases are kept for the end."""
+    from tau_rs_b200 import DecoderModel
+    from tau_rs_b200.config.specs import with_weight_format
+    from tau_rs_b200.parts.linear import StackedLinear
+
+    quantised = []
+    monkeypatch.setattr(kernels, "quantize_blocks", lambda weight: quantised.append(weight.clone()) or (weight.to(CODES), torch.ones(1)))
+    model = DecoderModel(with_weight_format(tiny_spec("B"), "fp8"), torch.bfloat16, "cpu")      # with biases
+    stacks = [stack for block in model.blocks for stack in (block.mixer.qkv, block.mixer.out, block.feed_forward.gate_up, block.feed_forward.down)]
+    for index, (name, spec) in enumerate(model.tensor_specs().items()):
+        model.assign(name, torch.full(spec.shape, 1.0 + index % 50, dtype=torch.bfloat16 if spec.role == "matrix" else torch.float32))
+        waiting = [stack for stack in stacks if any(part.dim() == 2 for part in stack._parts.values())]
+        assert len(waiting) <= 1 and len(quantised) == sum(stack.codes is not None for stack in stacks)
+    assert len(quantised) == len(stacks)
+    model.finalize_weights()
+    assert len(quantised) == len(stacks) and all(stack.weight is None and not stack._parts for stack in stacks)
+    assert all((stack.bias is not None) == stack.has_bias for stack in stacks)
+    late = StackedLinear([("a", 16), ("b", 16)], 32, True, torch.bfloat16, "cpu", interleave=0, weight_format="fp8")
+    for name in ("b.bias", "b.weight", "a.bias", "a.weight"):
+        late.assign(name, torch.full((16, 32) if "weight" in name else (16,), 1.0 if name[0] == "a" else 2.0))
+    late.finalize_weights()
+    assert torch.equal(quantised[-1][:, 0], late.bias) and late.bias.tolist() == [1.0] * 16 + [2.0] * 16
+    with pytest.raises(KeyError):
+        lacking = StackedLinear([("a", 16), ("b", 16)], 32, False, torch.bfloat16, "cpu", weight_format="fp8")
+        lacking.assign("a.weight", torch.zeros(16, 32))
+        lacking.finalize_weights()
