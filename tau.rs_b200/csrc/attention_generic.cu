@@ -8,7 +8,7 @@
 //
 // Cache layout of one layer: keys[page][kv_head][slot_in_page][d], the same for values; position `p` of
 // sequence `s` lies in page `page_rows[s * page_stride + p / page_tokens]` at `p % page_tokens`.
-#include "common.cuh"
+#include "eight_bit.cuh"
 
 #include <type_traits>
 
@@ -179,10 +179,16 @@ __global__ void attention_prepare_vec_kernel(
 // One warp per (token, query head).  Keys are taken 32 at a time: lane `l` scores key `l` of the chunk
 // with a full dot product, the chunk's maximum and sum are found by shuffles, and the values are
 // accumulated with each lane owning elements `lane, lane + 32, ...` of the head.
+// `C` is how the cache holds an element: as T, or as an e4m3 code (uint8_t) with a 32-bit scale for each page and key/value head (the product of both is exact).
 template <typename T>
+__device__ __forceinline__ float cached_value(T value, float) { return to_float(value); }
+template <>
+__device__ __forceinline__ float cached_value<uint8_t>(uint8_t code, float scale) { return half_to_float(static_cast<unsigned short>(decode_half2(code))) * scale; }
+
+template <typename T, typename C>
 __global__ void attention_generic_kernel(
-    const T* __restrict__ queries, const T* __restrict__ keys, const T* __restrict__ values, T* __restrict__ out,
-    const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ page_rows,
+    const T* __restrict__ queries, const C* __restrict__ keys, const C* __restrict__ values, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
+    T* __restrict__ out, const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ page_rows,
     int page_stride, int page_tokens, int n_tokens, int n_heads, int n_kv_heads, int head_dim, float scale, int window) {
     grid_dependents_launch();
     grid_dependency_wait();
@@ -205,19 +211,22 @@ __global__ void attention_generic_kernel(
 #pragma unroll
     for (int i = 0; i < kMaxPerLane; ++i) acc[i] = 0.0f;
     const size_t head_stride = static_cast<size_t>(page_tokens) * head_dim;
+    constexpr bool kScaled = std::is_same<C, uint8_t>::value;
 
     for (int chunk = first_key; chunk <= position; chunk += 32) {
         const int key = chunk + lane;
         const bool live = key <= position;
         float score = -INFINITY;
         size_t offset = 0;
+        float value_scale = 1.0f;
         if (live) {
-            const int page = pages[key / page_tokens];
-            offset = (static_cast<size_t>(page) * n_kv_heads + kv_head) * head_stride +
-                     static_cast<size_t>(key % page_tokens) * head_dim;
-            const T* key_row = keys + offset;
+            const size_t place = static_cast<size_t>(pages[key / page_tokens]) * n_kv_heads + kv_head;
+            offset = place * head_stride + static_cast<size_t>(key % page_tokens) * head_dim;
+            const C* key_row = keys + offset;
+            const float key_scale = kScaled ? key_scales[place] : 1.0f;
+            if (kScaled) value_scale = value_scales[place];
             float dot = 0.0f;
-            for (int e = 0; e < head_dim; ++e) dot = fmaf(query[e], to_float(key_row[e]), dot);
+            for (int e = 0; e < head_dim; ++e) dot = fmaf(query[e], cached_value<C>(key_row[e], key_scale), dot);
             score = dot * scale;
         }
         const float chunk_max = warp_max(score);
@@ -232,11 +241,12 @@ __global__ void attention_generic_kernel(
         for (int j = 0; j < in_chunk; ++j) {
             const float w = __shfl_sync(0xffffffffu, weight, j);
             const size_t value_offset = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(offset), j);
-            const T* value_row = values + value_offset;
+            const float row_scale = kScaled ? __shfl_sync(0xffffffffu, value_scale, j) : 1.0f;
+            const C* value_row = values + value_offset;
 #pragma unroll
             for (int i = 0; i < kMaxPerLane; ++i) {
                 const int e = lane + 32 * i;
-                if (e < head_dim) acc[i] = fmaf(w, to_float(value_row[e]), acc[i]);
+                if (e < head_dim) acc[i] = fmaf(w, cached_value<C>(value_row[e], row_scale), acc[i]);
             }
         }
     }
@@ -442,17 +452,33 @@ TAU_EXPORT int tau_attention_generic(
     const unsigned blocks = static_cast<unsigned>((pairs + warps - 1) / warps);
     const size_t shared = warps * head_dim * sizeof(float);
     if (dtype == TAU_F32)
-        tau_launch(attention_generic_kernel<float>, dim3(blocks), dim3(warps * 32), shared, s, 
-            static_cast<const float*>(queries), static_cast<const float*>(keys), static_cast<const float*>(values),
+        tau_launch(attention_generic_kernel<float, float>, dim3(blocks), dim3(warps * 32), shared, s,
+            static_cast<const float*>(queries), static_cast<const float*>(keys), static_cast<const float*>(values), nullptr, nullptr,
             static_cast<float*>(out), positions, token_seq, page_rows, page_stride, page_tokens, n_tokens, n_heads,
             n_kv_heads, head_dim, scale, window);
     else if (dtype == TAU_BF16)
-        tau_launch(attention_generic_kernel<bf16>, dim3(blocks), dim3(warps * 32), shared, s, 
-            static_cast<const bf16*>(queries), static_cast<const bf16*>(keys), static_cast<const bf16*>(values),
+        tau_launch(attention_generic_kernel<bf16, bf16>, dim3(blocks), dim3(warps * 32), shared, s,
+            static_cast<const bf16*>(queries), static_cast<const bf16*>(keys), static_cast<const bf16*>(values), nullptr, nullptr,
             static_cast<bf16*>(out), positions, token_seq, page_rows, page_stride, page_tokens, n_tokens, n_heads,
             n_kv_heads, head_dim, scale, window);
     else
         return cudaErrorInvalidValue;
+    return tau_launch_status();
+}
+
+// The same of bfloat16 queries over pages of 64 positions held as e4m3 codes with scales [pages, n_kv_heads].
+TAU_EXPORT int tau_attention8_generic(const void* queries, const void* keys, const void* values, const float* key_scales, const float* value_scales, void* out, const int* positions,
+                                      const int* token_seq, const int* page_rows, int page_stride, int n_tokens, int n_heads, int n_kv_heads, int head_dim, float scale, int window, void* stream) {
+    if (n_tokens <= 0) return 0;
+    if (!queries || !keys || !values || !key_scales || !value_scales || !out || !positions || !token_seq || !page_rows || head_dim <= 0 || head_dim > 32 * kMaxPerLane || n_heads <= 0 ||
+        n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || window < 0)
+        return cudaErrorInvalidValue;
+    constexpr int warps = 4;
+    const long long blocks = (static_cast<long long>(n_tokens) * n_heads + warps - 1) / warps;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    tau_launch(attention_generic_kernel<bf16, uint8_t>, dim3(static_cast<unsigned>(blocks)), dim3(warps * 32), warps * head_dim * sizeof(float), static_cast<cudaStream_t>(stream),
+               static_cast<const bf16*>(queries), static_cast<const uint8_t*>(keys), static_cast<const uint8_t*>(values), key_scales, value_scales, static_cast<bf16*>(out), positions, token_seq,
+               page_rows, page_stride, 64, n_tokens, n_heads, n_kv_heads, head_dim, scale, window);
     return tau_launch_status();
 }
 

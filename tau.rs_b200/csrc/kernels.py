@@ -1426,17 +1426,29 @@ def _check_attention8(queries, key_pages, value_pages, key_scales, value_scales,
     _here(queries, out, key_pages, value_pages, key_scales, value_scales, page_rows, step.seq_start, step.seq_len, step.cu_seqlens)
 
 
+def _attention8_generic(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
+    """The plain kernel, which the others are checked against: it reads the pages as they are held and needs no workspace."""
+    for tensor in (step.positions, step.token_seq):
+        _require(tensor.dtype == torch.int32 and tensor.numel() == step.n_tokens and tensor.is_contiguous(), "a step's positions and sequences must be int32, one to a token")
+    _here(step.positions, step.token_seq)
+    run = _function("attention_generic.cu", "tau_attention8_generic", "pppppppppiiiiifi")
+    _check(run(queries.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), out.data_ptr(), step.positions.data_ptr(),
+               step.token_seq.data_ptr(), page_rows.data_ptr(), page_rows.shape[1], step.n_tokens, n_heads, n_kv_heads, head_dim, scale, window, _stream_handle()), "attention")
+
+
 def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
     """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
     _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, window)
     if step.n_tokens == 0:
         return
-    if _prefer_optimized and (step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim))):
+    if not _prefer_optimized:
+        return _attention8_generic(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
+    if step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim)):
         return _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
-    # Every sequence has room for the longest, so they are taken a few at a time where that would be much (the plain kernel goes by the step's own numbers and takes all at once).
+    # Every sequence has room for the longest, so they are taken a few at a time where that would be much.
     sequences, stride = page_rows.shape
-    at_once = sequences if not _prefer_optimized else max(1, READ8_BYTES // (4 * stride * PAGE_TOKENS * n_kv_heads * head_dim))
+    at_once = max(1, READ8_BYTES // (4 * stride * PAGE_TOKENS * n_kv_heads * head_dim))
     for first in range(0, sequences, at_once):
         last = min(first + at_once, sequences)
         part = step if at_once >= sequences else replace(step, n_seqs=last - first, cu_seqlens=step.cu_seqlens[first : last + 1], seq_start=step.seq_start[first:last], seq_len=step.seq_len[first:last])

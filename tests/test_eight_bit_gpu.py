@@ -496,3 +496,45 @@ def test_attention_of_a_captured_step():
         kernels.attention8(queries, *cache.pages, again, step, *arguments)
         torch.cuda.synchronize()
         assert torch.equal(out, again)
+
+
+@pytest.fixture
+def plain_kernels():
+    kernels.prefer_optimized(False)
+    yield
+    kernels.prefer_optimized(True)
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, window", [(1, 1, 16, 0), (6, 2, 80, 90), (8, 2, 64, 1), (20, 1, 128, 0), (4, 2, 256, 70)])
+def test_the_plain_kernel(plain_kernels, heads, kv_heads, dim, window):
+    """Single tokens and runs against the statement, and bit for bit what the plain kernel of a 16-bit cache makes of the pages read back."""
+    check_attention([(length - 1, 1) for length in (1, 64, 65, 300)], heads, kv_heads, dim, window)
+    check_attention([(0, 70), (100, 1), (60, 9), (0, 1)], heads, kv_heads, dim, window)
+    cache, runs = Cache(9, kv_heads, dim, [3, 2, 4]), [(120, 40), (0, 70), (199, 1)]
+    cache.store([(0, 160), (0, 70), (0, 200)], *random_rows(430, kv_heads, dim, 5))
+    queries = torch.randn(111, heads * dim, device="cuda").to(torch.bfloat16)
+    found, wanted = torch.empty_like(queries), torch.empty_like(queries)
+    step = make_step(runs)
+    kernels.attention8(queries, *cache.pages, found, step, cache.rows, heads, kv_heads, dim, dim ** -0.5, window)
+    keys, values = kernels.cache8_read(*cache.pages, step, cache.rows)
+    places = torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4)
+    kernels.attention_generic(queries, keys, values, wanted, step.positions, step.token_seq, places, heads, kv_heads, dim, dim ** -0.5, window)
+    assert torch.equal(found, wanted)
+
+
+def test_the_plain_kernel_needs_no_workspace(plain_kernels):
+    """A captured step lists as many pages as a sequence may ever have: memory goes by none of them (laid out in 16 bits these would take 671 MB)."""
+    cache = Cache(40, 2, 64, [1] * 40)
+    cache.store([(0, 30)] * 40, *random_rows(1200, 2, 64, 5))
+    rows = torch.zeros(40, 512, dtype=torch.int32, device="cuda")
+    rows[:, :1] = cache.rows
+    queries = torch.randn(40, 8 * 64, device="cuda").to(torch.bfloat16)
+    out, wanted = torch.empty_like(queries), torch.empty_like(queries)
+    step = make_step([(29, 1)] * 40)
+    kernels.attention8(queries, *cache.pages, wanted, step, cache.rows, 8, 2, 64, 0.125, 0)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    kernels.attention8(queries, *cache.pages, out, step, rows, 8, 2, 64, 0.125, 0)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert torch.equal(out, wanted)
