@@ -323,22 +323,25 @@ constexpr int kReadHeads = 16;      // at most so many heads to a block
 __device__ __forceinline__ unsigned nan_codes(unsigned word) { return __vcmpeq4(word & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
 // Pages of the step's sequences as the bfloat16 values that they stand for (exact: 4 significant bits times a power of two).
-// grid (page of a sequence, sequence, groups of `heads` heads).  Positions that a sequence does not have are zeros; with `sparse` only pages that a query sees
-// are written at all (and `places` gets the numbers that the pages have in the result), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of
+// grid (`span` pages of a sequence, sequence, groups of `heads` heads), from the first page of a sequence on or, with `sparse`, from the first that a query sees.  Positions that a sequence does
+// not have are zeros; with `sparse` only pages that a query sees are written at all (and `places` gets the numbers that the pages have in the result; those of other pages are numbers that it has
+// too), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of
 // zero would not hide that.  Bound by memory: a page's heads lie one behind the other, so where there are pages enough a block takes several and pays for its page's number and
 // scale once (64 sequences of up to 200 positions, 8 heads of 128: 14 us for 17 MB of codes read and 34 MB of values written).
 __global__ void __launch_bounds__(256)
 read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
             bf16* __restrict__ keys, bf16* __restrict__ values, int* __restrict__ places, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
-            int page_stride, int n_kv_heads, int heads, int D, int window, int sparse) {
+            int page_stride, int span, int n_kv_heads, int heads, int D, int window, int sparse) {
     __shared__ unsigned char odd[kReadHeads * kPage];      // positions with a value that is not finite
     grid_dependents_launch();
     grid_dependency_wait();
-    const int page = blockIdx.x, seq = blockIdx.y, head0 = blockIdx.z * heads, here = min(heads, n_kv_heads - head0);
-    if (places != nullptr && blockIdx.z == 0 && threadIdx.x == 0) places[static_cast<size_t>(seq) * page_stride + page] = seq * page_stride + page;
+    const int seq = blockIdx.y, head0 = blockIdx.z * heads, here = min(heads, n_kv_heads - head0);
+    const int first_seen = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) : 0, first_page = first_seen / kPage, page = first_page + blockIdx.x;
+    if (places != nullptr && blockIdx.x == 0 && blockIdx.z == 0)
+        for (int p = threadIdx.x; p < page_stride; p += 256) places[static_cast<size_t>(seq) * page_stride + p] = seq * span + min(max(p - first_page, 0), span - 1);
     const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
-    const int first = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) - page * kPage : 0;      // the first position of this page that a query sees
-    if (sparse && (live <= 0 || first >= kPage)) return;
+    const int first = max(0, first_seen - page * kPage);      // the first position of this page that a query sees
+    if (sparse && live <= 0) return;
     const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * n_kv_heads + head0 : 0;
     const int per_head = kPage * D / 16, begin = first * D / 16, end = live * D / 16;      // pieces of 16 elements
     // For attention (`sparse`), where some queries see a position and others do not: a value that is not finite would reach those that do not, through a weight of zero.  It becomes zero
@@ -353,7 +356,7 @@ read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ v
     for (int pass = 0; pass < 2; ++pass) {      // values, then keys
         const uint4* codes = reinterpret_cast<const uint4*>((pass == 0 ? value_pages : key_pages) + place * kPage * D);
         const float* scales = (pass == 0 ? value_scales : key_scales) + place;
-        uint4* target = reinterpret_cast<uint4*>((pass == 0 ? values : keys) + ((static_cast<size_t>(seq) * page_stride + page) * n_kv_heads + head0) * kPage * D);
+        uint4* target = reinterpret_cast<uint4*>((pass == 0 ? values : keys) + ((static_cast<size_t>(seq) * span + blockIdx.x) * n_kv_heads + head0) * kPage * D);
         for (int base = threadIdx.x; base < here * per_head; base += 256 * kAhead) {
             uint4 raw[kAhead];
             float scale[kAhead];
@@ -473,18 +476,19 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
     return tau_launch_status();
 }
 
+// `span`: pages laid out for each sequence: all that the page rows list, or, with `sparse` and a window, as many as the queries of its run can see.
 TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* keys, void* values, int* places, const int* seq_start,
-                               const int* seq_len, const int* page_rows, int page_stride, int n_seqs, int n_kv_heads, int D, int window, int sparse, void* stream) {
+                               const int* seq_len, const int* page_rows, int page_stride, int span, int n_seqs, int n_kv_heads, int D, int window, int sparse, void* stream) {
     if (n_seqs <= 0) return 0;
     if (!key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len ||
-        !page_rows || page_stride <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
+        !page_rows || page_stride <= 0 || span <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || n_kv_heads > 65535)
         return cudaErrorInvalidValue;
-    const long long blocks = static_cast<long long>(n_kv_heads) * n_seqs * page_stride, wanted = 148 * 8;      // one head to a block as long as all fit the machine at once
+    const long long blocks = static_cast<long long>(n_kv_heads) * n_seqs * span, wanted = 148 * 8;      // one head to a block as long as all fit the machine at once
     const int most = n_kv_heads < kReadHeads ? n_kv_heads : kReadHeads;
     const int heads = blocks <= wanted ? 1 : static_cast<int>(blocks / wanted < most ? blocks / wanted : most);
-    tau_launch(read_kernel, dim3(page_stride, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
-               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, n_kv_heads, heads, D,
+    tau_launch(read_kernel, dim3(span, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
+               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, span, n_kv_heads, heads, D,
                window, sparse);
     return tau_launch_status();
 }

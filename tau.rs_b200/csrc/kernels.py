@@ -1284,16 +1284,16 @@ def attention8_queries(projected, queries, q_weight, eps: float, cos, sin, rotar
     attention_prepare(projected, queries, nothing, nothing, False, q_weight, None, eps, cos, sin, rotary_dim, step.positions, step.token_seq, places, n_heads, 1, head_dim)
 
 
-def _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, window: int, sparse: bool):
+def _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, span: int, window: int, sparse: bool):
     sequences, stride = page_rows.shape
     n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
     _require(sequences <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
-    pages = torch.empty((2, sequences * stride, n_kv_heads, PAGE_TOKENS, head_dim), dtype=torch.bfloat16, device=key_pages.device)
+    pages = torch.empty((2, sequences * span, n_kv_heads, PAGE_TOKENS, head_dim), dtype=torch.bfloat16, device=key_pages.device)
     places = torch.empty((sequences, stride), dtype=torch.int32, device=key_pages.device) if sparse else None
-    run = _function("eight_bit.cu", "tau_cache8_read", "ppppppppppiiiiii")
+    run = _function("eight_bit.cu", "tau_cache8_read", "ppppppppppiiiiiii")
     keys, values = pages.unbind()
     _check(run(key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(places), step.seq_start.data_ptr(),
-               step.seq_len.data_ptr(), page_rows.data_ptr(), stride, sequences, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
+               step.seq_len.data_ptr(), page_rows.data_ptr(), stride, span, sequences, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
     return keys, values, places
 
 
@@ -1302,7 +1302,7 @@ def cache8_read(key_pages, value_pages, key_scales, value_scales, step, page_row
     sequence `i` at `i * stride + j`; zeros where a sequence has no position."""
     _check_pages8(key_pages, value_pages, key_scales, value_scales, step, page_rows)
     _here(key_pages, value_pages, key_scales, value_scales, step.seq_start, step.seq_len, page_rows)
-    return _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, 0, False)[:2]
+    return _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, page_rows.shape[1], 0, False)[:2]
 
 
 def decode8_splits(n_seqs: int, max_len: int, kv_blocks: int, sms: Optional[int] = None) -> int:
@@ -1446,13 +1446,15 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     if step.all_single or (step.n_tokens <= 65535 and runs8_like_single_tokens(step.n_seqs, step.max_new, step.max_len, n_heads, n_kv_heads, head_dim)):
         return _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, scale, window)
     # Runs: the pages that the step's queries see are laid out in bfloat16, one sequence behind the other (and the numbers that they then have), and the kernels of a 16-bit cache take it from there.
-    # Every sequence has room for the longest, so they are taken a few at a time where that would be much.
-    sequences, stride = page_rows.shape
-    at_once = max(1, READ8_BYTES // (4 * stride * PAGE_TOKENS * n_kv_heads * head_dim))
+    # Every sequence has room for the longest, or for what the longest run sees through a window, so they are taken a few at a time where that would be much.
+    sequences, span = page_rows.shape
+    if window:
+        span = min(span, (window + step.max_new + PAGE_TOKENS - 3) // PAGE_TOKENS + 1)      # window + max_new - 1 positions, wherever they begin
+    at_once = max(1, READ8_BYTES // (4 * span * PAGE_TOKENS * n_kv_heads * head_dim))
     for first in range(0, sequences, at_once):
         last = min(first + at_once, sequences)
         part = step if at_once >= sequences else replace(step, n_seqs=last - first, cu_seqlens=step.cu_seqlens[first : last + 1], seq_start=step.seq_start[first:last], seq_len=step.seq_len[first:last])
-        keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, part, page_rows[first:last], window, True)
+        keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, part, page_rows[first:last], span, window, True)
         attention(queries, keys, values, out, part, places, n_heads, n_kv_heads, head_dim, scale, window)
 
 

@@ -538,3 +538,22 @@ def test_the_plain_kernel_needs_no_workspace(plain_kernels):
     kernels.attention8(queries, *cache.pages, out, step, rows, 8, 2, 64, 0.125, 0)
     assert torch.cuda.max_memory_allocated() - before < 1 << 20
     assert torch.equal(out, wanted)
+
+
+@pytest.mark.parametrize("dim", [32, 128])
+def test_runs_behind_a_window_lay_out_the_pages_that_they_see(monkeypatch, dim):
+    """A window of 100 and runs of up to 60 tokens see four pages wherever they begin, of the 63 that the longest sequence has: the workspace goes by the four."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: False)
+    for window in (1, 63, 64, 65, 100):
+        check_attention([(3950, 60), (0, 2), (129, 60), (64, 3), (3903, 60), (99, 1)], 4, 2, dim, window)
+    cache, runs = Cache(63, 2, dim, [63]), [(3950, 60)]
+    cache.store([(0, 4010)], *random_rows(4010, 2, dim, 5))
+    queries = torch.randn(60, 4 * dim, device="cuda").to(torch.bfloat16)
+    out, step = torch.empty_like(queries), make_step(runs)
+    arguments = (queries, *cache.pages, out, step, cache.rows, 4, 2, dim, dim ** -0.5, 100)
+    kernels.attention8(*arguments)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    kernels.attention8(*arguments)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * 4 * 2 * 64 * dim * 2 + 4096      # and the table of their places
