@@ -331,7 +331,7 @@ __device__ __forceinline__ unsigned nan_codes(unsigned word) { return __vcmpeq4(
 __global__ void __launch_bounds__(256)
 read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
             bf16* __restrict__ keys, bf16* __restrict__ values, int* __restrict__ places, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
-            int page_stride, int span, int n_kv_heads, int heads, int D, int window, int sparse) {
+            int page_stride, int span, int page_heads, int n_kv_heads, int heads, int D, int window, int sparse) {
     __shared__ unsigned char odd[kReadHeads * kPage];      // positions with a value that is not finite
     grid_dependents_launch();
     grid_dependency_wait();
@@ -342,7 +342,7 @@ read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ v
     const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
     const int first = max(0, first_seen - page * kPage);      // the first position of this page that a query sees
     if (sparse && live <= 0) return;
-    const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * n_kv_heads + head0 : 0;
+    const size_t place = live > 0 ? static_cast<size_t>(page_rows[static_cast<size_t>(seq) * page_stride + page]) * page_heads + head0 : 0;
     const int per_head = kPage * D / 16, begin = first * D / 16, end = live * D / 16;      // pieces of 16 elements
     // For attention (`sparse`), where some queries see a position and others do not: a value that is not finite would reach those that do not, through a weight of zero.  It becomes zero
     // and its position's key NaN, which a mask does hide.
@@ -476,19 +476,22 @@ TAU_EXPORT int tau_cache8_store(const void* keys, long long key_stride, const vo
     return tau_launch_status();
 }
 
-// `span`: pages laid out for each sequence: all that the page rows list, or, with `sparse` and a window, as many as the queries of its run can see.
+// `span`: pages laid out for each sequence: all that the page rows list, or, with `sparse` and a window, as many as the queries of its run can see.  `n_kv_heads` heads from `first_head` on are read
+// of pages of `page_heads`.
 TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, const float* key_scales, const float* value_scales, void* keys, void* values, int* places, const int* seq_start,
-                               const int* seq_len, const int* page_rows, int page_stride, int span, int n_seqs, int n_kv_heads, int D, int window, int sparse, void* stream) {
+                               const int* seq_len, const int* page_rows, int page_stride, int span, int n_seqs, int page_heads, int first_head, int n_kv_heads, int D, int window, int sparse, void* stream) {
     if (n_seqs <= 0) return 0;
     if (!key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len ||
-        !page_rows || page_stride <= 0 || span <= 0 || n_kv_heads <= 0 || D < 16 || D > 256 ||
+        !page_rows || page_stride <= 0 || span <= 0 || n_kv_heads <= 0 || first_head < 0 || first_head + n_kv_heads > page_heads || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || n_kv_heads > 65535)
         return cudaErrorInvalidValue;
     const long long blocks = static_cast<long long>(n_kv_heads) * n_seqs * span, wanted = 148 * 8;      // one head to a block as long as all fit the machine at once
     const int most = n_kv_heads < kReadHeads ? n_kv_heads : kReadHeads;
     const int heads = blocks <= wanted ? 1 : static_cast<int>(blocks / wanted < most ? blocks / wanted : most);
-    tau_launch(read_kernel, dim3(span, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages),
-               static_cast<const uint8_t*>(value_pages), key_scales, value_scales, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len, page_rows, page_stride, span, n_kv_heads, heads, D,
+    const size_t before = static_cast<size_t>(first_head) * kPage * D;
+    tau_launch(read_kernel, dim3(span, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages) + before,
+               static_cast<const uint8_t*>(value_pages) + before, key_scales + first_head, value_scales + first_head, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len,
+               page_rows, page_stride, span, page_heads, n_kv_heads, heads, D,
                window, sparse);
     return tau_launch_status();
 }

@@ -1284,16 +1284,17 @@ def attention8_queries(projected, queries, q_weight, eps: float, cos, sin, rotar
     attention_prepare(projected, queries, nothing, nothing, False, q_weight, None, eps, cos, sin, rotary_dim, step.positions, step.token_seq, places, n_heads, 1, head_dim)
 
 
-def _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, span: int, window: int, sparse: bool):
+def _read8(key_pages, value_pages, key_scales, value_scales, step, page_rows, span: int, window: int, sparse: bool, first_head: int = 0, heads: Optional[int] = None):
     sequences, stride = page_rows.shape
-    n_kv_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
-    _require(sequences <= 65535 and 2 * n_kv_heads <= 65535, "at most 65,535 sequences are read back at once")
-    pages = torch.empty((2, sequences * span, n_kv_heads, PAGE_TOKENS, head_dim), dtype=torch.bfloat16, device=key_pages.device)
+    page_heads, head_dim = key_pages.shape[1], key_pages.shape[3]
+    heads = page_heads if heads is None else heads
+    _require(sequences <= 65535 and 2 * page_heads <= 65535, "at most 65,535 sequences are read back at once")
+    pages = torch.empty((2, sequences * span, heads, PAGE_TOKENS, head_dim), dtype=torch.bfloat16, device=key_pages.device)
     places = torch.empty((sequences, stride), dtype=torch.int32, device=key_pages.device) if sparse else None
-    run = _function("eight_bit.cu", "tau_cache8_read", "ppppppppppiiiiiii")
+    run = _function("eight_bit.cu", "tau_cache8_read", "ppppppppppiiiiiiiii")
     keys, values = pages.unbind()
     _check(run(key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(), values.data_ptr(), _address(places), step.seq_start.data_ptr(),
-               step.seq_len.data_ptr(), page_rows.data_ptr(), stride, span, sequences, n_kv_heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
+               step.seq_len.data_ptr(), page_rows.data_ptr(), stride, span, sequences, page_heads, first_head, heads, head_dim, window, 1 if sparse else 0, _stream_handle()), "cache8_read")
     return keys, values, places
 
 
@@ -1411,7 +1412,7 @@ _decode8_functions = {}
 DECODE8_CLUSTERED = 8      # up to so many ranges of a sequence meet in a cluster's shared memory
 
 
-READ8_BYTES = 1 << 30      # of pages read back at once
+READ8_BYTES = 1 << 30      # of pages read back at once; a sequence of which one head alone takes more (2,097,152 positions of 128 elements) takes what that head does
 
 
 def _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, window: int) -> None:
@@ -1450,12 +1451,23 @@ def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, s
     sequences, span = page_rows.shape
     if window:
         span = min(span, (window + step.max_new + PAGE_TOKENS - 3) // PAGE_TOKENS + 1)      # window + max_new - 1 positions, wherever they begin
-    at_once = max(1, READ8_BYTES // (4 * span * PAGE_TOKENS * n_kv_heads * head_dim))
-    for first in range(0, sequences, at_once):
-        last = min(first + at_once, sequences)
-        part = step if at_once >= sequences else replace(step, n_seqs=last - first, cu_seqlens=step.cu_seqlens[first : last + 1], seq_start=step.seq_start[first:last], seq_len=step.seq_len[first:last])
-        keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, part, page_rows[first:last], span, window, True)
-        attention(queries, keys, values, out, part, places, n_heads, n_kv_heads, head_dim, scale, window)
+    a_head = 4 * span * PAGE_TOKENS * head_dim      # bytes of a sequence's keys and values of one head
+    at_once = max(1, READ8_BYTES // (n_kv_heads * a_head))
+    # ... and of one sequence so many heads at a time: more than 262,144 positions of 8 heads of 128, say.  Their queries and results are then columns apart, which the kernels below do not read.
+    heads = n_kv_heads if at_once > 1 else max(1, min(n_kv_heads, READ8_BYTES // a_head))
+    group = n_heads // n_kv_heads
+    for first_head in range(0, n_kv_heads, heads):
+        here = min(heads, n_kv_heads - first_head)
+        columns = slice(first_head * group * head_dim, (first_head + here) * group * head_dim)
+        some_queries, some_out = (queries, out) if here == n_kv_heads else (queries[:, columns].contiguous(), out[:, columns].contiguous())
+        for first in range(0, sequences, at_once):
+            last = min(first + at_once, sequences)
+            part = step if at_once >= sequences else replace(step, n_seqs=last - first, cu_seqlens=step.cu_seqlens[first : last + 1], seq_start=step.seq_start[first:last], seq_len=step.seq_len[first:last])
+            keys, values, places = _read8(key_pages, value_pages, key_scales, value_scales, part, page_rows[first:last], span, window, True, first_head, here)
+            attention(some_queries, keys, values, some_out, part, places, here * group, here, head_dim, scale, window)
+            del keys, values, places      # before the next ones are asked for
+        if here != n_kv_heads:
+            out[:, columns] = some_out
 
 
 # ---------------------------------------------------------------------------- latent attention

@@ -557,3 +557,25 @@ def test_runs_behind_a_window_lay_out_the_pages_that_they_see(monkeypatch, dim):
     torch.cuda.reset_peak_memory_stats()
     kernels.attention8(*arguments)
     assert torch.cuda.max_memory_allocated() - before <= 2 * 4 * 2 * 64 * dim * 2 + 4096      # and the table of their places
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, at_once", [(6, 3, 48, 2), (8, 4, 64, 3), (3, 3, 128, 1), (8, 2, 256, 1)])
+def test_runs_whose_pages_are_read_back_a_few_heads_at_a_time(monkeypatch, heads, kv_heads, dim, at_once):
+    """Less room than one sequence takes: heads are read a few at a time, results are the same bit for bit, and memory stays within the room."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: False)
+    cache, runs = Cache(40, kv_heads, dim, [33, 5]), [(2000, 90), (255, 65)]
+    cache.store([(0, 2090), (0, 320)], *random_rows(2410, kv_heads, dim, 5))
+    queries = torch.randn(155, heads * dim, device="cuda").to(torch.bfloat16)
+    out, wanted, step = torch.full_like(queries, 7.0), torch.full_like(queries, 7.0), make_step(runs)
+    for window in (0, 100):
+        kernels.attention8(queries, *cache.pages, wanted, step, cache.rows, heads, kv_heads, dim, dim ** -0.5, window)
+        torch.cuda.synchronize()
+        span = 33 if window == 0 else 4      # 189 positions, wherever they begin
+        room = at_once * span * 4 * 64 * dim
+        with monkeypatch.context() as patch:
+            patch.setattr(kernels, "READ8_BYTES", room)
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            kernels.attention8(queries, *cache.pages, out, step, cache.rows, heads, kv_heads, dim, dim ** -0.5, window)
+            assert torch.cuda.max_memory_allocated() - before <= room + 2 * queries.numel() * 2 + 8192
+        assert torch.equal(out, wanted)
