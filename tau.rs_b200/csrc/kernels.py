@@ -1329,6 +1329,11 @@ def _passes8(columns: int, head_dim: int) -> int:
     return -(-columns // (16 if columns > 8 and head_dim <= 128 else 8))
 
 
+def attention8_decode_splits(n_seqs: int, max_len: int, n_heads: int, n_kv_heads: int, head_dim: int, window: int, new: int = 1) -> int:
+    """`decode8_splits` for a layer's heads and window, `new` tokens to a sequence."""
+    return decode8_splits(n_seqs, min(max_len, window) if window else max_len, n_kv_heads * _passes8(n_heads // n_kv_heads * new, head_dim))
+
+
 def attention_decode8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
     """`attention8` by the kernel that reads pages as they are held, whatever the step: one query token per sequence over its `seq_len` cached positions, or a few."""
     _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, window)
@@ -1340,8 +1345,7 @@ def _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, ste
     """The launch; its arguments are checked.  `prepare`: see `attention8_decode_fused`; `queries` is then None."""
     n_seqs, n_tokens = step.n_seqs, step.n_tokens
     single = step.all_single
-    passes = _passes8(n_heads // n_kv_heads * (1 if single else step.max_new), head_dim)
-    splits = (step.decode_splits if single else 0) or decode8_splits(n_seqs, min(step.max_len, window) if window else step.max_len, n_kv_heads * passes)
+    splits = (step.decode_splits if single else 0) or attention8_decode_splits(n_seqs, step.max_len, n_heads, n_kv_heads, head_dim, window, 1 if single else step.max_new)
     splits = min(splits, window // PAGE_TOKENS + 2 if window and single else 256, 256)      # a window lies in so many pages
     scratch = torch.empty(n_tokens * n_heads * splits * (head_dim + 2), dtype=torch.float32, device=out.device) if splits > DECODE8_CLUSTERED else None
     run = _decode8_functions.get(head_dim)

@@ -65,6 +65,9 @@ class Attention(Mixer):
         heads_per_pass = 8 if group >= 8 else 4 if group > 2 else group
         return self.spec.n_kv_heads * -(-group // heads_per_pass)
 
+    def decode_splits8(self, n_seqs: int, max_len: int) -> int:
+        return kernels.attention8_decode_splits(n_seqs, max_len, self.spec.n_heads, self.spec.n_kv_heads, self.spec.head_dim, self.spec.window or 0)
+
     def tensor_specs(self):
         specs = {}
         for part in self._children:

@@ -116,6 +116,11 @@ class Mixer(Part):
         are resident at once, and it is part of a captured graph's key."""
         return None
 
+    def decode_splits8(self, n_seqs: int, max_len: int) -> Optional[int]:
+        """How many ranges a decode step of `n_seqs` sequences, the longest of `max_len` positions, is best cut into over a cache held in 8 bits, where the mixer works on such a cache (None: it does
+        not).  The same for all lengths with the next power of two in common, as captured graphs are keyed."""
+        return None
+
     def extra_cache_needs(self) -> Dict[str, CacheNeed]:
         """What the mixer keeps for a sequence beside `cache_need()`, by role (the tail of inputs of a convolution, say); `forward`
         finds the views under `cache.extra[role]`.  The block hands the roles on (`Block.extra_cache_needs`)."""
@@ -164,6 +169,10 @@ class Block(Part):
 
     def decode_blocks(self) -> Optional[int]:
         """The mixer's answer (see `Mixer.decode_blocks`)."""
+        return None
+
+    def decode_splits8(self, n_seqs: int, max_len: int) -> Optional[int]:
+        """The mixer's answer (see `Mixer.decode_splits8`)."""
         return None
 
     def extra_cache_needs(self) -> Dict[str, CacheNeed]:

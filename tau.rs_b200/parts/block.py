@@ -51,6 +51,9 @@ class PreNormBlock(Block):
     def decode_blocks(self):
         return self.mixer.decode_blocks()
 
+    def decode_splits8(self, n_seqs: int, max_len: int):
+        return self.mixer.decode_splits8(n_seqs, max_len)
+
     def tensor_specs(self):
         specs = {}
         for part in self._children:
@@ -161,6 +164,7 @@ class ParallelBlock(Block):
 
     cache_need = PreNormBlock.cache_need
     decode_blocks = PreNormBlock.decode_blocks
+    decode_splits8 = PreNormBlock.decode_splits8
     tensor_specs = PreNormBlock.tensor_specs
     assign = PreNormBlock.assign
     finalize_weights = PreNormBlock.finalize_weights
@@ -245,6 +249,7 @@ class SublayerNormBlock(Block):
 
     cache_need = PreNormBlock.cache_need
     decode_blocks = PreNormBlock.decode_blocks
+    decode_splits8 = PreNormBlock.decode_splits8
 
     def extra_cache_needs(self):
         from .base import CacheNeed
@@ -389,6 +394,7 @@ class SandwichBlock(Block):
 
     cache_need = PreNormBlock.cache_need
     decode_blocks = PreNormBlock.decode_blocks
+    decode_splits8 = PreNormBlock.decode_splits8
     tensor_specs = SublayerNormBlock.tensor_specs
     assign = SublayerNormBlock.assign
 

@@ -138,10 +138,12 @@ class DecoderModel:
         return total + self.spec.vocab_size * self.spec.hidden * torch.empty((), dtype=self.dtype).element_size()
 
     def decode_splits(self, n_seqs: int, max_len: int, eight_bit: bool = False) -> int:
-        """Context splits for a decode step of `n_seqs` sequences (part of a captured graph's key), over a cache in the run's dtype or in 8 bits."""
+        """Context splits for a decode step of `n_seqs` sequences (part of a captured graph's key), over a cache in the run's dtype or in 8 bits: as many as the layer wants that wants
+        most of them."""
+        if eight_bit:
+            return max((wanted for wanted in (block.decode_splits8(n_seqs, max_len) for block in self.blocks) if wanted), default=1)
         blocks = [count for count in (block.decode_blocks() for block in self.blocks) if count]
-        rule = kernels.decode8_splits if eight_bit else kernels.decode_splits
-        return rule(n_seqs, max_len, min(blocks)) if blocks else 1
+        return kernels.decode_splits(n_seqs, max_len, min(blocks)) if blocks else 1
 
     # ---- forward -----------------------------------------------------------------
     def forward(self, step, cache) -> Optional[torch.Tensor]:

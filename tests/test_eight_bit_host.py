@@ -335,3 +335,36 @@ def test_weights_are_brought_to_8_bits_as_the_tensors_arrive(monkeypatch):
         lacking = StackedLinear([("a", 16), ("b", 16)], 32, False, torch.bfloat16, "cpu", weight_format="fp8")
         lacking.assign("a.weight", torch.zeros(16, 32))
         lacking.finalize_weights()
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, window", [(8, 8, 128, None), (32, 8, 128, None), (40, 8, 128, None), (28, 4, 128, None), (64, 4, 128, None), (64, 8, 64, None), (20, 1, 128, None), (16, 1, 256, None),
+                                                          (24, 8, 96, None), (32, 8, 128, 1000), (40, 8, 64, 128)])
+def test_an_engine_asks_for_the_ranges_that_a_call_by_itself_takes(heads, kv_heads, dim, window):
+    """One answer for every length with the same next power of two, with a window as without: a captured step serves all of them."""
+    from dataclasses import replace
+
+    from tau_rs_b200 import DecoderModel
+
+    spec = tiny_spec("B")
+    spec = replace(spec, blocks=tuple(replace(block, mixer=replace(block.mixer, n_heads=heads, n_kv_heads=kv_heads, head_dim=dim, window=window, qk_norm=None, position=None)) for block in spec.blocks))
+    model = DecoderModel(spec, torch.bfloat16, "cpu")
+    passes = -(-(heads // kv_heads) // (16 if heads // kv_heads > 8 and dim <= 128 else 8))
+    for n_seqs, length in [(1, 300), (4, 1000), (8, 2048), (8, 16000), (2, 120000), (40, 6000), (1, 64)]:
+        wanted = kernels.decode8_splits(n_seqs, min(length, window) if window else length, kv_heads * passes)
+        assert model.decode_splits(n_seqs, length, eight_bit=True) == wanted
+        bucket = 1 << (length - 1).bit_length()
+        assert all(model.decode_splits(n_seqs, other, eight_bit=True) == wanted for other in (bucket // 2 + 1, bucket))
+    if (heads, kv_heads) == (40, 8) and not window:      # once half as many, from the blocks of the 16-bit kernel
+        assert [model.decode_splits(n, length, eight_bit=True) for n, length in ((2, 120000), (8, 2048), (4, 1000), (8, 16000))] == [37, 4, 4, 8]
+
+
+def test_a_model_of_several_windows_takes_the_ranges_of_the_layer_that_wants_most():
+    from dataclasses import replace
+
+    from tau_rs_b200 import DecoderModel
+
+    spec = tiny_spec("B")
+    blocks = [replace(block, mixer=replace(block.mixer, window=window)) for block, window in zip(spec.blocks, (64, None, 200))]
+    schedule = [replace(entry, cache_group=f"g{index}", cache_layer=0) for index, entry in enumerate(spec.schedule)]
+    model = DecoderModel(replace(spec, blocks=tuple(blocks), schedule=tuple(schedule)), torch.bfloat16, "cpu")
+    assert model.decode_splits(1, 5000, eight_bit=True) == kernels.decode8_splits(1, 5000, 1) > kernels.decode8_splits(1, 200, 1)
