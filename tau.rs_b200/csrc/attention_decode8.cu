@@ -750,6 +750,17 @@ int page_map(CUtensorMap* map, const void* pages, long long boxes) {
 template <int Groups>
 constexpr int shared_bytes() { return static_cast<int>(sizeof(Shared)) + 1024 + kStagesOf<Groups> * kStageBytes; }
 
+// Multiprocessors of the current device, asked for once.
+int multiprocessors() {
+    static int counts[64] = {};
+    int device = 0, count = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 1;
+    if (device < 64 && counts[device]) return counts[device];
+    if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || count < 1) return 1;
+    if (device < 64) counts[device] = count;
+    return count;
+}
+
 struct Call {
     const bf16* queries;
     bf16* out;
@@ -778,7 +789,7 @@ int launch_groups(const CUtensorMap& key_map, const CUtensorMap& value_map, cons
     // Long sequences start first, so that the SMs share them out and short ones fill what is left at the end, up to three times as many blocks as there are places: 40 of 64 to 6,000
     // positions 74 -> 59 us, 64 of up to 2,048 46 -> 36, 200 of up to 1,000 58 -> 52, 8 of 2,048 no slower; beyond that putting them in order costs a block more than it gives
     // (256 of up to 300: 36 -> 38).
-    const long long places = 148ll * (NT == 1 && kHalves == 1 && !Runs && Groups == 1 ? 4 : 2), blocks = static_cast<long long>(grid.x) * grid.y * grid.z;
+    const long long places = static_cast<long long>(multiprocessors()) * (NT == 1 && kHalves == 1 && !Runs && Groups == 1 ? 4 : 2), blocks = static_cast<long long>(grid.x) * grid.y * grid.z;
     const int longest_first = !Runs && c.n_seqs > 1 && c.n_seqs <= kMostOrdered && blocks <= 3 * places;
     // Beside the kernel before it only where all blocks find room at once (8 sequences of 2,048 positions 14.4 -> 13.9 us; 640 blocks of 40 sequences 73 -> 78).
     const bool early = blocks <= places;
@@ -801,7 +812,7 @@ int launch(const CUtensorMap& key_map, const CUtensorMap& value_map, const Call&
     // eight 0.608 and 0.646).
     if constexpr (NT == 1 && kHalves == 1 && !Runs) {
         const bool crowded = c.splits > 4 && c.splits <= kMostClustered;
-        if (static_cast<long long>(c.splits) * c.n_kv_heads * c.passes * c.n_seqs <= (crowded ? 148 : 2 * 148)) return launch_groups<NT, Runs, 2>(key_map, value_map, c, stream);
+        if (static_cast<long long>(c.splits) * c.n_kv_heads * c.passes * c.n_seqs <= (crowded ? 1 : 2) * multiprocessors()) return launch_groups<NT, Runs, 2>(key_map, value_map, c, stream);
     }
     return launch_groups<NT, Runs, 1>(key_map, value_map, c, stream);
 }

@@ -485,7 +485,15 @@ TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, c
         !page_rows || page_stride <= 0 || span <= 0 || n_kv_heads <= 0 || first_head < 0 || first_head + n_kv_heads > page_heads || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || n_kv_heads > 65535)
         return cudaErrorInvalidValue;
-    const long long blocks = static_cast<long long>(n_kv_heads) * n_seqs * span, wanted = 148 * 8;      // one head to a block as long as all fit the machine at once
+    static int counts[64] = {};      // multiprocessors of each device, asked for once
+    int device = 0, sms = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return cudaErrorInvalidDevice;
+    if (device < 64) sms = counts[device];
+    if (!sms) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return cudaErrorInvalidDevice;
+        if (device < 64) counts[device] = sms;
+    }
+    const long long blocks = static_cast<long long>(n_kv_heads) * n_seqs * span, wanted = 8ll * sms;      // one head to a block as long as all fit the machine at once
     const int most = n_kv_heads < kReadHeads ? n_kv_heads : kReadHeads;
     const int heads = blocks <= wanted ? 1 : static_cast<int>(blocks / wanted < most ? blocks / wanted : most);
     const size_t before = static_cast<size_t>(first_head) * kPage * D;

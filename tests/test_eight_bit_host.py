@@ -368,3 +368,14 @@ def test_a_model_of_several_windows_takes_the_ranges_of_the_layer_that_wants_mos
     schedule = [replace(entry, cache_group=f"g{index}", cache_layer=0) for index, entry in enumerate(spec.schedule)]
     model = DecoderModel(replace(spec, blocks=tuple(blocks), schedule=tuple(schedule)), torch.bfloat16, "cpu")
     assert model.decode_splits(1, 5000, eight_bit=True) == kernels.decode8_splits(1, 5000, 1) > kernels.decode8_splits(1, 200, 1)
+
+
+@pytest.mark.parametrize("source", ["attention_decode8.cu", "eight_bit.cu", "gemm8_skinny.cu", "gemm8_tc.cu"])
+def test_rules_of_launches_ask_the_device_for_its_multiprocessors(source):
+    """No count of this machine stands in the code (comments say what was measured on it)."""
+    import os
+    import re
+
+    path = os.path.join(os.path.dirname(os.path.abspath(kernels.__file__)), source)
+    code = re.sub(r"//[^\n]*", "", open(path).read())
+    assert not re.search(r"\b148", code) and "MultiProcessorCount" in code
