@@ -230,7 +230,7 @@ gemm8_tc_kernel(const __grid_constant__ CUtensorMap input_map, const __grid_cons
             }
         }
     } else {
-        // ---- adders: a warp owns 32 tokens (those lanes of tensor memory that its number allows) and half of the features
+        // ---- adders: a warp owns 32 tokens (those lanes of tensor memory that its number allows) and 64 of the features
         const int quarter = warp & 3, part = (warp - 2) >> 2;
         uint32_t number = 0;
         bool alive = true;
