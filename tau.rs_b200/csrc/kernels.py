@@ -89,7 +89,7 @@ _CLASS_OF = {
     "side_gate": "activation", "unit_add_mix": "norm", "norm_rows": "norm", "relu_squared": "activation",
     "short_conv": "recurrence", "delta_prepare": "recurrence", "delta_rule": "recurrence", "selective_scan": "recurrence",
     "masked_prepare": "attention", "masked_attention": "attention", "talking_decode": "attention", "shared_key_decode": "attention", "gated_rows": "attention",
-    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gemm8_skinny": "product", "gemm8_stream": "product", "gemm8_tc": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
+    "quantize_blocks": "product", "quantize_rows": "product", "gemm8_simt": "product", "gemm8_skinny": "product", "gemm8_stream": "product", "gemm8_tc": "product", "linear8": "product", "gate_groups": "activation", "cache8_store": "attention", "attention_decode8": "attention", "cache8_read": "attention",
     "token_shift": "recurrence", "tanh": "activation", "channel_decay": "recurrence", "wkv": "recurrence", "forget_gates": "recurrence", "turn_heads": "recurrence",
 }
 _timing = None     # while timing: [last event, [(class, event after the launch), ...]]

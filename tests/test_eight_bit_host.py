@@ -379,3 +379,13 @@ def test_rules_of_launches_ask_the_device_for_its_multiprocessors(source):
     path = os.path.join(os.path.dirname(os.path.abspath(kernels.__file__)), source)
     code = re.sub(r"//[^\n]*", "", open(path).read())
     assert not re.search(r"\b148", code) and "MultiProcessorCount" in code
+
+
+def test_every_launch_is_booked_under_a_class():
+    """A traced run shows milliseconds by class: what is launched under a name without one would count as something else."""
+    import ast
+
+    with open(kernels.__file__) as handle:
+        tree = ast.parse(handle.read())
+    names = {call.args[1].value for call in ast.walk(tree) if isinstance(call, ast.Call) and getattr(call.func, "id", "") == "_check" and isinstance(call.args[1], ast.Constant)}
+    assert "linear8" in names and not names - set(kernels._CLASS_OF)
