@@ -7,7 +7,7 @@ which sequence and which position each row has.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -29,7 +29,8 @@ class CacheNeed:
     starts, whatever its length.  `keep_first` (beside a window): the first that many positions
     are read by every query and kept as long as the sequence lives.  `eight_bit` (kind "kv"): the
     mixer can also work on keys and values held in 8 bits with a scale for each page and head, if the
-    engine keeps its cache so.
+    engine keeps its cache so; layers that differ in nothing else may share a group, which is then held in 8 bits
+    only if all of them can.
     """
 
     kind: str
@@ -41,7 +42,7 @@ class CacheNeed:
     row_width: int = 0
     chunk: Optional[int] = None
     keep_first: int = 0
-    eight_bit: bool = False
+    eight_bit: bool = field(default=False, compare=False)
 
 
 class Pending(tuple):

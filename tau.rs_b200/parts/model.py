@@ -60,6 +60,8 @@ class DecoderModel:
             if known is not None and known[0] != need:
                 raise ValueError(f"cache group {entry.cache_group!r} is shared by layers with different needs")
             layers = max(known[1] if known else 0, entry.cache_layer + 1)
+            if known is not None and not known[0].eight_bit:      # the needs differ in this at most
+                need = known[0]
             groups[entry.cache_group] = (need, layers)
             key = (entry.cache_group, entry.cache_layer)
             if entry.writes_cache:

@@ -389,3 +389,27 @@ def test_every_launch_is_booked_under_a_class():
         tree = ast.parse(handle.read())
     names = {call.args[1].value for call in ast.walk(tree) if isinstance(call, ast.Call) and getattr(call.func, "id", "") == "_check" and isinstance(call.args[1], ast.Constant)}
     assert "linear8" in names and not names - set(kernels._CLASS_OF)
+
+
+@pytest.mark.parametrize("order", [(0, 1, 0), (1, 0, 1), (0, 0, 1)])
+def test_layers_of_two_kinds_share_a_cache_group(order):
+    """Attention can work on a cache in 8 bits and masked attention cannot; what they keep is the same: one group, held in the run's dtype."""
+    from dataclasses import replace
+
+    from tau_rs_b200 import DecoderModel, SequenceCache
+    from tau_rs_b200.config import MaskedAttentionSpec
+
+    spec = tiny_spec("B")
+    mixers = (replace(spec.blocks[0].mixer, n_heads=4, n_kv_heads=2, head_dim=64, qk_norm=None, position=None),
+              MaskedAttentionSpec(hidden=spec.hidden, n_heads=4, n_kv_heads=2, dim=64, value_dim=64, softmax_scale=0.125))
+    model = DecoderModel(replace(spec, blocks=tuple(replace(block, mixer=mixers[kind]) for block, kind in zip(spec.blocks, order))), torch.bfloat16, "cpu")
+    (need, layers), = model.cache_groups().values()
+    assert layers == 3 and not need.eight_bit
+    SequenceCache(model.cache_groups(), 256, 256, torch.bfloat16, "cpu")
+    with pytest.raises(ValueError, match="run's dtype"):
+        SequenceCache(model.cache_groups(), 256, 256, torch.bfloat16, "cpu", cache_format="fp8")
+    alone = DecoderModel(replace(spec, blocks=tuple(replace(block, mixer=mixers[0]) for block in spec.blocks)), torch.bfloat16, "cpu")
+    assert all(need.eight_bit for need, _ in alone.cache_groups().values())
+    narrow = replace(mixers[1], dim=32, value_dim=32)
+    with pytest.raises(ValueError, match="different needs"):
+        DecoderModel(replace(spec, blocks=tuple(replace(block, mixer=mixer) for block, mixer in zip(spec.blocks, (mixers[0], narrow, mixers[0])))), torch.bfloat16, "cpu")
