@@ -72,7 +72,7 @@ class Engine:
         if self.attention_block_size:
             bucket = 1 << max(0, (max_len - 1).bit_length())   # as the graphs are keyed: a power of two of positions
             return max(1, min(-(-bucket // self.attention_block_size), MAX_DECODE_SPLITS))
-        return self.model.decode_splits(n_seqs, max_len, eight_bit=bool(self.cache.cache_format))
+        return self.model.decode_splits(n_seqs, max_len, eight_bit=True) if self.cache.cache_format else self.model.decode_splits(n_seqs, max_len)
 
     def ring(self, ints: int) -> PinnedRing:
         """The pinned staging ring, grown if a step needs more room."""

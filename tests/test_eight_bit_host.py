@@ -413,3 +413,16 @@ def test_layers_of_two_kinds_share_a_cache_group(order):
     narrow = replace(mixers[1], dim=32, value_dim=32)
     with pytest.raises(ValueError, match="different needs"):
         DecoderModel(replace(spec, blocks=tuple(replace(block, mixer=mixer) for block, mixer in zip(spec.blocks, (mixers[0], narrow, mixers[0])))), torch.bfloat16, "cpu")
+
+
+def test_a_model_with_a_rule_of_its_own_for_ranges_serves_a_cache_in_16_bits():
+    """`decode_splits(n_seqs, max_len)` is what an engine asks of any model; only a cache in 8 bits asks for more."""
+    from tau_rs_b200 import DecoderModel, Engine
+
+    class Fixed(DecoderModel):
+        def decode_splits(self, n_seqs, max_len):
+            return 3
+
+    assert Engine(Fixed(tiny_spec("B"), torch.bfloat16, "cpu"), 256).decode_splits(2, 100) == 3
+    engine = Engine(DecoderModel(tiny_spec("B"), torch.bfloat16, "cpu"), 256, cache_format="fp8")
+    assert engine.decode_splits(1, 5000) == kernels.decode8_splits(1, 5000, 1)
