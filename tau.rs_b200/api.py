@@ -69,6 +69,7 @@ def load_model(folder: str, dtype: str = "auto", device="gpu", enforce_declared_
     With `enforce_declared_dtype` a bfloat16 run needs a folder that declares bfloat16, as
     the reference demands; without it any folder runs in either dtype.  `weights` "fp8" brings the weights of the
     attention and feed-forward products to 8 bits (e4m3, a scale for each 128 x 128) as they are loaded; a bfloat16 run only.
+    Those products then round their inputs to 8 bits as well (a scale for each row and 128 columns); sums stay in 32 bits.
     """
     raw = read_config_json(folder)
     metadata = metadata_from_json(raw)
@@ -143,7 +144,8 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new_tokens=None, tempe
     the folder's generation settings (16 if it has none) and `stop_tokens` to its
     `eos_token_id`.  `temperature == 0` is greedy.  Results keep the prompts' order.  `metrics` may bring a
     `GenerationMetrics` of the caller's (with a `sink` and a `log_interval_s`, say, to watch the decode rate while it runs).
-    `weights` (of a model folder) and `cache` "fp8" hold weights and cache in 8 bits, as in `load_engine`.
+    `weights` (of a model folder) and `cache` "fp8" hold weights and cache in 8 bits, as in `load_engine`; with `weights` the
+    products' activations are rounded to 8 bits too.
     """
     cache_format = _format("cache", cache)
     if not isinstance(model, str) and _format("weights", weights):

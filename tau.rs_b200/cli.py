@@ -40,7 +40,8 @@ def build_parser() -> argparse.ArgumentParser:
     execution.add_argument("--optimize-kernel", default="true", choices=["true", "false"],
                            help="Prefer optimized kernels. [default: true] false: the plain kernels that the others are checked against.")
     execution.add_argument("--weights", default="auto", choices=["auto", "fp8"],
-                           help="How the products' weights are held. [default: auto] auto: the run's dtype; fp8: 8 bits with a scale for each 128 x 128 (BF16 runs).")
+                           help="How the products' weights are held. [default: auto] auto: the run's dtype; fp8: 8 bits with a scale for each 128 x 128, "
+                                "and the products' activations rounded to 8 bits with a scale for each 128 of a row (BF16 runs).")
     execution.add_argument("--cache", default="auto", choices=["auto", "fp8"],
                            help="How cached keys and values are held. [default: auto] auto: the run's dtype; fp8: 8 bits with a scale for each 64 positions and head (BF16 runs).")
     execution.add_argument("--cuda-graph", default="full", choices=["none", "full"], help="CUDA graph policy for decode steps. [default: full]")

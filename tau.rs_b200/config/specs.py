@@ -488,7 +488,7 @@ class ModelSpec:
 
 def with_weight_format(spec: "ModelSpec", weight_format: str) -> "ModelSpec":
     """The same model with the weights of its attention and feed-forward products held in `weight_format` ("" as the run's dtype, or "fp8": e4m3 codes with a scale for each
-    128 x 128).  The embedding and the head stay as they are.  Refused where a layer has a mixer or a feed-forward whose products are not served in 8 bits."""
+    128 x 128; these products round their activations to e4m3 too, with a scale for each row and 128 columns).  The embedding and the head stay as they are.  Refused where a layer has a mixer or a feed-forward whose products are not served in 8 bits."""
     if not weight_format:
         return spec
     if weight_format != "fp8":

@@ -426,3 +426,13 @@ def test_a_model_with_a_rule_of_its_own_for_ranges_serves_a_cache_in_16_bits():
     assert Engine(Fixed(tiny_spec("B"), torch.bfloat16, "cpu"), 256).decode_splits(2, 100) == 3
     engine = Engine(DecoderModel(tiny_spec("B"), torch.bfloat16, "cpu"), 256, cache_format="fp8")
     assert engine.decode_splits(1, 5000) == kernels.decode8_splits(1, 5000, 1)
+
+
+def test_whoever_chooses_weights_in_8_bits_is_told_of_the_activations():
+    from tau_rs_b200 import api
+    from tau_rs_b200.cli import build_parser
+    from tau_rs_b200.config.specs import with_weight_format
+
+    help_text = " ".join(build_parser().format_help().split())
+    assert "products' activations rounded to 8 bits" in help_text
+    assert "round their inputs to 8 bits" in api.load_model.__doc__ and "activations" in api.generate.__doc__ and "activations" in with_weight_format.__doc__
