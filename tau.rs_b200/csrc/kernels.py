@@ -1215,7 +1215,8 @@ def _linear8(values, codes, scales, bias, out, gated: bool, limit: float) -> Non
 
 def linear8(values, codes, scales, bias, out) -> None:
     """`out = values @ weight.T + bias` with the weight in 8 bits (`quantize_blocks`) and the activations brought to 8 bits within the call, a scale for each
-    row and 128 columns; sums in 32 bits, one rounding to the output's type."""
+    row and 128 columns; sums in 32 bits, one rounding to the output's type.  Codes and scales are asked for while the kernel in front of this call may still run: `quantize_blocks`, copies and torch's
+    kernels are complete by then."""
     _check_linear8(values, codes, scales, bias, out, False)
     _linear8(values, codes, scales, bias, out, False, 0.0)
 
@@ -1365,7 +1366,7 @@ def _decode8(queries, key_pages, value_pages, key_scales, value_scales, out, ste
 def attention8_decode_fused(projected, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, write_cache: bool, q_weight, k_weight, eps: float, cos, sin, rotary_dim: int,
                             n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> bool:
     """Norm, rotation, the store (`cache8_store`, unless another run stored this step's keys and values) and attention in one kernel, where that exists: one token to a sequence and a group
-    of query heads that one block serves.  Returns False (and does nothing) otherwise."""
+    of query heads that one block serves.  Returns False (and does nothing) otherwise.  What `attention8` says of `seq_len` holds for the norm weights and the rotation tables too."""
     group = n_heads // n_kv_heads if n_kv_heads > 0 else 0
     if not (step.all_single and _prefer_optimized and group > 0 and _passes8(group, head_dim) == 1):
         return False
@@ -1442,7 +1443,10 @@ def _attention8_generic(queries, key_pages, value_pages, key_scales, value_scale
 
 
 def attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int) -> None:
-    """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim]."""
+    """`attention` over pages held in 8 bits (which hold the step's own keys already): bfloat16 queries [tokens, n_heads * head_dim].
+
+    The step's `seq_len` is read while the kernel in front of this call may still run.  Copies and torch's kernels are complete by then; a kernel of this library directly in front must not be what
+    writes it."""
     _check_attention8(queries, key_pages, value_pages, key_scales, value_scales, out, step, page_rows, n_heads, n_kv_heads, head_dim, window)
     if step.n_tokens == 0:
         return
