@@ -230,7 +230,6 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     // The range with the newest position: nobody else reads that page of that head.
     const bool stores = !Runs && prepare.projected != nullptr && prepare.store && count > 0 && page_hi == pages_end;
     float running_max[NT][2], running_sum[NT][2];      // log2 units; the sums and accumulators belong to weights exp2(score - max + 14)
-    int asked = 0;                     // producer: pages that copies have been asked for
     float unit[2] = {0.0f, 0.0f};      // producer: what one in a group's accumulators stands for, the greatest value scale of its pages so far
     float acc[NT][kValueRounds][8][4];
 #pragma unroll
@@ -249,6 +248,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         // ---- the pages, in order: the numbers and scales of 32 at a time, a lane each
         const int* pages = page_rows + static_cast<size_t>(seq) * page_stride;
         bool alive = true;
+        int asked = 0;
         for (int base = 0; base < count && alive; base += 32) {
             const bool mine = base + lane < count;
             const int place = mine ? pages[page_lo + base + lane] * n_kv_heads + kv_head : 0;
@@ -301,6 +301,8 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
         if (lane == 0) {
             shared->unit[0] = unit[0];
             shared->unit[1] = unit[1];
+            // Whoever gives up, this warp or one that adds: the copies in flight own their stages until they have landed.
+            for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
         }
     } else {
         if (!Runs && prepare.projected != nullptr && count > 0) {
@@ -595,12 +597,7 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
                 running_sum[n][h] += __shfl_xor_sync(0xffffffffu, running_sum[n][h], 16);
             }
     }
-    // The stages are done with.  (The flag is read once for all threads: another block of the cluster may raise it at any time.)
-    if (__syncthreads_or(*abort_flag)) {      // somebody gave up, the asking warp or one that adds, so copies may be in flight: they own their stages until they have landed
-        if (warp == kWarps && lane == 0)
-            for (int number = max(0, asked - kStages); number < asked; ++number) barrier_outlast(&shared->full[number % kStages], (number / kStages) & 1);
-        __syncthreads();
-    }
+    __syncthreads();      // the stages are done with
     grid_dependents_launch();      // only now: what starts beside this kernel takes room that its own later blocks, or clusters, wait for
     if (warp < kWarps) {
         const float one = shared->unit[Groups == 1 ? 0 : warp / kGroupWarps];
