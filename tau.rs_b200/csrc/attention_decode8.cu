@@ -688,10 +688,13 @@ decode8_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constan
     cluster_sync_all();      // nobody leaves while its results are read
 }
 
-// Joins the records of a sequence's ranges in their order: a block (of whole warps) to a head, a thread to a column.  A head of which a range failed is left as it was.
-__global__ void join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out, int n_heads, int splits) {
+// Joins the records of a sequence's ranges in their order: a block (of whole warps) to a head, a thread to a column.  A head of which a range failed is left as it was, and
+// so are rows behind the last run (`cu_seqlens`), of which there are no records.
+__global__ void join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, bf16* __restrict__ out, const int* __restrict__ cu_seqlens, int n_seqs, int n_heads,
+                            int splits) {
     grid_dependents_launch();
     grid_dependency_wait();
+    if (cu_seqlens && static_cast<int>(blockIdx.y) >= cu_seqlens[n_seqs]) return;
     __shared__ float factor[256];
     __shared__ float inverse;
     __shared__ bool failed;
@@ -798,7 +801,7 @@ int launch_groups(const CUtensorMap& key_map, const CUtensorMap& value_map, cons
         code = tau_launch_as(early, decode8_kernel<NT, Runs, Groups>, grid, dim3((kGroupWarps * Groups + 1) * 32), shared_bytes<Groups>(), stream, key_map, value_map, c.queries, c.out, c.key_pages, c.value_pages, c.key_scales, c.value_scales, c.partial_o,
                              c.partial_ml, c.seq_len, c.cu_seqlens, c.page_rows, c.page_stride, c.n_heads, c.n_kv_heads, c.passes, c.scale, c.window, c.splits, 0, longest_first, c.prepare);
     if (code == 0 && c.splits > kMostClustered)
-        code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? (D + 31) / 32 * 32 : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.n_heads, c.splits);
+        code = tau_launch(join_kernel, dim3(c.n_heads, c.n_tokens), dim3(D < 128 ? (D + 31) / 32 * 32 : 128), 0, stream, c.partial_o, c.partial_ml, c.out, c.cu_seqlens, c.n_seqs, c.n_heads, c.splits);
     return code ? code : tau_launch_status();
 }
 

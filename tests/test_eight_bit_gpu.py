@@ -577,3 +577,30 @@ def test_runs_whose_pages_are_read_back_a_few_heads_at_a_time(monkeypatch, heads
             most = most_asked_for(lambda: kernels.attention8(queries, *cache.pages, out, step, cache.rows, heads, kv_heads, dim, dim ** -0.5, window))
             assert most <= room + 2 * queries.numel() * 2 + 4096      # queries and results of those heads, and the table of the pages' places
         assert torch.equal(out, wanted)
+
+
+@pytest.mark.parametrize("directly", [0, 1])
+@pytest.mark.parametrize("longest", [600, 9000])
+def test_rows_behind_the_last_run_stay_as_they_were(monkeypatch, directly, longest):
+    """More rows than the runs have tokens: keys, values, queries and results behind the last run are neither read nor written, by a few ranges of a sequence or by many."""
+    monkeypatch.setattr(kernels, "runs8_like_single_tokens", lambda *sizes: bool(directly))
+    runs, counts = [(longest - 3, 3), (40, 2)], [-(-longest // 64), 1]
+    cache, padded = Cache(sum(counts), 2, 64, counts), Cache(sum(counts), 2, 64, counts)
+    keys, values = random_rows(longest + 42, 2, 64, 3)
+    queries = torch.randn(9, 4 * 64, device="cuda").to(torch.bfloat16)
+    new = torch.cat([torch.arange(longest - 3, longest), torch.arange(longest + 40, longest + 42)])
+    results = []
+    for each, rows in ((cache, 5), (padded, 9)):
+        kernels.cache8_store(torch.cat([keys[: longest - 3], keys[longest : longest + 40]]).cuda(), torch.cat([values[: longest - 3], values[longest : longest + 40]]).cuda(), *each.pages,
+                             make_step([(0, longest - 3), (0, 40)]), each.rows)
+        step = make_step(runs)
+        step.n_tokens = rows
+        more = [torch.cat([each_[new], torch.full((rows - 5, 2, 64), float("nan"), dtype=torch.bfloat16)]).cuda() for each_ in (keys, values)]
+        kernels.cache8_store(*more, *each.pages, step, each.rows)
+        out = torch.full((rows, 4 * 64), 7.0, device="cuda", dtype=torch.bfloat16)
+        kernels.attention8(queries[:rows], *each.pages, out, step, each.rows, 4, 2, 64, 0.125, 0)
+        results.append(out)
+    assert directly == 0 or (kernels.decode8_splits(2, longest, 2) > 8) == (longest == 9000)
+    assert torch.equal(results[1][:5], results[0]) and bool((results[1][5:] == 7.0).all())
+    for found, wanted in zip(padded.pages, cache.pages):
+        assert torch.equal(found.view(torch.uint8), wanted.view(torch.uint8))
