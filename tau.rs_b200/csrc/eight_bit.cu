@@ -328,6 +328,7 @@ __device__ __forceinline__ unsigned nan_codes(unsigned word) { return __vcmpeq4(
 // too), and positions that none sees are zeros: what a window left behind may be NaN, and a weight of
 // zero would not hide that.  Bound by memory: a page's heads lie one behind the other, so where there are pages enough a block takes several and pays for its page's number and
 // scale once (64 sequences of up to 200 positions, 8 heads of 128: 14 us for 17 MB of codes read and 34 MB of values written).
+template <bool Windowed>
 __global__ void __launch_bounds__(256)
 read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ value_pages, const float* __restrict__ key_scales, const float* __restrict__ value_scales,
             bf16* __restrict__ keys, bf16* __restrict__ values, int* __restrict__ places, const int* __restrict__ seq_start, const int* __restrict__ seq_len, const int* __restrict__ page_rows,
@@ -336,9 +337,13 @@ read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ v
     grid_dependents_launch();
     grid_dependency_wait();
     const int seq = blockIdx.y, head0 = blockIdx.z * heads, here = min(heads, n_kv_heads - head0);
-    const int first_seen = sparse && window > 0 ? max(0, seq_start[seq] + 1 - window) : 0, first_page = first_seen / kPage, page = first_page + blockIdx.x;
-    if (places != nullptr && blockIdx.x == 0 && blockIdx.z == 0)
-        for (int p = threadIdx.x; p < page_stride; p += 256) places[static_cast<size_t>(seq) * page_stride + p] = seq * span + min(max(p - first_page, 0), span - 1);
+    const int first_seen = Windowed ? max(0, seq_start[seq] + 1 - window) : 0, first_page = first_seen / kPage, page = first_page + blockIdx.x;
+    if constexpr (Windowed) {
+        if (blockIdx.x == 0 && blockIdx.z == 0)
+            for (int p = threadIdx.x; p < page_stride; p += 256) places[static_cast<size_t>(seq) * page_stride + p] = seq * span + min(max(p - first_page, 0), span - 1);
+    } else {
+        if (places != nullptr && blockIdx.z == 0 && threadIdx.x == 0) places[static_cast<size_t>(seq) * page_stride + page] = seq * span + page;
+    }
     const int live = min(kPage, seq_len[seq] - page * kPage);      // positions that the sequence has in this page
     const int first = max(0, first_seen - page * kPage);      // the first position of this page that a query sees
     if (sparse && live <= 0) return;
@@ -346,7 +351,7 @@ read_kernel(const uint8_t* __restrict__ key_pages, const uint8_t* __restrict__ v
     const int per_head = kPage * D / 16, begin = first * D / 16, end = live * D / 16;      // pieces of 16 elements
     // For attention (`sparse`), where some queries see a position and others do not: a value that is not finite would reach those that do not, through a weight of zero.  It becomes zero
     // and its position's key NaN, which a mask does hide.
-    const bool guarded = sparse && ((page + 1) * kPage > seq_start[seq] || window > 0);
+    const bool guarded = sparse && (Windowed || (page + 1) * kPage > seq_start[seq]);
     if (guarded) {
         for (int index = threadIdx.x; index < here * kPage; index += 256) odd[index] = 0;
         __syncthreads();
@@ -482,7 +487,7 @@ TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, c
                                const int* seq_len, const int* page_rows, int page_stride, int span, int n_seqs, int page_heads, int first_head, int n_kv_heads, int D, int window, int sparse, void* stream) {
     if (n_seqs <= 0) return 0;
     if (!key_pages || !value_pages || ((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) & 15) || !key_scales || !value_scales || !keys || !values || !seq_start || !seq_len ||
-        !page_rows || page_stride <= 0 || span <= 0 || n_kv_heads <= 0 || first_head < 0 || first_head + n_kv_heads > page_heads || D < 16 || D > 256 ||
+        !page_rows || page_stride <= 0 || span <= 0 || (sparse ? !places : span != page_stride) || (window <= 0 && span != page_stride) || n_kv_heads <= 0 || first_head < 0 || first_head + n_kv_heads > page_heads || D < 16 || D > 256 ||
         (D & 15) || n_seqs > 65535 || n_kv_heads > 65535)
         return cudaErrorInvalidValue;
     static int counts[64] = {};      // multiprocessors of each device, asked for once
@@ -497,9 +502,12 @@ TAU_EXPORT int tau_cache8_read(const void* key_pages, const void* value_pages, c
     const int most = n_kv_heads < kReadHeads ? n_kv_heads : kReadHeads;
     const int heads = blocks <= wanted ? 1 : static_cast<int>(blocks / wanted < most ? blocks / wanted : most);
     const size_t before = static_cast<size_t>(first_head) * kPage * D;
-    tau_launch(read_kernel, dim3(span, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages) + before,
-               static_cast<const uint8_t*>(value_pages) + before, key_scales + first_head, value_scales + first_head, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len,
-               page_rows, page_stride, span, page_heads, n_kv_heads, heads, D,
-               window, sparse);
+    auto run = [&](auto kernel) {
+        tau_launch(kernel, dim3(span, n_seqs, (n_kv_heads + heads - 1) / heads), dim3(256), 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(key_pages) + before,
+                   static_cast<const uint8_t*>(value_pages) + before, key_scales + first_head, value_scales + first_head, static_cast<bf16*>(keys), static_cast<bf16*>(values), places, seq_start, seq_len,
+                   page_rows, page_stride, span, page_heads, n_kv_heads, heads, D, window, sparse);
+    };
+    if (sparse && window > 0) run(read_kernel<true>);
+    else run(read_kernel<false>);
     return tau_launch_status();
 }
