@@ -1169,6 +1169,7 @@ def _stream8(values, codes, scales, bias, out, gated: bool, gate_limit: float) -
 
 def gemm8_stream(values, codes, scales, bias, out, gated: bool = False, gate_limit: float = 0.0) -> None:
     """The product of at most 8 bfloat16 rows: a block to an SM, which quantises the rows once and streams its share of the weight's codes."""
+    _two(values, codes)
     _require(values.dtype == torch.bfloat16 and values.shape[0] <= STREAM8_MAX_ROWS and codes.shape[1] <= STREAM8_MAX_DEPTH,
              f"the streaming product takes at most {STREAM8_MAX_ROWS} bfloat16 rows of at most {STREAM8_MAX_DEPTH} columns")
     _check_linear8(values, codes, scales, bias, out, gated)

@@ -436,3 +436,12 @@ def test_whoever_chooses_weights_in_8_bits_is_told_of_the_activations():
     help_text = " ".join(build_parser().format_help().split())
     assert "products' activations rounded to 8 bits" in help_text
     assert "round their inputs to 8 bits" in api.load_model.__doc__ and "activations" in api.generate.__doc__ and "activations" in with_weight_format.__doc__
+
+
+@pytest.mark.parametrize("product, first", [(kernels.gemm8_stream, ()), (kernels.gemm8_tc, (torch.ones(1, 3),)), (kernels.linear8, ())])
+def test_products_refuse_operands_of_one_dimension(product, first):
+    operands = product_operands()
+    values = operands["values"] if not first else torch.zeros(3, 32, dtype=torch.uint8).view(CODES)
+    for wrong in ((values[0], operands["codes"]), (values, operands["codes"][0])):
+        with pytest.raises(kernels.KernelError, match="shapes"):
+            product(wrong[0], *first, wrong[1], operands["scales"], None, operands["out"])
